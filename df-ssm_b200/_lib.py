@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int8, c_int32, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int8, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libdfssm.so")
 
@@ -54,6 +54,14 @@ SIGNATURES = {
     "dfssm_ssm_step": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "dfssm_rmsnorm_quantize": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dfssm_gated_delta_step": (c_int, [c_void_p, c_int] * 5 + [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                       c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    "dfssm_gated_delta_workspace": (c_size_t, [c_int] * 7),
+    "dfssm_gated_delta_prefill": (c_int, [c_void_p, c_int] * 5 + [c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                          c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
+                                          c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "dfssm_sample_filtered": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "dfssm_lm_head_workspace": (c_size_t, [c_int]),
     "dfssm_lm_head_argmax": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                      c_void_p, c_void_p]),

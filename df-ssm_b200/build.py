@@ -13,7 +13,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libdfssm.so")
-SOURCES = ["dfssm_capi.cu", "persistent.cu"]
+SOURCES = ["dfssm_capi.cu", "persistent.cu", "gated_delta.cu", "sample_filtered.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -247,6 +247,65 @@ int dfssm_sample(const float* logits, int batch, int vocab, uint32_t* seen_bits,
  * The returned logits stay the raw fp32 logits. */
 int dfssm_set_sampling(dfssm_engine* e, float temperature, float top_p, float rep_penalty, uint64_t seed);
 
+/* ---- gated delta rule and filtered sampling (no counterpart in the reference) ---- */
+
+typedef enum dfssm_dtype { DFSSM_F16 = 0, DFSSM_BF16 = 1, DFSSM_F32 = 2 } dfssm_dtype;
+
+/* One token of `batch` sequences through the gated delta rule, the state update next to dfssm_ssm_step
+ * whose state is also corrected along the key: for every value head
+ *   g = -exp(A_log) softplus(a + dt_bias),  beta = sigmoid(b),
+ *   S <- e^g S + beta (v - e^g S k) k^T,    o = scale * S q.
+ * With qk_norm, q and k are first scaled to unit length, x / sqrt(|x|^2 + 1e-6).  Row i of each array is
+ * sequence i: q, k [batch][k_heads][dk] (row strides ld_q, ld_k in elements), v, o [batch][v_heads][dv]
+ * (ld_v, ld_o), a, b [batch][v_heads] (ld_a, ld_b), all of `dtype` (DFSSM_F16 or DFSSM_BF16); A_log,
+ * dt_bias fp32 [v_heads].  Value head h takes key head h / (v_heads / k_heads).  state fp32
+ * [n_slots][v_heads][dv][dk], updated in place (dfssm_ssm_step's layout: headdim = dv, d_state = dk);
+ * slots int32 [batch] (device) names each sequence's slot, NULL = slot i for sequence i.  A sequence whose
+ * slot is outside [0, n_slots), or is also the slot of an earlier sequence of the call, takes no part:
+ * its state and its row of o are left as they were.  o must not overlap the inputs.  dk 64 or 128; dv a
+ * multiple of 16 up to 256; q, k, v, o and state 16-byte aligned, ld_q, ld_k, ld_v, ld_o multiples of 8. */
+int dfssm_gated_delta_step(const void* q, int ld_q, const void* k, int ld_k, const void* v, int ld_v, const void* a,
+                           int ld_a, const void* b, int ld_b, const float* A_log, const float* dt_bias, float* state,
+                           int n_slots, const int32_t* slots, int batch, void* o, int ld_o, int k_heads, int v_heads,
+                           int dk, int dv, float scale, int qk_norm, int dtype, void* stream);
+
+/* Scratch bytes dfssm_gated_delta_prefill needs (it may be 0). */
+size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dv, int dtype);
+/* The same recurrence over ragged prompts: sequence i owns the token rows [cu_seqlens[i],
+ * cu_seqlens[i + 1]) of q, k, v, a, b and o (`tokens` rows in all), starts from the state in its slot and
+ * leaves its final state there; dfssm_gated_delta_step continues from it.  cu_seqlens int32 [n_seq + 1]
+ * (device, non-decreasing; offsets are clamped to [0, tokens], so no other row is read).  A sequence of no
+ * tokens changes nothing; rows of o outside every sequence are left as they were.  `workspace` is device
+ * memory of dfssm_gated_delta_workspace bytes, 256-byte aligned, used by this call alone until it has run:
+ * calls that may overlap (other streams, graphs replayed at once) need one each.  Neither call allocates or
+ * synchronises, and both can be captured into a graph. */
+int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, const void* v, int ld_v, const void* a,
+                              int ld_a, const void* b, int ld_b, const float* A_log, const float* dt_bias,
+                              float* state, int n_slots, const int32_t* slots, const int32_t* cu_seqlens, int n_seq,
+                              int tokens, void* o, int ld_o, int k_heads, int v_heads, int dk, int dv, float scale,
+                              int qk_norm, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Token choice with filters and given random numbers, next to dfssm_sample: every row has its own
+ * settings, and the draw uses uniform[b] instead of a counter.  logits [batch][vocab] of `dtype` (fp32,
+ * fp16 or bf16; row stride ld in elements).  Per row, with the tokens ordered by falling
+ * x = fp32(l / temperature) (divided by rep_penalty where the row's bit of seen_bits is set), the lower
+ * index first among equal ones, and w = exp(x - max x):
+ *   top-k  the first top_k tokens stay (top_k <= 0: all);
+ *   top-p  of these, a token stays while the weight before it is <= top_p of their sum (>= 1: all);
+ *   min-p  of these, the first one and those with w >= min_p stay;
+ *   next   the first kept token in vocabulary order whose running weight exceeds uniform[b] x the kept
+ *          weight (uniform is taken into [0, 1)).
+ * temperature <= 0 takes the first token of the order.  NaN and -inf logits never stay; a row that holds
+ * nothing else gets next = -1, kept_count 0 and prob 0.  temperature, top_p, min_p fp32 [batch] and top_k
+ * int32 [batch] (device) may each be NULL: 1, all, 0, all.  seen_bits as in dfssm_sample, or NULL.
+ * Outputs: next int32 [batch]; kept_count int32 [batch] and prob fp32 [batch] (the token's share of the kept
+ * weight), either may be NULL.  Weights are summed as 64-bit integers, so the choice does not depend on the
+ * order of any sum.  vocab up to 2^24. */
+int dfssm_sample_filtered(const void* logits, int64_t ld, int dtype, int batch, int vocab, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p, const uint32_t* seen_bits,
+                          float rep_penalty, const float* uniform, int32_t* next, int32_t* kept_count, float* prob,
+                          void* stream);
+
 /* Self-test (no counterpart in the reference): checks, on device `device`, the kernels'
  * two-FMA division (common.cuh div_rn_rcp, used by the activation quantiser) against IEEE fp32
  * division for every pair of finite fp16 operands with a positive divisor.  Writes the number
