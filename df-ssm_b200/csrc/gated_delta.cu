@@ -1,7 +1,8 @@
 // Gated delta rule ops: the token-loop kernel (one token per sequence, short sequences) and the C ABI.
-#include "gated_delta.cuh"
+#include "gated_delta_chunk.cuh"
 
 #include <cmath>
+#include <cstdlib>
 
 #include "op_host.h"
 
@@ -147,6 +148,45 @@ int launch_loop(const GatedDeltaArgs& p, int dk, int dtype, cudaStream_t s) {
   return DFSSM_OK;
 }
 
+size_t gd_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dtype) {
+  const size_t n = (size_t)gd_chunk_slots(tokens, n_seq);
+  return n * v_heads * kGdBlock + (dtype == DFSSM_BF16 ? n * k_heads * 2 * kGdC * dk * 2 : 0);
+}
+
+template <typename T, int DK, int W>
+int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16, int slots_total, cudaStream_t s) {
+  static SmemLimit limit;
+  constexpr int bytes = gd_chunk_smem<DK, W>();
+  const auto fn = gated_delta_chunk_kernel<T, DK, W>;
+  DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
+  const int parts = (p.dv + 16 * W - 1) / (16 * W);
+  const long long grid = (long long)p.n_seq * p.v_heads * parts;
+  if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
+  fn<<<(unsigned)grid, 32 * W, bytes, s>>>(p, blocks, kq16, parts, slots_total);
+  DFSSM_CU(cudaGetLastError());
+  return DFSSM_OK;
+}
+
+template <typename T, int DK>
+int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
+  static SmemLimit limit;
+  constexpr int bytes = gd_prep_smem<DK>();
+  const long long n = gd_chunk_slots(p.tokens, p.n_seq), grid = n * p.v_heads;
+  if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
+  __half* kq16 = std::is_same<T, __half>::value ? nullptr
+                                               : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
+  const auto fn = gated_delta_prep_kernel<T, DK>;
+  DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
+  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16);
+  DFSSM_CU(cudaGetLastError());
+  static const int force = getenv("DFSSM_GD_W") ? atoi(getenv("DFSSM_GD_W")) : 0;
+  switch (force ? force : 4) {
+    case 8: return launch_walk<T, DK, 8>(p, workspace, kq16, (int)n, s);
+    case 4: return launch_walk<T, DK, 4>(p, workspace, kq16, (int)n, s);
+    default: return launch_walk<T, DK, 2>(p, workspace, kq16, (int)n, s);
+  }
+}
+
 // What both entry points ask of their arguments.
 int check_args(const GatedDeltaArgs& p, int dk, int dtype) {
   // arrays without rows have no address
@@ -191,8 +231,9 @@ int dfssm_gated_delta_step(const void* q, int ld_q, const void* k, int ld_k, con
 }
 
 size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dv, int dtype) {
-  (void)tokens, (void)n_seq, (void)k_heads, (void)v_heads, (void)dk, (void)dv, (void)dtype;
-  return 0;
+  (void)dv;
+  if (tokens < 1 || n_seq < 1 || k_heads < 1 || v_heads < 1 || dk < 1) return 0;
+  return gd_workspace(tokens, n_seq, k_heads, v_heads, dk, dtype);
 }
 
 int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, const void* v, int ld_v, const void* a,
@@ -208,7 +249,12 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
   if (need && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need))
     return dfssm_fail(DFSSM_ERR_ARG, "the workspace must be %zu bytes, 256-byte aligned", need);
   if (n_seq == 0 || tokens == 0) return DFSSM_OK;
-  return launch_loop(p, dk, dtype, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  static const int loop = getenv("DFSSM_GD_LOOP") ? atoi(getenv("DFSSM_GD_LOOP")) : 4;
+  if (tokens <= (long long)loop * n_seq) return launch_loop(p, dk, dtype, s);
+  char* w = static_cast<char*>(workspace);
+  if (dtype == DFSSM_F16) return dk == 128 ? launch_chunked<__half, 128>(p, w, s) : launch_chunked<__half, 64>(p, w, s);
+  return dk == 128 ? launch_chunked<__nv_bfloat16, 128>(p, w, s) : launch_chunked<__nv_bfloat16, 64>(p, w, s);
 }
 
 }  // extern "C"

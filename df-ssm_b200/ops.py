@@ -17,36 +17,53 @@ from . import _lib
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _need(ok, what: str):
-    if not ok:
-        raise ValueError(what)
+# The checks run before every launch, which a one-token op waits for: messages are only put together on failure.
+
+
+def _refuse(t, name: str, what: str, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device (there is no CPU fallback)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+    raise ValueError(f"{name} must be {what}, not {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
 
 
 def _on(t, name: str, device=None):
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(t.is_cuda, f"{name} must be on a CUDA device (there is no CPU fallback)")
-    _need(device is None or t.device == device, f"{name} is on {t.device}, not {device}")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or (device is not None and t.device != device):
+        _refuse(t, name, "a tensor", device)
 
 
 def _vector(t, name: str, n: int, dtype, device):
-    _on(t, name, device)
-    _need(t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1),
-          f"{name} must be a contiguous {dtype} tensor of {n} elements")
+    """Pointer of a contiguous [n]."""
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != (n,)
+            or (n > 1 and t.stride(0) != 1)):
+        _refuse(t, name, f"a contiguous {dtype} vector of {n}", device)
     return t.data_ptr()
 
 
-def _rows(t, name: str, n: int, inner, dtype, device):
-    """Pointer and row stride of [n, *inner] whose rows are contiguous."""
-    _on(t, name, device)
-    _need(t.dtype == dtype and tuple(t.shape) == (n, *inner),
-          f"{name} must be a {dtype} tensor of shape {(n, *inner)}, not {t.dtype} {tuple(t.shape)}")
-    width = 1
-    for d, s in zip(reversed(inner), reversed(t.stride()[1:])):
-        _need(d == 1 or s == width, f"{name} must be contiguous within a row")
-        width *= d
-    ld = t.stride(0) if n > 1 else width
-    _need(width <= ld < 2**31, f"{name}: row stride {ld} of rows of {width}")
-    return t.data_ptr(), ld
+def _heads(t, name: str, shape, dtype, device):
+    """Pointer and row stride of [rows, heads, width] whose rows are contiguous."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape:
+        n, h, d = shape
+        ld, sh, sd = t.stride()
+        if n < 2:
+            ld = h * d
+        if sd == 1 and (sh == d or h == 1) and h * d <= ld < 2**31:
+            return t.data_ptr(), ld
+    _refuse(t, name, f"{dtype} {tuple(shape)} with contiguous rows", device)
+
+
+def _gates(t, name: str, shape, dtype, device):
+    """Pointer and row stride of [rows, heads] whose rows are contiguous."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape:
+        ld, sh = t.stride()
+        if shape[0] < 2:
+            ld = shape[1]
+        if (sh == 1 or shape[1] == 1) and shape[1] <= ld < 2**31:
+            return t.data_ptr(), ld
+    _refuse(t, name, f"{dtype} {tuple(shape)} with contiguous rows", device)
 
 
 def _call(device, fn, *args):
@@ -61,25 +78,24 @@ def _call(device, fn, *args):
 def _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale):
     _on(q, "q")
     dev, dtype = q.device, q.dtype
-    _need(dtype in (torch.float16, torch.bfloat16), f"q must be fp16 or bf16, not {dtype}")
-    _need(q.dim() == 3 and isinstance(v, torch.Tensor) and v.dim() == 3, "q and v must be [tokens, heads, width]")
-    n, hk, dk = q.shape
-    hv, dv = v.shape[1], v.shape[2]
-    _on(state, "state", dev)
-    _need(state.dtype == torch.float32 and state.dim() == 4 and tuple(state.shape[1:]) == (hv, dv, dk) and
-          state.is_contiguous(), f"state must be contiguous fp32 [slots, {hv}, {dv}, {dk}]")
-    qp = _rows(q, "q", n, (hk, dk), dtype, dev)
-    kp = _rows(k, "k", n, (hk, dk), dtype, dev)
-    vp = _rows(v, "v", n, (hv, dv), dtype, dev)
-    ap = _rows(a, "a", n, (hv,), dtype, dev)
-    bp = _rows(b, "b", n, (hv,), dtype, dev)
+    if dtype not in (torch.float16, torch.bfloat16) or q.dim() != 3:
+        _refuse(q, "q", "fp16 or bf16 [tokens, k_heads, dk]")
+    if not isinstance(v, torch.Tensor) or v.dim() != 3:
+        _refuse(v, "v", "[tokens, v_heads, dv]")
+    keys, values = q.shape, v.shape
+    n, hk, dk = keys
+    hv, dv = values[1:]
+    values = (n, hv, dv)
+    if (not isinstance(state, torch.Tensor) or state.dtype is not torch.float32 or state.device != dev or state.dim() != 4
+            or state.shape[1:] != (hv, dv, dk) or not state.is_contiguous()):
+        _refuse(state, "state", f"contiguous fp32 [slots, {hv}, {dv}, {dk}]", dev)
     if out is None:
-        out = torch.empty(n, hv, dv, dtype=dtype, device=dev)
-    op = _rows(out, "out", n, (hv, dv), dtype, dev)
-    al, db = _vector(A_log, "A_log", hv, torch.float32, dev), _vector(dt_bias, "dt_bias", hv, torch.float32, dev)
-    sl = None if slots is None else _vector(slots, "slots", n_seq, torch.int32, dev)
-    head = (*qp, *kp, *vp, *ap, *bp, al, db, state.data_ptr(), state.shape[0], sl)
-    tail = (*op, hk, hv, dk, dv, dk ** -0.5 if scale is None else float(scale))
+        out = torch.empty(values, dtype=dtype, device=dev)
+    head = (*_heads(q, "q", keys, dtype, dev), *_heads(k, "k", keys, dtype, dev), *_heads(v, "v", values, dtype, dev),
+            *_gates(a, "a", (n, hv), dtype, dev), *_gates(b, "b", (n, hv), dtype, dev),
+            _vector(A_log, "A_log", hv, torch.float32, dev), _vector(dt_bias, "dt_bias", hv, torch.float32, dev),
+            state.data_ptr(), state.shape[0], None if slots is None else _vector(slots, "slots", n_seq, torch.int32, dev))
+    tail = (*_heads(out, "out", values, dtype, dev), hk, hv, dk, dv, dk ** -0.5 if scale is None else float(scale))
     return dev, head, tail, out, (n, hk, hv, dk, dv, _DTYPES[dtype])
 
 
@@ -112,8 +128,8 @@ def gated_delta_prefill(q, k, v, a, b, A_log, dt_bias, state, cu_seqlens, *, slo
     one; else it comes from torch's allocator for the length of the call.  Rows of a new o that no sequence
     owns are undefined."""
     _on(q, "q")
-    _need(isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1,
-          "cu_seqlens must hold one offset more than there are sequences")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        _refuse(cu_seqlens, "cu_seqlens", "int32 [sequences + 1]")
     n_seq = cu_seqlens.shape[0] - 1
     cu = _vector(cu_seqlens, "cu_seqlens", n_seq + 1, torch.int32, q.device)
     dev, head, tail, out, dims = _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale)
@@ -121,9 +137,9 @@ def gated_delta_prefill(q, k, v, a, b, A_log, dt_bias, state, cu_seqlens, *, slo
     need = lib.dfssm_gated_delta_workspace(dims[0], n_seq, *dims[1:])
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _on(workspace, "workspace", dev)
-    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need,
-          f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    elif (not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.device != dev
+          or not workspace.is_contiguous() or workspace.numel() < need):
+        _refuse(workspace, "workspace", f"contiguous uint8 of at least {need} bytes", dev)
     _call(dev, lib.dfssm_gated_delta_prefill, *head, cu, n_seq, dims[0], *tail, int(bool(qk_norm)), dims[-1],
           workspace.data_ptr(), workspace.numel())
     return out
@@ -149,21 +165,24 @@ def sample_filtered(logits, uniform, *, temperature=None, top_k=None, top_p=None
     prob fp32 [B]): the token, how many tokens the filters kept, and the token's share of their weight;
     -1, 0, 0 for a row without a finite logit.  `out`: that triple to write into."""
     _on(logits, "logits")
-    _need(logits.dtype in _DTYPES and logits.dim() == 2 and logits.shape[1] > 0, "logits must be [rows, vocab] in fp32, fp16 or bf16")
+    if logits.dtype not in _DTYPES or logits.dim() != 2 or logits.shape[1] < 1:
+        _refuse(logits, "logits", "[rows, vocab] in fp32, fp16 or bf16")
     dev = logits.device
     B, V = logits.shape
-    _need(V == 1 or logits.stride(1) == 1, "logits must be contiguous within a row")
-    ld = logits.stride(0) if B > 1 else V
-    _need(ld >= V, "the rows of logits overlap")
+    ld, step = logits.stride()
+    if B < 2:
+        ld = V
+    if (V > 1 and step != 1) or ld < V:
+        _refuse(logits, "logits", "contiguous within a row, rows apart")
     u = _vector(uniform, "uniform", B, torch.float32, dev)
     temperature = _per_row(temperature, "temperature", B, torch.float32, dev)
     top_k = _per_row(top_k, "top_k", B, torch.int32, dev)
     top_p = _per_row(top_p, "top_p", B, torch.float32, dev)
     min_p = _per_row(min_p, "min_p", B, torch.float32, dev)
     if seen_bits is not None:
-        _on(seen_bits, "seen_bits", dev)
-        _need(seen_bits.dtype == torch.int32 and tuple(seen_bits.shape) == (B, (V + 31) // 32) and seen_bits.is_contiguous(),
-              f"seen_bits must be contiguous int32 [{B}, {(V + 31) // 32}]")
+        if (not isinstance(seen_bits, torch.Tensor) or seen_bits.dtype is not torch.int32 or seen_bits.device != dev
+                or seen_bits.shape != (B, (V + 31) // 32) or not seen_bits.is_contiguous()):
+            _refuse(seen_bits, "seen_bits", f"contiguous int32 [{B}, {(V + 31) // 32}]", dev)
     if out is None:
         out = (torch.empty(B, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev),
                torch.empty(B, dtype=torch.float32, device=dev))
