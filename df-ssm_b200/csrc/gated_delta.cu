@@ -162,7 +162,7 @@ int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16,
   const int parts = (p.dv + 16 * W - 1) / (16 * W);
   const long long grid = (long long)p.n_seq * p.v_heads * parts;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
-  fn<<<(unsigned)grid, 32 * W, bytes, s>>>(p, blocks, kq16, parts, slots_total);
+  fn<<<(unsigned)grid, 64 * W, bytes, s>>>(p, blocks, kq16, parts, slots_total);
   DFSSM_CU(cudaGetLastError());
   return DFSSM_OK;
 }
@@ -171,17 +171,23 @@ template <typename T, int DK>
 int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   static SmemLimit limit;
   constexpr int bytes = gd_prep_smem<DK>();
-  const long long n = gd_chunk_slots(p.tokens, p.n_seq), grid = n * p.v_heads;
+  const long long n = gd_chunk_slots(p.tokens, p.n_seq);
+  const int rep = p.v_heads / p.k_heads;
+  static const int pg = getenv("DFSSM_GD_PG") ? atoi(getenv("DFSSM_GD_PG")) : 0;
+  int per_group = pg ? pg : 4;
+  if (per_group > rep) per_group = rep;
+  while (per_group > 1 && n * p.k_heads * ((rep + per_group - 1) / per_group) < 600) per_group /= 2;
+  const int groups = (rep + per_group - 1) / per_group;
+  const long long grid = n * p.k_heads * groups;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
   const auto fn = gated_delta_prep_kernel<T, DK>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16);
+  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, groups, per_group);
   DFSSM_CU(cudaGetLastError());
   static const int force = getenv("DFSSM_GD_W") ? atoi(getenv("DFSSM_GD_W")) : 0;
   switch (force ? force : 4) {
-    case 8: return launch_walk<T, DK, 8>(p, workspace, kq16, (int)n, s);
     case 4: return launch_walk<T, DK, 4>(p, workspace, kq16, (int)n, s);
     default: return launch_walk<T, DK, 2>(p, workspace, kq16, (int)n, s);
   }

@@ -64,6 +64,12 @@ __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
+// m16n8k16 fp16 MMA that the compiler may schedule among the others
+__device__ __forceinline__ void mma_acc(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void ldsm4(unsigned (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -92,32 +98,119 @@ __device__ __forceinline__ uint32_t kq_off(int t, int u) {
 }
 
 // ------------------------------------------------------------------ T, P and the factors of every chunk
+//
+// One block per chunk, key head and group of the value heads that share it: k.k^T and q.k^T are taken once
+// (mma.sync, kept in registers) and serve every head of the group, whose gates differ.  The decay between
+// tokens of different 16-token blocks is a product of two factors that meet at the block boundary before t,
+// each at most 1, so only the diagonal blocks take an exponential per element.  T is inverted blockwise: the
+// 16 x 16 diagonal blocks by forward substitution in fp32, then the corners -T22 (L21 T11) of 32 and of 64 with
+// TF32 MMAs on split operands.
 
 constexpr int kPrepThreads = 128;
 constexpr int kLS = 68;  // row stride of the fp32 matrices in shared memory
 
 template <int DK>
-__host__ __device__ constexpr int gd_prep_smem() { return 2 * kGdC * DK * 2 + 2 * kGdC * kLS * 4 + 1024 * 5 + 64 * 8; }
+__host__ __device__ constexpr int gd_prep_tiles() {  // K and Q; once they are multiplied, T [64][kLS]
+  return 2 * kGdC * DK * 2 > kGdC * kLS * 4 ? 2 * kGdC * DK * 2 : kGdC * kLS * 4;
+}
+template <int DK>
+__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 8; }
 
-// One block per chunk number and value head.  kq16: for bf16 inputs, the fp16 tiles K and Q
-// [chunk][k_heads][2][64][DK] that the chunk kernel reads.
+// Three TF32 MMAs for a product of fp32 values (22 bits): a, b split here.
+__device__ __forceinline__ void tf32_split2(float v, unsigned& hi, unsigned& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));
+}
+__device__ __forceinline__ void mma_tf32_acc(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The corner of the 2N x 2N block of T at (o, o): Y = -T22 (L21 T11), taken transposed, M^T = T11^T L21^T and
+// Y^T = -M^T T22^T, so that M^T passes from accumulators to left operands in registers (an operand's k-th
+// and k+4-th columns are the accumulator's columns 2k and 2k+1; the right operand follows).  A warp takes 16
+// rows mt of the transposed matrices and, of Y^T, half the columns.
+template <int N>
+__device__ __forceinline__ void corner(const float* L, float* X, int o, int half, int mt, int lane) {
+  constexpr int NTI = N / 8;
+  const int g = lane >> 2, c = lane & 3;
+  const float* L21 = L + (o + N) * kLS + o;
+  const float* T11 = X + o * kLS + o + 16 * mt;
+  const float* T22 = X + (o + N) * kLS + o + N;
+  float m[NTI][4] = {};
+#pragma unroll
+  for (int k = 0; k < N; k += 8) {
+    if (k + 8 > 16 * mt) {  // T11^T is upper triangular
+      unsigned ah[4], al[4];
+      const float* x = T11 + (k + 2 * c) * kLS + g;
+      tf32_split2(x[0], ah[0], al[0]);
+      tf32_split2(x[8], ah[1], al[1]);
+      tf32_split2(x[kLS], ah[2], al[2]);
+      tf32_split2(x[kLS + 8], ah[3], al[3]);
+#pragma unroll
+      for (int j = 0; j < NTI; ++j) {
+        const float2 l = *reinterpret_cast<const float2*>(L21 + (8 * j + g) * kLS + k + 2 * c);
+        unsigned bh0, bl0, bh1, bl1;
+        tf32_split2(l.x, bh0, bl0);
+        tf32_split2(l.y, bh1, bl1);
+        mma_tf32_acc(m[j], al, bh0, bh1);
+        mma_tf32_acc(m[j], ah, bl0, bl1);
+        mma_tf32_acc(m[j], ah, bh0, bh1);
+      }
+    }
+  }
+  float y[NTI / 2][4] = {};
+#pragma unroll
+  for (int i = 0; i < NTI; ++i) {  // columns 8 i.. of M^T
+    unsigned ah[4], al[4];
+    tf32_split2(m[i][0], ah[0], al[0]);
+    tf32_split2(m[i][2], ah[1], al[1]);
+    tf32_split2(m[i][1], ah[2], al[2]);
+    tf32_split2(m[i][3], ah[3], al[3]);
+#pragma unroll
+    for (int j = 0; j < NTI / 2; ++j) {
+      const float2 t = *reinterpret_cast<const float2*>(T22 + (8 * (half * (NTI / 2) + j) + g) * kLS + 8 * i + 2 * c);
+      unsigned bh0, bl0, bh1, bl1;
+      tf32_split2(t.x, bh0, bl0);
+      tf32_split2(t.y, bh1, bl1);
+      mma_tf32_acc(y[j], al, bh0, bh1);
+      mma_tf32_acc(y[j], ah, bl0, bl1);
+      mma_tf32_acc(y[j], ah, bh0, bh1);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NTI / 2; ++j) {
+    float* out = X + (o + N + 8 * (half * (NTI / 2) + j) + 2 * c) * kLS + o + 16 * mt + g;
+    out[0] = -y[j][0];
+    out[kLS] = -y[j][1];
+    out[8] = -y[j][2];
+    out[kLS + 8] = -y[j][3];
+  }
+}
+
+// kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.
 template <typename T, int DK>
-__global__ void __launch_bounds__(kPrepThreads)
-gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __half* __restrict__ kq16) {
+__global__ void __launch_bounds__(kPrepThreads, 4)
+gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __half* __restrict__ kq16, int groups,
+                        int per_group) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int UPR = DK / 8;  // 16-byte units per row
   extern __shared__ __align__(128) char smem[];
   __half* Ks = reinterpret_cast<__half*>(smem);
   __half* Qs = Ks + kGdC * DK;
-  float* L = reinterpret_cast<float*>(Qs + kGdC * DK);  // [64][kLS]
-  float* X = L + kGdC * kLS;                            // [64][kLS]: T
-  float* rk = X + kGdC * kLS;                           // row factors of K and Q as staged
+  float* X = reinterpret_cast<float*>(smem);  // T, once K and Q have been multiplied
+  float* L = reinterpret_cast<float*>(smem + gd_prep_tiles<DK>());  // [64][kLS]
+  double* G = reinterpret_cast<double*>(L + kGdC * kLS);            // running log decay
+  float* rk = reinterpret_cast<float*>(G + 64);                     // row factors of K and Q as staged
   float* rq = rk + 64;
-  float* beta = rq + 64;
-  double* G = reinterpret_cast<double*>(beta + 64);  // running log decay
-  float* tmax = reinterpret_cast<float*>(G + 64);    // [2][64]
+  float* fk = rq + 64;      // rk beta
+  float* rowf = fk + 64;    // e^(G_t - boundary before t's block)
+  float* colf = rowf + 64;  // [3][64]: e^(boundary before block 1, 2, 3 - G_w) rk_w beta_w
+  float* up_t = colf + 192;  // the rows' scales of T
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int h = blockIdx.x % p.v_heads, num = blockIdx.x / p.v_heads;
+  const int rep = p.v_heads / p.k_heads;
+  const int grp = blockIdx.x % groups, hk = (blockIdx.x / groups) % p.k_heads, num = blockIdx.x / (groups * p.k_heads);
   // the sequence of chunk `num`: the last one whose first chunk is not behind it
   int lo = 0, hi = p.n_seq - 1;
   while (lo < hi) {
@@ -131,7 +224,6 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   if (cn < 0 || cn * kGdC >= count) return;
   first += cn * kGdC;
   count = min(count - cn * kGdC, kGdC);
-  const int rep = p.v_heads / p.k_heads, hk = h / rep;
   // K and Q rows: DK / 8 lanes per row, one 16-byte unit each; the row's factor is 1 / |row| (qk_norm) times,
   // for bf16, the power of two that undoes the staging's
   {
@@ -151,268 +243,281 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
       for (int i = 0; i < kGdC / RPI; ++i) {
         const int t = r0 + i * RPI;
         const T* e = reinterpret_cast<const T*>(&raw[i]);
-        float f[8], ss = 0.f, mx = 0.f;
+        float factor = 1.f;
+        if (BF || p.qk_norm) {
+          float f[8], ss = 0.f, mx = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[j] = to_f(e[j]);
-          ss += f[j] * f[j];
-          mx = fmaxf(mx, fabsf(f[j]));
-        }
+          for (int j = 0; j < 8; ++j) {
+            f[j] = to_f(e[j]);
+            ss = fmaf(f[j], f[j], ss);
+            if constexpr (BF) mx = fmaxf(mx, fabsf(f[j]));
+          }
 #pragma unroll
-        for (int o = UPR / 2; o > 0; o >>= 1) {
-          ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if constexpr (BF) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        }
-        float factor = p.qk_norm ? 1.0f / sqrtf(ss + kQkEps) : 1.0f;
-        if constexpr (BF) {
-          float up, down;
-          row_scale(mx, up, down);
-          factor *= down;
-          uint4 out;
-          unsigned* ow = reinterpret_cast<unsigned*>(&out);
+          for (int o = UPR / 2; o > 0; o >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if constexpr (BF) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          }
+          if (p.qk_norm) factor = 1.0f / sqrtf(ss + kQkEps);
+          if constexpr (BF) {
+            float up, down;
+            row_scale(mx, up, down);
+            factor *= down;
+            uint4 out;
+            unsigned* ow = reinterpret_cast<unsigned*>(&out);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) ow[j] = h2_bits(__floats2half2_rn(f[2 * j] * up, f[2 * j + 1] * up));
-          raw[i] = out;
-          if (h % rep == 0)
-            *reinterpret_cast<uint4*>(kq16 + ((((size_t)num * p.k_heads + hk) * 2 + which) * kGdC + t) * DK + u * 8) = out;
+            for (int j = 0; j < 4; ++j) ow[j] = h2_bits(__floats2half2_rn(f[2 * j] * up, f[2 * j + 1] * up));
+            raw[i] = out;
+            if (grp == 0)
+              *reinterpret_cast<uint4*>(kq16 + ((((size_t)num * p.k_heads + hk) * 2 + which) * kGdC + t) * DK + u * 8) = out;
+          }
         }
         *reinterpret_cast<uint4*>(reinterpret_cast<char*>(which ? Qs : Ks) + kq_off<DK>(t, u)) = raw[i];
         if (u == 0) (which ? rq : rk)[t] = factor;
       }
     }
   }
-  // gates: one thread per token, the running sum in double precision
-  if (tid < 64) {
-    double gl = 0.0;
-    float bt = 0.f;
-    if (tid < count) {
-      gl = gd_log_decay(to_f(static_cast<const T*>(p.a)[(size_t)(first + tid) * p.ld_a + h]), p.dt_bias[h], p.A_log[h]);
-      bt = gd_beta(to_f(static_cast<const T*>(p.b)[(size_t)(first + tid) * p.ld_b + h]));
-    }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, gl, o);
-      if (lane >= o) gl += x;
-    }
-    G[tid] = gl;
-    beta[tid] = bt;
-  }
   __syncthreads();
-  if (tid >= 32 && tid < 64) G[tid] += G[31];
-  __syncthreads();
-  const double Glast = G[63];
-  char* blk = blocks + ((size_t)num * p.v_heads + h) * kGdBlock;
-  float* vec = reinterpret_cast<float*>(blk + 2 * kGdTri);
   // Q K^T rows 16 wid.. and K K^T rows 16 (3 - wid)..: ten 16 x 8 tiles for every warp
-  const uint32_t ks = smem_u32(Ks), qs = smem_u32(Qs);
-  auto gram = [&](uint32_t a_tile, int mt, float (&acc)[8][4]) {
+  const int mk = 3 - wid;
+  float qk[8][4], kk_[8][4];
+  {
+    const uint32_t ks = smem_u32(Ks), qs = smem_u32(Qs);
+    auto gram = [&](uint32_t a_tile, int mt, float (&acc)[8][4]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+      for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < DK / 16; ++kk) {
-      unsigned a[4];
-      ldsm4(a, a_tile + kq_off<DK>(16 * mt + (lane & 15), 2 * kk + (lane >> 4)));
+      for (int kk = 0; kk < DK / 16; ++kk) {
+        unsigned a[4];
+        ldsm4(a, a_tile + kq_off<DK>(16 * mt + (lane & 15), 2 * kk + (lane >> 4)));
 #pragma unroll
-      for (int jp = 0; jp < 4; ++jp) {
-        if (jp <= mt) {
-          unsigned b[4];
-          ldsm4(b, ks + kq_off<DK>(16 * jp + ((lane >> 4) << 3) + (lane & 7), 2 * kk + ((lane >> 3) & 1)));
-          mma_f16(acc[2 * jp], a[0], a[1], a[2], a[3], b[0], b[1]);
-          mma_f16(acc[2 * jp + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+        for (int jp = 0; jp < 4; ++jp) {
+          if (jp <= mt) {
+            unsigned b[4];
+            ldsm4(b, ks + kq_off<DK>(16 * jp + ((lane >> 4) << 3) + (lane & 7), 2 * kk + ((lane >> 3) & 1)));
+            mma_acc(acc[2 * jp], a, b[0], b[1]);
+            mma_acc(acc[2 * jp + 1], a, b[2], b[3]);
+          }
+        }
+      }
+    };
+    gram(qs, wid, qk);
+    gram(ks, mk, kk_);
+  }
+  __syncthreads();
+  for (int i = tid; i < 512 / 4; i += kPrepThreads) {  // the two blocks of T above the diagonal that are read below
+    const int o = 32 * (i >> 6), r = (i & 63) >> 2, w = (i & 3) * 4;
+    *reinterpret_cast<float4*>(X + (o + r) * kLS + o + 16 + w) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const int h1 = min(hk * rep + (grp + 1) * per_group, (hk + 1) * rep);
+  for (int h = hk * rep + grp * per_group; h < h1; ++h) {
+    // gates: one thread per token, the running sum in double precision
+    if (tid < 64) {
+      double gl = 0.0;
+      float bt = 0.f;
+      if (tid < count) {
+        gl = gd_log_decay(to_f(static_cast<const T*>(p.a)[(size_t)(first + tid) * p.ld_a + h]), p.dt_bias[h], p.A_log[h]);
+        bt = gd_beta(to_f(static_cast<const T*>(p.b)[(size_t)(first + tid) * p.ld_b + h]));
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, gl, o);
+        if (lane >= o) gl += x;
+      }
+      G[tid] = gl;
+      fk[tid] = rk[tid] * bt;
+    }
+    __syncthreads();
+    if (tid >= 32 && tid < 64) G[tid] += G[31];
+    __syncthreads();
+    char* blk = blocks + ((size_t)num * p.v_heads + h) * kGdBlock;
+    float* vec = reinterpret_cast<float*>(blk + 2 * kGdTri);
+    {
+      const int t = tid & 63;
+      const double Gt = G[t];
+      if (tid < 64) {  // factors of the chunk kernel
+        const float eg = expf((float)Gt);
+        vec[kGdBk + t] = -eg * rk[t];
+        vec[kGdC2 + t] = expf((float)(G[63] - Gt)) * fk[t];
+        vec[kGdOq + t] = p.scale * eg * rq[t];
+        if (t == 0) vec[kGdLast] = expf((float)G[63]);
+        if (t < 32) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
+      } else {  // factors of this one
+        if (t >= 16) rowf[t] = expf((float)(Gt - G[(t & ~15) - 1]));
+        if (t < 16) colf[t] = expf((float)(G[15] - Gt)) * fk[t];
+        if (t < 32) colf[64 + t] = expf((float)(G[31] - Gt)) * fk[t];
+        else if (t < 48) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
+      }
+    }
+    __syncthreads();
+    // P: rows ta, tb of Q K^T
+    {
+      const int ta = 16 * wid + g, tb = ta + 8;
+      const float ra = p.scale * rq[ta], rb = p.scale * rq[tb];
+      float x[8][4], ma = 0.f, mb = 0.f;
+      if (wid > 0) {
+        const float fa = ra * rowf[ta], fb = rb * rowf[tb];
+        const float* cf = colf + 64 * (wid - 1) + 2 * c;
+#pragma unroll
+        for (int j = 0; j < 6; ++j) {
+          if (j < 2 * wid) {
+            const float2 f = *reinterpret_cast<const float2*>(cf + 8 * j);
+            x[j][0] = qk[j][0] * fa * f.x;
+            x[j][1] = qk[j][1] * fa * f.y;
+            x[j][2] = qk[j][2] * fb * f.x;
+            x[j][3] = qk[j][3] * fb * f.y;
+            ma = fmaxf(ma, fmaxf(fabsf(x[j][0]), fabsf(x[j][1])));
+            mb = fmaxf(mb, fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
+          }
+        }
+      }
+      const double Ga = G[ta], Gb = G[tb];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j == 2 * wid || j == 2 * wid + 1) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int w = 8 * j + 2 * c + i;
+            x[j][i] = w <= ta ? qk[j][i] * ra * (fk[w] * expf((float)(Ga - G[w]))) : 0.f;
+            x[j][2 + i] = w <= tb ? qk[j][2 + i] * rb * (fk[w] * expf((float)(Gb - G[w]))) : 0.f;
+            ma = fmaxf(ma, fabsf(x[j][i]));
+            mb = fmaxf(mb, fabsf(x[j][2 + i]));
+          }
+        }
+      }
+      float ua, da, ub, db;
+      row_scale(quad_max(ma), ua, da);
+      row_scale(quad_max(mb), ub, db);
+      if (c == 0) {
+        vec[kGdOp + ta] = da;
+        vec[kGdOp + tb] = db;
+      }
+      uint4* P = reinterpret_cast<uint4*>(blk + kGdTri);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        if (kk <= wid) {
+          unsigned ha0, la0, ha1, la1, hb0, lb0, hb1, lb1;
+          split2(x[2 * kk][0] * ua, x[2 * kk][1] * ua, ha0, la0);
+          split2(x[2 * kk + 1][0] * ua, x[2 * kk + 1][1] * ua, ha1, la1);
+          split2(x[2 * kk][2] * ub, x[2 * kk][3] * ub, hb0, lb0);
+          split2(x[2 * kk + 1][2] * ub, x[2 * kk + 1][3] * ub, hb1, lb1);
+          P[gd_frag(2 * wid, kk) * 32 + lane] = make_uint4(ha0, ha1, la0, la1);
+          P[gd_frag(2 * wid + 1, kk) * 32 + lane] = make_uint4(hb0, hb1, lb0, lb1);
         }
       }
     }
-  };
-  {
-    float acc[8][4];
-    gram(qs, wid, acc);
-    const int ta = 16 * wid + g, tb = ta + 8;
-    const double Ga = G[ta], Gb = G[tb];
-    const float fa = p.scale * rq[ta], fb = p.scale * rq[tb];
-    float ma = 0.f, mb = 0.f;
+    // L: rows of K K^T
+    {
+      const int ta = 16 * mk + g, tb = ta + 8;
+      const float ra = rk[ta], rb = rk[tb];
+      if (mk > 0) {
+        const float fa = ra * rowf[ta], fb = rb * rowf[tb];
+        const float* cf = colf + 64 * (mk - 1) + 2 * c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j <= 2 * wid + 1) {
+        for (int j = 0; j < 6; ++j) {
+          if (j < 2 * mk) {
+            const float2 f = *reinterpret_cast<const float2*>(cf + 8 * j);
+            *reinterpret_cast<float2*>(L + ta * kLS + 8 * j + 2 * c) = make_float2(kk_[j][0] * fa * f.x, kk_[j][1] * fa * f.y);
+            *reinterpret_cast<float2*>(L + tb * kLS + 8 * j + 2 * c) = make_float2(kk_[j][2] * fb * f.x, kk_[j][3] * fb * f.y);
+          }
+        }
+      }
+      const double Ga = G[ta], Gb = G[tb];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int w = 8 * j + 2 * c + i;
-          const float ea = expf((float)(Ga - G[w])), eb = expf((float)(Gb - G[w]));
-          const float fw = rk[w] * beta[w];
-          acc[j][i] = w <= ta ? acc[j][i] * fa * fw * ea : 0.f;
-          acc[j][2 + i] = w <= tb ? acc[j][2 + i] * fb * fw * eb : 0.f;
-          ma = fmaxf(ma, fabsf(acc[j][i]));
-          mb = fmaxf(mb, fabsf(acc[j][2 + i]));
+      for (int j = 0; j < 8; ++j) {
+        if (j == 2 * mk || j == 2 * mk + 1) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int w = 8 * j + 2 * c + i;
+            L[ta * kLS + w] = w < ta ? kk_[j][i] * ra * (fk[w] * expf((float)(Ga - G[w]))) : 0.f;
+            L[tb * kLS + w] = w < tb ? kk_[j][2 + i] * rb * (fk[w] * expf((float)(Gb - G[w]))) : 0.f;
+          }
+        }
+      }
+      __syncwarp();
+      // the diagonal block of these rows: a lane per column of its inverse
+      if (lane < 16) {
+        const float* Lb = L + 16 * mk * kLS + 16 * mk;
+        float* Xb = X + 16 * mk * kLS + 16 * mk + lane;
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float l[16];
+#pragma unroll
+          for (int m = 0; m < i; m += 4) *reinterpret_cast<float4*>(l + m) = *reinterpret_cast<const float4*>(Lb + i * kLS + m);
+          float s0 = i == lane ? 1.f : 0.f, s1 = 0.f;
+#pragma unroll
+          for (int m = 0; m < i; ++m) {
+            if (m & 1) s1 = fmaf(-l[m], y[m], s1);
+            else s0 = fmaf(-l[m], y[m], s0);
+          }
+          y[i] = s0 + s1;
+          Xb[i * kLS] = y[i];
         }
       }
     }
-    float ua, da, ub, db;
-    row_scale(quad_max(ma), ua, da);
-    row_scale(quad_max(mb), ub, db);
-    if (c == 0) {
-      vec[kGdOp + ta] = da;
-      vec[kGdOp + tb] = db;
-    }
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      if (kk <= wid) {
-        unsigned ha0, la0, ha1, la1, hb0, lb0, hb1, lb1;
-        split2(acc[2 * kk][0] * ua, acc[2 * kk][1] * ua, ha0, la0);
-        split2(acc[2 * kk + 1][0] * ua, acc[2 * kk + 1][1] * ua, ha1, la1);
-        split2(acc[2 * kk][2] * ub, acc[2 * kk][3] * ub, hb0, lb0);
-        split2(acc[2 * kk + 1][2] * ub, acc[2 * kk + 1][3] * ub, hb1, lb1);
-        uint4* P = reinterpret_cast<uint4*>(blk + kGdTri);
-        P[gd_frag(2 * wid, kk) * 32 + lane] = make_uint4(ha0, ha1, la0, la1);
-        P[gd_frag(2 * wid + 1, kk) * 32 + lane] = make_uint4(hb0, hb1, lb0, lb1);
-      }
-    }
-  }
-  {
-    float acc[8][4];
-    const int mt = 3 - wid;
-    gram(ks, mt, acc);
-    const int ta = 16 * mt + g, tb = ta + 8;
-    const double Ga = G[ta], Gb = G[tb];
-    const float fa = rk[ta], fb = rk[tb];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int w = 8 * j + 2 * c + i;
-        const bool va = j <= 2 * mt + 1 && w < ta, vb = j <= 2 * mt + 1 && w < tb;
-        const float fw = rk[w] * beta[w];
-        L[ta * kLS + w] = va ? acc[j][i] * fa * fw * expf((float)(Ga - G[w])) : 0.f;
-        L[tb * kLS + w] = vb ? acc[j][2 + i] * fb * fw * expf((float)(Gb - G[w])) : 0.f;
-      }
-    }
-  }
-  // per-token factors
-  if (tid < 64) {
-    const double Gt = G[tid];
-    const float eg = expf((float)Gt);
-    vec[kGdBk + tid] = -eg * rk[tid];
-    vec[kGdC2 + tid] = expf((float)(Glast - Gt)) * rk[tid] * beta[tid];
-    vec[kGdOq + tid] = p.scale * eg * rq[tid];
-    if (tid == 0) vec[kGdLast] = expf((float)Glast);
-  }
-  __syncthreads();
-  // T = (I + L)^-1: the 16 x 16 diagonal blocks by forward substitution, a lane per column ...
-  for (int i = tid; i < kGdC * kLS; i += kPrepThreads) X[i] = 0.f;
-  __syncthreads();
-  if (lane < 16) {
-    const float* Lb = L + 16 * wid * kLS + 16 * wid;
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == lane ? 1.f : 0.f;
-#pragma unroll
-      for (int m = 0; m < i; ++m) s = fmaf(-Lb[i * kLS + m], x[m], s);
-      x[i] = s;
-      X[(16 * wid + i) * kLS + 16 * wid + lane] = s;
-    }
-  }
-  __syncthreads();
-  // ... then pairs of blocks joined, 16 to 32 and 32 to 64: the corner is -T22 (L21 T11)
-  float* M = reinterpret_cast<float*>(smem);  // K and Q are not read again: [2][16][20], then [32][36]
-  {
-    const int pair = tid >> 6, r = (tid & 63) >> 2, c0 = (tid & 3) * 4, o = 32 * pair;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int m = 0; m < 16; ++m) {
-      const float l = L[(o + 16 + r) * kLS + o + m];
-      const float4 x = *reinterpret_cast<const float4*>(X + (o + m) * kLS + o + c0);
-      s[0] = fmaf(l, x.x, s[0]), s[1] = fmaf(l, x.y, s[1]), s[2] = fmaf(l, x.z, s[2]), s[3] = fmaf(l, x.w, s[3]);
-    }
-    *reinterpret_cast<float4*>(M + (pair * 16 + r) * 20 + c0) = make_float4(s[0], s[1], s[2], s[3]);
     __syncthreads();
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int m = 0; m < 16; ++m) {
-      const float l = X[(o + 16 + r) * kLS + o + 16 + m];
-      const float4 x = *reinterpret_cast<const float4*>(M + (pair * 16 + m) * 20 + c0);
-      y[0] = fmaf(-l, x.x, y[0]), y[1] = fmaf(-l, x.y, y[1]), y[2] = fmaf(-l, x.z, y[2]), y[3] = fmaf(-l, x.w, y[3]);
-    }
-    *reinterpret_cast<float4*>(X + (o + 16 + r) * kLS + o + c0) = make_float4(y[0], y[1], y[2], y[3]);
-  }
-  __syncthreads();
-  {
-    const int r = (tid >> 3) * 2, c0 = (tid & 7) * 4;  // 16 x 8 threads of 2 x 4 outputs
-    float s[2][4] = {};
-#pragma unroll 8
-    for (int m = 0; m < 32; ++m) {
-      const float4 x = *reinterpret_cast<const float4*>(X + m * kLS + c0);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float l = L[(32 + r + i) * kLS + m];
-        s[i][0] = fmaf(l, x.x, s[i][0]), s[i][1] = fmaf(l, x.y, s[i][1]);
-        s[i][2] = fmaf(l, x.z, s[i][2]), s[i][3] = fmaf(l, x.w, s[i][3]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<float4*>(M + (r + i) * 36 + c0) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+    corner<16>(L, X, 32 * (wid >> 1), wid & 1, 0, lane);  // of the two 32 x 32 blocks
     __syncthreads();
-    float y[2][4] = {};
-#pragma unroll 8
-    for (int m = 0; m < 32; ++m) {
-      const float4 x = *reinterpret_cast<const float4*>(M + m * 36 + c0);
+    corner<32>(L, X, 0, wid >> 1, wid & 1, lane);
+    __syncthreads();
+    {  // the rows' scales
+      const int t = tid >> 1, half = tid & 1;
+      float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float l = X[(32 + r + i) * kLS + 32 + m];
-        y[i][0] = fmaf(-l, x.x, y[i][0]), y[i][1] = fmaf(-l, x.y, y[i][1]);
-        y[i][2] = fmaf(-l, x.z, y[i][2]), y[i][3] = fmaf(-l, x.w, y[i][3]);
+      for (int w = 0; w < 32; w += 4) {
+        if (32 * half + w <= t) {
+          const float4 x = *reinterpret_cast<const float4*>(X + t * kLS + 32 * half + w);
+          m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        }
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      float up, down;
+      row_scale(m, up, down);
+      if (half == 0) {
+        up_t[t] = up;
+        vec[kGdTs + t] = down;
       }
     }
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<float4*>(X + (32 + r + i) * kLS + c0) = make_float4(y[i][0], y[i][1], y[i][2], y[i][3]);
-  }
-  __syncthreads();
-  {  // the rows' scales
-    const int t = tid >> 1, half = tid & 1;
-    float m = 0.f;
+    for (int f = 0; f < kGdFrags / 4; ++f) {  // fragment 4 f + wid
+      const int id = 4 * f + wid;
+      int j = 0;
 #pragma unroll
-    for (int w = 0; w < 32; w += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(X + t * kLS + 32 * half + w);
-      m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+      for (int x = 1; x < 8; ++x) j += id >= gd_frag(x, 0);
+      const int kk = id - gd_frag(j, 0), t = 8 * j + g;
+      const float up = up_t[t];
+      const float2 x = *reinterpret_cast<const float2*>(X + t * kLS + 16 * kk + 2 * c);
+      const float2 y = *reinterpret_cast<const float2*>(X + t * kLS + 16 * kk + 2 * c + 8);
+      unsigned h0, l0, h1, l1;
+      split2(x.x * up, x.y * up, h0, l0);
+      split2(y.x * up, y.y * up, h1, l1);
+      reinterpret_cast<uint4*>(blk)[id * 32 + lane] = make_uint4(h0, h1, l0, l1);
     }
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    float up, down;
-    row_scale(m, up, down);
-    if (half == 0) {
-      tmax[t] = up;
-      vec[kGdTs + t] = down;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int f = 0; f < kGdFrags / 4; ++f) {  // fragment 4 f + wid
-    const int id = 4 * f + wid;
-    int j = 0;
-#pragma unroll
-    for (int x = 1; x < 8; ++x) j += id >= gd_frag(x, 0);
-    const int kk = id - gd_frag(j, 0), t = 8 * j + g;
-    const float up = tmax[t];
-    const float* x = X + t * kLS + 16 * kk + 2 * c;
-    unsigned h0, l0, h1, l1;
-    split2(x[0] * up, x[1] * up, h0, l0);
-    split2(x[8] * up, x[9] * up, h1, l1);
-    reinterpret_cast<uint4*>(blk)[id * 32 + lane] = make_uint4(h0, h1, l0, l1);
+    // the next head's gates touch nothing that is still read: G and the factors were last used before
+    // the barriers above
   }
 }
 
 // ------------------------------------------------------------------ the walk over a sequence's chunks
 //
-// A warp owns 16 rows of one head's state, S^T as MMA accumulators (64 registers per thread at dk = 128).  All
-// products are taken transposed, with the state, r and u as left operands: the accumulator layout of one
-// product is the left operand's layout of the next, so nothing but k, q, v, T and P passes through shared
-// memory, and warps meet only where its buffers change hands.
+// A pair of warps owns 16 rows of one head's state.  The first, the chain warp, holds S^T as MMA accumulators
+// (64 registers per thread at dk = 128) and computes what the next chunk waits for: S k, r, u, the new S.  The
+// second, the output warp, takes the operands that the first has split anyway (S and u as fp16 pairs, through
+// shared memory) and computes S q + u P^T and the rows of o; it also fetches the next chunk (cp.async).  All
+// products are taken transposed, with S, r and u as left operands: the accumulator layout of one product is
+// the left operand's layout of the next, so nothing of the chain itself passes through shared memory.
 //   S k, S q : [16 x dk] [dk x 64]     u = r T^T, u P^T : [16 x 64] [64 x 64]     u k : [16 x 64] [64 x dk]
-// K is double buffered; Q, V, T, P and the factors of the next chunk arrive (cp.async) while the products that
-// do not read them run.
+// K is double buffered; Q, V, T, P and the factors of the next chunk are fetched while the products that do
+// not read them run.
+//
+// Bound: the chain of a chunk is 316 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM) and
+// the splits between them, one after the other; a second pair per scheduler fills the gaps when there are
+// enough sequences and heads.
 
 template <int DK, int W>
 __host__ __device__ constexpr int gd_chunk_smem() {
-  return 3 * kGdC * DK * 2 + kGdC * 32 * W + kGdBlock;
+  return 3 * kGdC * DK * 2 + kGdC * 32 * W + kGdBlock + W * (DK / 16 * 1024 + 4096 + 128);
 }
 
 // Byte offset of 16-byte unit u of token t in the V tile [64][16 W].
@@ -421,14 +526,43 @@ __device__ __forceinline__ uint32_t v_off(int t, int u) {
   const int f = W >= 4 ? (t & 7) : (W == 2 ? ((t >> 1) & 3) : ((t >> 2) & 1));
   return (uint32_t)(t * 32 * W + ((u ^ f) << 4));
 }
+// Named barriers: 0 the block, 1 the output warps, 2 + 3 pair + {0: S is split, 1: u is split, 2: both are read}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 
-// ldb: element strides of the K / Q tiles' rows.  For fp16 inputs kq16 is NULL and the tiles are rows of k and q.
+// x[j] += rows of (ah + al) times the 64 x 64 triangular matrix in fragment order, for n-tiles J0 .. J0 + 3
+template <int J0>
+__device__ __forceinline__ void tri_product(float (&x)[4][4], const unsigned (&ah)[4][4], const unsigned (&al)[4][4],
+                                            const uint4* F) {
+#pragma unroll
+  for (int kk = 0; kk <= (J0 + 3) / 2; ++kk) {
+    uint4 b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (kk <= (J0 + i) / 2) b[i] = F[gd_frag(J0 + i, kk) * 32];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk], b[i].z, b[i].w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (kk <= (J0 + i) / 2) mma_acc(x[i], al[kk], b[i].x, b[i].y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk], b[i].x, b[i].y);
+  }
+}
+
+// kq16: the fp16 tiles of K and Q for bf16 inputs; for fp16 inputs the tiles are rows of k and q themselves.
 template <typename T, int DK, int W>
-__global__ void __launch_bounds__(32 * W, 8 / W)
+__global__ void __launch_bounds__(64 * W, W == 2 ? 2 : 1)
 gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
                          int parts, int slots_total) {
   constexpr bool BF = !std::is_same<T, __half>::value;
-  constexpr int NT = 32 * W, NK = DK / 8, UPR = DK / 8;
+  constexpr int NT = 64 * W, NL = 32 * W, NK = DK / 8, UPR = DK / 8;
   extern __shared__ __align__(128) char smem[];
   char* vt = smem + 3 * kGdC * DK * 2;
   char* tp = vt + kGdC * 32 * W;
@@ -444,44 +578,147 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   const int base = gd_chunk_base(p.cu, seq, p.tokens);
   const int chunks = min((count + kGdC - 1) / kGdC, slots_total - base);
   const int hk = h / (p.v_heads / p.k_heads);
-  const int dv0 = part * 16 * W, row0 = dv0 + 16 * wid;
-  const bool active = row0 < p.dv;  // dv is a multiple of 16: a warp's rows are all there or none
+  const bool chain = wid < W;
+  const int pair = chain ? wid : wid - W;
+  const int dv0 = part * 16 * W, row0 = dv0 + 16 * pair;
+  const bool active = row0 < p.dv;  // dv is a multiple of 16: a pair's rows are all there or none
+  char* ex = tp + kGdBlock + pair * (DK / 16 * 1024 + 4096 + 128);
+  uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;                           // S: [dk / 16][hi, lo][32]
+  uint4* u_ex = reinterpret_cast<uint4*>(ex + DK / 16 * 1024) + lane;          // u: [4][hi, lo][32]
+  float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);            // [2][16] the rows' scales
+  const int bar = 2 + 3 * pair;
+  // lane parts of the ldmatrix addresses
+  const int bt = ((lane >> 4) << 3) + (lane & 7), bu = (lane >> 3) & 1;  // B from [token][dk] rows, two n-tiles
+  const int tt = (((lane >> 3) & 1) << 3) + (lane & 7), tu = lane >> 4;  // the same, transposed
 
-  auto load_kq = [&](int ch) {  // K and Q of chunk ch
-    const int n = count - ch * kGdC;
-    const uint32_t kd = k_s + (ch & 1) * kGdC * DK * 2;
-    const size_t row = (size_t)first + (size_t)ch * kGdC;
-    for (int i = tid; i < kGdC * UPR; i += NT) {
-      const int t = i / UPR, u = i % UPR;
-      if constexpr (BF) {
-        const __half* src = kq16 + (((size_t)(base + ch) * p.k_heads + hk) * 2 * kGdC + t) * DK + u * 8;
-        cp16(kd + kq_off<DK>(t, u), src, true);
-        cp16(q_s + kq_off<DK>(t, u), src + kGdC * DK, true);
-      } else {
-        const bool ok = t < n;
-        const size_t r = ok ? row + t : row;
-        cp16(kd + kq_off<DK>(t, u), static_cast<const __half*>(p.k) + r * p.ld_k + hk * DK + u * 8, ok);
-        cp16(q_s + kq_off<DK>(t, u), static_cast<const __half*>(p.q) + r * p.ld_q + hk * DK + u * 8, ok);
+  if (!chain) {
+    // ---------------------------------------------------------------- output warp
+    const int lt = tid - NL;
+    auto load_kq = [&](int ch) {  // K and Q of chunk ch
+      const int n = count - ch * kGdC;
+      const uint32_t kd = k_s + (ch & 1) * kGdC * DK * 2;
+      const size_t row = (size_t)first + (size_t)ch * kGdC;
+#pragma unroll 4
+      for (int i = lt; i < kGdC * UPR; i += NL) {
+        const int t = i / UPR, u = i % UPR;
+        if constexpr (BF) {
+          const __half* src = kq16 + (((size_t)(base + ch) * p.k_heads + hk) * 2 * kGdC + t) * DK + u * 8;
+          cp16(kd + kq_off<DK>(t, u), src, true);
+          cp16(q_s + kq_off<DK>(t, u), src + kGdC * DK, true);
+        } else {
+          const bool ok = t < n;
+          const size_t r = ok ? row + t : row;
+          cp16(kd + kq_off<DK>(t, u), static_cast<const __half*>(p.k) + r * p.ld_k + hk * DK + u * 8, ok);
+          cp16(q_s + kq_off<DK>(t, u), static_cast<const __half*>(p.q) + r * p.ld_q + hk * DK + u * 8, ok);
+        }
       }
+      cp_commit();
+    };
+    auto load_vtp = [&](int ch) {  // V, T, P and the factors of chunk ch
+      const int n = count - ch * kGdC;
+      const size_t row = (size_t)first + (size_t)ch * kGdC;
+      const int units = min(16 * W, p.dv - dv0) / 8;
+#pragma unroll
+      for (int i = lt; i < kGdC * 2 * W; i += NL) {
+        const int t = i / (2 * W), u = i % (2 * W);
+        const bool ok = t < n && u < units;
+        cp16(v_s + v_off<W>(t, u), static_cast<const T*>(p.v) + (ok ? (row + t) * p.ld_v + h * p.dv + dv0 + u * 8 : 0), ok);
+      }
+      const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock;
+#pragma unroll 4
+      for (int i = lt; i < kGdBlock / 16; i += NL) cp16(tp_s + i * 16, blk + i * 16, true);
+      cp_commit();
+    };
+    load_kq(0);
+    load_vtp(0);
+    for (int ch = 0; ch < chunks; ++ch) {
+      cp_wait<1>();
+      bar_sync(0, NT);  // K and Q are there
+      bar_sync(bar, 64);
+      float o[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < DK / 16; ++kk) {
+        const uint4 hv = s_ex[(2 * kk) * 32], lv = s_ex[(2 * kk + 1) * 32];
+        const unsigned ah[4] = {hv.x, hv.y, hv.z, hv.w}, al[4] = {lv.x, lv.y, lv.z, lv.w};
+        unsigned b[4][4];
+#pragma unroll
+        for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], q_s + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mma_acc(o[j], al, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mma_acc(o[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+      }
+      const float ds0 = sc[g], ds1 = sc[g + 8];
+      bar_sync(1, NL);  // Q is free, and the other K buffer, which the chains left before they split S
+      if (ch + 1 < chunks) load_kq(ch + 1);
+      else cp_commit();
+      cp_wait<1>();
+      bar_sync(0, NT);  // V, T and P are there
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 oq = *reinterpret_cast<const float2*>(vec + kGdOq + 8 * j + 2 * c);
+        o[j][0] *= oq.x * ds0;
+        o[j][1] *= oq.y * ds0;
+        o[j][2] *= oq.x * ds1;
+        o[j][3] *= oq.y * ds1;
+      }
+      bar_sync(bar + 1, 64);
+      unsigned ah[4][4], al[4][4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const uint4 hv = u_ex[(2 * kk) * 32], lv = u_ex[(2 * kk + 1) * 32];
+        ah[kk][0] = hv.x, ah[kk][1] = hv.y, ah[kk][2] = hv.z, ah[kk][3] = hv.w;
+        al[kk][0] = lv.x, al[kk][1] = lv.y, al[kk][2] = lv.z, al[kk][3] = lv.w;
+      }
+      const float du0 = sc[16 + g], du1 = sc[24 + g];
+      if (ch + 1 < chunks) bar_arrive(bar + 2, 64);
+      const uint4* Pf = reinterpret_cast<const uint4*>(tp + kGdTri) + lane;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[4][4] = {};
+        if (half == 0) tri_product<0>(x, ah, al, Pf);
+        else tri_product<4>(x, ah, al, Pf);
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+          unsigned out[4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int j = 4 * half + 2 * jp + i;
+            const float2 op = *reinterpret_cast<const float2*>(vec + kGdOp + 8 * j + 2 * c);
+            T r[4];
+            r[0] = from_f<T>(fmaf(x[2 * jp + i][0], op.x * du0, o[j][0]));
+            r[1] = from_f<T>(fmaf(x[2 * jp + i][1], op.y * du0, o[j][1]));
+            r[2] = from_f<T>(fmaf(x[2 * jp + i][2], op.x * du1, o[j][2]));
+            r[3] = from_f<T>(fmaf(x[2 * jp + i][3], op.y * du1, o[j][3]));
+            out[i] = (unsigned)__builtin_bit_cast(unsigned short, r[0]) | (unsigned)__builtin_bit_cast(unsigned short, r[1]) << 16;
+            out[2 + i] = (unsigned)__builtin_bit_cast(unsigned short, r[2]) | (unsigned)__builtin_bit_cast(unsigned short, r[3]) << 16;
+          }
+          // into the pair's own columns of V, which its chain warp has read
+          stsm4t(v_s + v_off<W>(32 * half + 16 * jp + tt, 2 * pair + tu), out);
+        }
+      }
+      __syncwarp();
+      if (active) {  // 16 rows of 32 bytes per store
+        T* og = static_cast<T*>(p.o) + ((size_t)first + (size_t)ch * kGdC) * p.ld_o + h * p.dv + row0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * i + (lane >> 1);
+          if (t < count - ch * kGdC)
+            *reinterpret_cast<uint4*>(og + (size_t)t * p.ld_o + (lane & 1) * 8) =
+                *reinterpret_cast<const uint4*>(vt + v_off<W>(t, 2 * pair + (lane & 1)));
+        }
+      }
+      bar_sync(1, NL);  // V, T, P and the factors are free: the chains left them before their u was split
+      if (ch + 1 < chunks) load_vtp(ch + 1);
+      else cp_commit();
     }
-    cp_commit();
-  };
-  auto load_vtp = [&](int ch) {  // V, T, P and the factors of chunk ch
-    const int n = count - ch * kGdC;
-    const size_t row = (size_t)first + (size_t)ch * kGdC;
-    const int units = min(16 * W, p.dv - dv0) / 8;
-    for (int i = tid; i < kGdC * 2 * W; i += NT) {
-      const int t = i / (2 * W), u = i % (2 * W);
-      const bool ok = t < n && u < units;
-      cp16(v_s + v_off<W>(t, u), static_cast<const T*>(p.v) + (ok ? (row + t) * p.ld_v + h * p.dv + dv0 + u * 8 : 0), ok);
-    }
-    const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock;
-    for (int i = tid; i < kGdBlock / 16; i += NT) cp16(tp_s + i * 16, blk + i * 16, true);
-    cp_commit();
-  };
+    cp_wait<0>();
+    return;
+  }
 
-  load_kq(0);
-  load_vtp(0);
+  // ------------------------------------------------------------------ chain warp
   float* Sg = p.state + (((size_t)slot * p.v_heads + h) * p.dv + row0 + g) * DK + 2 * c;
   float s[NK][4];
 #pragma unroll
@@ -493,30 +730,18 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     }
     s[j][0] = x.x, s[j][1] = x.y, s[j][2] = y.x, s[j][3] = y.y;
   }
-  // lane parts of the ldmatrix addresses
-  const int bt = ((lane >> 4) << 3) + (lane & 7), bu = (lane >> 3) & 1;   // B from [token][dk] rows, two n-tiles
-  const int tt = (((lane >> 3) & 1) << 3) + (lane & 7), tu = lane >> 4;   // the same, transposed
-
   for (int ch = 0; ch < chunks; ++ch) {
     const uint32_t kd = k_s + (ch & 1) * kGdC * DK * 2;
-    cp_wait<1>();
-    __syncthreads();  // K and Q are there
-    float ks[8][4], qs[8][4], up0, dn0, up1, dn1;
-    {
-      float m0 = 0.f, m1 = 0.f;
+    float up0, dn0, up1, dn1, m0 = 0.f, m1 = 0.f;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        m0 = fmaxf(m0, fmaxf(fabsf(s[j][0]), fabsf(s[j][1])));
-        m1 = fmaxf(m1, fmaxf(fabsf(s[j][2]), fabsf(s[j][3])));
-      }
-      row_scale(quad_max(m0), up0, dn0);
-      row_scale(quad_max(m1), up1, dn1);
+    for (int j = 0; j < NK; ++j) {
+      m0 = fmaxf(m0, fmaxf(fabsf(s[j][0]), fabsf(s[j][1])));
+      m1 = fmaxf(m1, fmaxf(fabsf(s[j][2]), fabsf(s[j][3])));
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ks[j][0] = ks[j][1] = ks[j][2] = ks[j][3] = 0.f;
-      qs[j][0] = qs[j][1] = qs[j][2] = qs[j][3] = 0.f;
-    }
+    row_scale(quad_max(m0), up0, dn0);
+    row_scale(quad_max(m1), up1, dn1);
+    if (ch) bar_sync(bar + 2, 64);  // the last chunk's S and u have been taken
+    float ks[8][4];
 #pragma unroll
     for (int kk = 0; kk < DK / 16; ++kk) {
       unsigned ah[4], al[4];
@@ -524,35 +749,37 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       split2(s[2 * kk][2] * up1, s[2 * kk][3] * up1, ah[1], al[1]);
       split2(s[2 * kk + 1][0] * up0, s[2 * kk + 1][1] * up0, ah[2], al[2]);
       split2(s[2 * kk + 1][2] * up1, s[2 * kk + 1][3] * up1, ah[3], al[3]);
-#pragma unroll
-      for (int jp = 0; jp < 4; ++jp) {
-        unsigned b[4], q[4];
-        ldsm4(b, kd + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
-        ldsm4(q, q_s + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
-        mma_f16(ks[2 * jp], ah[0], ah[1], ah[2], ah[3], b[0], b[1]);
-        mma_f16(ks[2 * jp + 1], ah[0], ah[1], ah[2], ah[3], b[2], b[3]);
-        mma_f16(qs[2 * jp], ah[0], ah[1], ah[2], ah[3], q[0], q[1]);
-        mma_f16(qs[2 * jp + 1], ah[0], ah[1], ah[2], ah[3], q[2], q[3]);
-        mma_f16(ks[2 * jp], al[0], al[1], al[2], al[3], b[0], b[1]);
-        mma_f16(ks[2 * jp + 1], al[0], al[1], al[2], al[3], b[2], b[3]);
-        mma_f16(qs[2 * jp], al[0], al[1], al[2], al[3], q[0], q[1]);
-        mma_f16(qs[2 * jp + 1], al[0], al[1], al[2], al[3], q[2], q[3]);
-      }
+      s_ex[(2 * kk) * 32] = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+      s_ex[(2 * kk + 1) * 32] = make_uint4(al[0], al[1], al[2], al[3]);
     }
-    cp_wait<0>();
-    __syncthreads();  // V, T and P are there; Q and the other K buffer are free
-    if (ch + 1 < chunks) load_kq(ch + 1);
-    else cp_commit();
+    if (c == 0) sc[g] = dn0, sc[g + 8] = dn1;
+    bar_sync(0, NT);  // K and Q are there
+    bar_arrive(bar, 64);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ks[j][0] = ks[j][1] = ks[j][2] = ks[j][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < DK / 16; ++kk) {
+      const uint4 hv = s_ex[(2 * kk) * 32], lv = s_ex[(2 * kk + 1) * 32];  // each lane its own
+      const unsigned ah[4] = {hv.x, hv.y, hv.z, hv.w}, al[4] = {lv.x, lv.y, lv.z, lv.w};
+      unsigned b[4][4];
+#pragma unroll
+      for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], kd + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mma_acc(ks[j], al, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mma_acc(ks[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+    }
+    bar_sync(0, NT);  // V, T and P are there
     // r = v - e^G (S k), in ks
-    float m0 = 0.f, m1 = 0.f;
+    m0 = m1 = 0.f;
 #pragma unroll
     for (int jp = 0; jp < 4; ++jp) {
       unsigned v[4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
-      ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * wid + tu));
+      ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int j = 2 * jp + i, t = 8 * j + 2 * c;
-        const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + t);
+        const int j = 2 * jp + i;
+        const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + 8 * j + 2 * c);
         const T* x = reinterpret_cast<const T*>(&v[i]);
         const T* y = reinterpret_cast<const T*>(&v[2 + i]);
         ks[j][0] = fmaf(bk.x * dn0, ks[j][0], to_f(x[0]));
@@ -561,12 +788,6 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         ks[j][3] = fmaf(bk.y * dn1, ks[j][3], to_f(y[1]));
         m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
         m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
-        // S q, complete: o = qs + P u
-        const float2 oq = *reinterpret_cast<const float2*>(vec + kGdOq + t);
-        qs[j][0] *= oq.x * dn0;
-        qs[j][1] *= oq.y * dn0;
-        qs[j][2] *= oq.x * dn1;
-        qs[j][3] *= oq.y * dn1;
       }
     }
     row_scale(quad_max(m0), up0, dn0);
@@ -586,53 +807,31 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     const uint4* Tf = reinterpret_cast<const uint4*>(tp) + lane;
     m0 = m1 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int half = 0; half < 2; ++half) {
+      float x[4][4] = {};
+      if (half == 0) tri_product<0>(x, ah, al, Tf);
+      else tri_product<4>(x, ah, al, Tf);
 #pragma unroll
-      for (int kk = 0; kk <= j / 2; ++kk) {
-        const uint4 b = Tf[gd_frag(j, kk) * 32];
-        mma_f16(x, ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], b.z, b.w);
-        mma_f16(x, al[kk][0], al[kk][1], al[kk][2], al[kk][3], b.x, b.y);
-        mma_f16(x, ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], b.x, b.y);
+      for (int i = 0; i < 4; ++i) {
+        const int j = 4 * half + i;
+        const float2 ts = *reinterpret_cast<const float2*>(vec + kGdTs + 8 * j + 2 * c);
+        ks[j][0] = x[i][0] * (ts.x * dn0);
+        ks[j][1] = x[i][1] * (ts.y * dn0);
+        ks[j][2] = x[i][2] * (ts.x * dn1);
+        ks[j][3] = x[i][3] * (ts.y * dn1);
+        m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
+        m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
       }
-      const float2 ts = *reinterpret_cast<const float2*>(vec + kGdTs + 8 * j + 2 * c);
-      ks[j][0] = x[0] * (ts.x * dn0);
-      ks[j][1] = x[1] * (ts.y * dn0);
-      ks[j][2] = x[2] * (ts.x * dn1);
-      ks[j][3] = x[3] * (ts.y * dn1);
-      m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
-      m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
     }
     row_scale(quad_max(m0), up0, dn0);
     row_scale(quad_max(m1), up1, dn1);
     split_rows(ks);
-    // o = S q + u P^T
-    const uint4* Pf = Tf + kGdFrags * 32;
 #pragma unroll
-    for (int jp = 0; jp < 4; ++jp) {
-      unsigned out[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = 2 * jp + i;
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk <= jp; ++kk) {
-          const uint4 b = Pf[gd_frag(j, kk) * 32];
-          mma_f16(x, ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], b.z, b.w);
-          mma_f16(x, al[kk][0], al[kk][1], al[kk][2], al[kk][3], b.x, b.y);
-          mma_f16(x, ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], b.x, b.y);
-        }
-        const float2 op = *reinterpret_cast<const float2*>(vec + kGdOp + 8 * j + 2 * c);
-        T r[4];
-        r[0] = from_f<T>(fmaf(x[0], op.x * dn0, qs[j][0]));
-        r[1] = from_f<T>(fmaf(x[1], op.y * dn0, qs[j][1]));
-        r[2] = from_f<T>(fmaf(x[2], op.x * dn1, qs[j][2]));
-        r[3] = from_f<T>(fmaf(x[3], op.y * dn1, qs[j][3]));
-        out[i] = *reinterpret_cast<unsigned*>(r);
-        out[2 + i] = *reinterpret_cast<unsigned*>(r + 2);
-      }
-      stsm4t(v_s + v_off<W>(16 * jp + tt, 2 * wid + tu), out);  // into this warp's columns of V, read above
+    for (int kk = 0; kk < 4; ++kk) {
+      u_ex[(2 * kk) * 32] = make_uint4(ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3]);
+      u_ex[(2 * kk + 1) * 32] = make_uint4(al[kk][0], al[kk][1], al[kk][2], al[kk][3]);
     }
+    if (c == 0) sc[16 + g] = dn0, sc[24 + g] = dn1;
     // beta e^(G_C - G) u for the state's update
     m0 = m1 = 0.f;
 #pragma unroll
@@ -645,24 +844,11 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
       m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
     }
+    const float el = vec[kGdLast];
+    bar_arrive(bar + 1, 64);  // u is split; this warp reads V, T and the factors no more
     row_scale(quad_max(m0), up0, dn0);
     row_scale(quad_max(m1), up1, dn1);
     split_rows(ks);
-    const float el = vec[kGdLast];
-    __syncwarp();
-    if (active) {  // 16 rows of 32 bytes per store
-      T* og = static_cast<T*>(p.o) + ((size_t)first + (size_t)ch * kGdC) * p.ld_o + h * p.dv + row0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * i + (lane >> 1);
-        if (t < count - ch * kGdC)
-          *reinterpret_cast<uint4*>(og + (size_t)t * p.ld_o + (lane & 1) * 8) =
-              *reinterpret_cast<const uint4*>(vt + v_off<W>(t, 2 * wid + (lane & 1)));
-      }
-    }
-    __syncthreads();  // V, T and P are free
-    if (ch + 1 < chunks) load_vtp(ch + 1);
-    else cp_commit();
     // S <- e^G_C S + u k
 #pragma unroll
     for (int jp = 0; jp < NK / 4; ++jp) {
@@ -672,14 +858,14 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         unsigned b[4], d[4];
         ldsm4t(b, kd + kq_off<DK>(16 * kk + tt, 4 * jp + tu));
         ldsm4t(d, kd + kq_off<DK>(16 * kk + tt, 4 * jp + 2 + tu));
-        mma_f16(x[0], al[kk][0], al[kk][1], al[kk][2], al[kk][3], b[0], b[1]);
-        mma_f16(x[1], al[kk][0], al[kk][1], al[kk][2], al[kk][3], b[2], b[3]);
-        mma_f16(x[2], al[kk][0], al[kk][1], al[kk][2], al[kk][3], d[0], d[1]);
-        mma_f16(x[3], al[kk][0], al[kk][1], al[kk][2], al[kk][3], d[2], d[3]);
-        mma_f16(x[0], ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], b[0], b[1]);
-        mma_f16(x[1], ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], b[2], b[3]);
-        mma_f16(x[2], ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], d[0], d[1]);
-        mma_f16(x[3], ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3], d[2], d[3]);
+        mma_acc(x[0], al[kk], b[0], b[1]);
+        mma_acc(x[1], al[kk], b[2], b[3]);
+        mma_acc(x[2], al[kk], d[0], d[1]);
+        mma_acc(x[3], al[kk], d[2], d[3]);
+        mma_acc(x[0], ah[kk], b[0], b[1]);
+        mma_acc(x[1], ah[kk], b[2], b[3]);
+        mma_acc(x[2], ah[kk], d[0], d[1]);
+        mma_acc(x[3], ah[kk], d[2], d[3]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -691,7 +877,6 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       }
     }
   }
-  cp_wait<0>();
   if (!active) return;
 #pragma unroll
   for (int j = 0; j < NK; ++j) {
