@@ -13,9 +13,11 @@
 // Precision.  The state is an fp32 result, so no product may lose more than fp32 sums do.  k and q are 16-bit
 // inputs and exact as fp16 operands (bf16 rows are brought to fp16 by a power of two per row: bf16 has
 // fewer mantissa bits, and what falls under fp16's smallest number is 2^-31 of the row's largest).  fp32
-// operands (S, r, u, T, P) are scaled by a power of two per row, so that the row's largest is in [2^13, 2^14),
-// and split in two fp16 numbers hi + lo, which keep 22 bits of what is above 2^-17 of the row's largest and
-// 2^-39 of that below; a product of two such pairs takes three MMAs (hi hi, hi lo, lo hi).  Sums run in fp32 accumulators, and the state's update in one of its own, added to the
+// operands are scaled by a power of two per row (T: for the whole matrix), so that the largest is below 2^14,
+// and split in two fp16 numbers hi + lo, which keep 22 bits of what is above 2^-17 of that and 2^-39 of it
+// below; a product of two such pairs takes three MMAs (hi hi, hi lo, lo hi).  The scales of S and P come
+// from their largest elements; those of r and u from bounds known before the products end,
+//   |r| <= max |v| + sqrt(dk) max |S| max |k|,   |u| <= max |r| max_t sum_w |T[t][w]|.  Sums run in fp32 accumulators, and the state's update in one of its own, added to the
 // decayed state with one rounding.  Decays are differences of sums in double precision: in fp32 a sum of
 // -100 already leaves e^(G_t - G_w) an error of 4e-6.
 #pragma once
@@ -26,10 +28,12 @@ namespace dfssm {
 constexpr int kGdC = 64;                // tokens per chunk
 constexpr int kGdFrags = 20;            // 8 x 16 fragments of a lower triangular 64 x 64 matrix
 constexpr int kGdTri = kGdFrags * 512;  // bytes of one such matrix as fp16 hi/lo pairs, in fragment order
-// per-token factors of a chunk, 64 floats each, then e^G_C
-enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdTs = 256, kGdLast = 320, kGdVecs = 324 };
-constexpr int kGdBlock = 2 * kGdTri + 1408;  // bytes per chunk and value head: T, P, factors
-static_assert(kGdVecs * 4 <= 1408 && kGdBlock % 128 == 0, "");
+// Factors of a chunk: per token -e^G / |k|, the update's beta e^(G_C - G) / |k| scaled to at most 1, scale e^G / |q|
+// and the inverse scale of P's row; then e^G_C, the inverse scale of T, the largest absolute row sum of T, the
+// update's scale, and the largest norm of a key.
+enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdLast = 256, kGdTdn, kGdTsum, kGdCdn, kGdKn, kGdVecs };
+constexpr int kGdBlock = 2 * kGdTri + 1152;  // bytes per chunk and value head: T, P, factors
+static_assert(kGdVecs * 4 <= 1152 && kGdBlock % 128 == 0, "");
 
 // Chunks are numbered without a plan: sequence i's chunk c is cu[i] / 64 + i + c.  That leaves at most one
 // number per sequence unused and gives no number twice.
@@ -46,13 +50,29 @@ static_assert(gd_frag(0, 0) == 0 && gd_frag(1, 0) == 1 && gd_frag(2, 0) == 2 && 
                   gd_frag(5, 0) == 9 && gd_frag(6, 0) == 12 && gd_frag(7, 3) == kGdFrags - 1, "");
 
 __device__ __forceinline__ unsigned h2_bits(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
-// two fp32 values as fp16 pairs hi + lo (22 bits)
-__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = h2_bits(h);
-  lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+// Two fp32 operations in one instruction (sm_100 packed fp32).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 dup(float x) { return make_float2(x, x); }
+// Two fp32 values as fp16 pairs hi + lo (22 bits).
+__device__ __forceinline__ void split2(float2 x, unsigned& hi, unsigned& lo) {
+  const __half2 h = __float22half2_rn(x);
+  const float2 d = fma2(__half22float2(h), dup(-1.f), x);
+  hi = h2_bits(h);
+  lo = h2_bits(__float22half2_rn(d));
+}
+__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) { split2(make_float2(x, y), hi, lo); }
 // The power of two that brings a row whose largest magnitude is m into [2^13, 2^14), and its inverse.
 __device__ __forceinline__ void row_scale(float m, float& up, float& down) {
   const int e = (int)(__float_as_uint(m) >> 23);  // m >= 0
@@ -114,7 +134,7 @@ __host__ __device__ constexpr int gd_prep_tiles() {  // K and Q; once they are m
   return 2 * kGdC * DK * 2 > kGdC * kLS * 4 ? 2 * kGdC * DK * 2 : kGdC * kLS * 4;
 }
 template <int DK>
-__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 8; }
+__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 9 + 64; }
 
 // Three TF32 MMAs for a product of fp32 values (22 bits): a, b split here.
 __device__ __forceinline__ void tf32_split2(float v, unsigned& hi, unsigned& lo) {
@@ -189,6 +209,31 @@ __device__ __forceinline__ void corner(const float* L, float* X, int o, int half
   }
 }
 
+// e^(G_t - G_w) rk_w beta_w of rows t, t + 8 and columns w, w + 1 of one diagonal block: the product of the
+// tables' factors where the block's decay stays within e^kMild, so that neither factor overflows, else an
+// exponential each.  Above the diagonal the values mean nothing (they may be infinite).
+constexpr float kMild = 40.f;
+__device__ __forceinline__ void diag_decay(float (&d)[4], bool mild, int t, int w, const double* G, const float* fk,
+                                           const float* rowd, const float* cold) {
+  if (mild) {
+    const float a = rowd[t], b = rowd[t + 8];
+    const float2 f = *reinterpret_cast<const float2*>(cold + w);
+    d[0] = a * f.x, d[1] = a * f.y, d[2] = b * f.x, d[3] = b * f.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = fk[w + (i & 1)] * expf((float)(G[t + (i & 2) * 4] - G[w + (i & 1)]));
+  }
+}
+
+// the n-tile of fragment i, three bits each
+constexpr unsigned long long frag_rows() {
+  unsigned long long v = 0;
+  for (int j = 7; j >= 0; --j)
+    for (int kk = j / 2; kk >= 0; --kk) v |= (unsigned long long)j << (3 * gd_frag(j, kk));
+  return v;
+}
+constexpr unsigned long long kFragRow = frag_rows();
+
 // kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.
 template <typename T, int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4)
@@ -207,7 +252,9 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   float* fk = rq + 64;      // rk beta
   float* rowf = fk + 64;    // e^(G_t - boundary before t's block)
   float* colf = rowf + 64;  // [3][64]: e^(boundary before block 1, 2, 3 - G_w) rk_w beta_w
-  float* up_t = colf + 192;  // the rows' scales of T
+  float* rowd = colf + 192;  // e^(G_t - last of t's block), where that is at most e^kMild
+  float* cold = rowd + 64;   // e^(last of w's block - G_w) rk_w beta_w
+  float* red = cold + 64;    // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   const int rep = p.v_heads / p.k_heads;
   const int grp = blockIdx.x % groups, hk = (blockIdx.x / groups) % p.k_heads, num = blockIdx.x / (groups * p.k_heads);
@@ -224,64 +271,72 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   if (cn < 0 || cn * kGdC >= count) return;
   first += cn * kGdC;
   count = min(count - cn * kGdC, kGdC);
-  // K and Q rows: DK / 8 lanes per row, one 16-byte unit each; the row's factor is 1 / |row| (qk_norm) times,
-  // for bf16, the power of two that undoes the staging's
+  // K and Q rows as they are, then a thread per row (64 of K, 64 of Q) for its norm and, for bf16, its fp16 form
+  const uint32_t ks = smem_u32(Ks), qs = smem_u32(Qs);
+  for (int i = tid; i < kGdC * UPR; i += kPrepThreads) {
+    const int t = i / UPR, u = i % UPR;
+    const bool ok = t < count;
+    const size_t r = (size_t)first + (ok ? t : 0);
+    cp16(ks + kq_off<DK>(t, u), static_cast<const T*>(p.k) + r * p.ld_k + hk * DK + u * 8, ok);
+    cp16(qs + kq_off<DK>(t, u), static_cast<const T*>(p.q) + r * p.ld_q + hk * DK + u * 8, ok);
+  }
+  cp_commit();
+  cp_wait<0>();
+  __syncthreads();
   {
-    constexpr int RPI = kPrepThreads / UPR;  // rows per pass
-    const int u = tid % UPR, r0 = tid / UPR;
+    const int t = tid & 63;
+    char* rowp = smem + (tid < 64 ? 0 : kGdC * DK * 2);
+    float ss = 0.f, s1 = 0.f, mx = 0.f;
+#pragma unroll 4
+    for (int u = 0; u < UPR; ++u) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(rowp + kq_off<DK>(t, u));
+      const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const T* src = static_cast<const T*>(which ? p.q : p.k) + hk * DK + u * 8;
-      const int ld = which ? p.ld_q : p.ld_k;
-      uint4 raw[kGdC / RPI];
-#pragma unroll
-      for (int i = 0; i < kGdC / RPI; ++i) {
-        const int t = r0 + i * RPI;
-        raw[i] = t < count ? *reinterpret_cast<const uint4*>(src + (size_t)(first + t) * ld) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < 8; j += 2) {
+        const float x = to_f(e[j]), y = to_f(e[j + 1]);
+        ss = fmaf(x, x, ss);
+        s1 = fmaf(y, y, s1);
+        if constexpr (BF) mx = fmaxf(mx, fmaxf(fabsf(x), fabsf(y)));
       }
+    }
+    ss += s1;
+    float factor = p.qk_norm ? 1.0f / sqrtf(ss + kQkEps) : 1.0f;
+    float kn = p.qk_norm ? 1.0f : sqrtf(ss);  // the norm that the products see
+    if constexpr (BF) {
+      float up, down;
+      row_scale(mx, up, down);
+      factor *= down;
+#pragma unroll 4
+      for (int u = 0; u < UPR; ++u) {
+        uint4* at = reinterpret_cast<uint4*>(rowp + kq_off<DK>(t, u));
+        const uint4 raw = *at;
+        const T* e = reinterpret_cast<const T*>(&raw);
+        unsigned w[4];
 #pragma unroll
-      for (int i = 0; i < kGdC / RPI; ++i) {
-        const int t = r0 + i * RPI;
-        const T* e = reinterpret_cast<const T*>(&raw[i]);
-        float factor = 1.f;
-        if (BF || p.qk_norm) {
-          float f[8], ss = 0.f, mx = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            f[j] = to_f(e[j]);
-            ss = fmaf(f[j], f[j], ss);
-            if constexpr (BF) mx = fmaxf(mx, fabsf(f[j]));
-          }
-#pragma unroll
-          for (int o = UPR / 2; o > 0; o >>= 1) {
-            ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if constexpr (BF) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          }
-          if (p.qk_norm) factor = 1.0f / sqrtf(ss + kQkEps);
-          if constexpr (BF) {
-            float up, down;
-            row_scale(mx, up, down);
-            factor *= down;
-            uint4 out;
-            unsigned* ow = reinterpret_cast<unsigned*>(&out);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ow[j] = h2_bits(__floats2half2_rn(f[2 * j] * up, f[2 * j + 1] * up));
-            raw[i] = out;
-            if (grp == 0)
-              *reinterpret_cast<uint4*>(kq16 + ((((size_t)num * p.k_heads + hk) * 2 + which) * kGdC + t) * DK + u * 8) = out;
-          }
-        }
-        *reinterpret_cast<uint4*>(reinterpret_cast<char*>(which ? Qs : Ks) + kq_off<DK>(t, u)) = raw[i];
-        if (u == 0) (which ? rq : rk)[t] = factor;
+        for (int j = 0; j < 4; ++j) w[j] = h2_bits(__floats2half2_rn(to_f(e[2 * j]) * up, to_f(e[2 * j + 1]) * up));
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
       }
+    }
+    if (tid < 64) {
+      rk[t] = factor;
+      kn = warp_max(kn);
+      if (lane == 0) red[8 + wid] = kn;
+    } else {
+      rq[t] = factor;
     }
   }
   __syncthreads();
+  if (BF && grp == 0) {
+    __half* dst = kq16 + ((size_t)num * p.k_heads + hk) * 2 * kGdC * DK;
+    for (int i = tid; i < 2 * kGdC * UPR; i += kPrepThreads) {
+      const int t = i / UPR, u = i % UPR;  // rows 64.. are Q's: its tile follows K's here too
+      *reinterpret_cast<uint4*>(dst + (size_t)i * 8) = *reinterpret_cast<const uint4*>(smem + (t >> 6) * kGdC * DK * 2 + kq_off<DK>(t & 63, u));
+    }
+  }
   // Q K^T rows 16 wid.. and K K^T rows 16 (3 - wid)..: ten 16 x 8 tiles for every warp
   const int mk = 3 - wid;
   float qk[8][4], kk_[8][4];
   {
-    const uint32_t ks = smem_u32(Ks), qs = smem_u32(Qs);
     auto gram = [&](uint32_t a_tile, int mt, float (&acc)[8][4]) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -333,19 +388,29 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
     float* vec = reinterpret_cast<float*>(blk + 2 * kGdTri);
     {
       const int t = tid & 63;
-      const double Gt = G[t];
+      const double Gt = G[t], Ge = G[t | 15];  // of the token, and of the last in its block of 16
       if (tid < 64) {  // factors of the chunk kernel
-        const float eg = expf((float)Gt);
+        const float eg = expf((float)Gt), c2 = expf((float)(G[63] - Gt)) * fk[t];
         vec[kGdBk + t] = -eg * rk[t];
-        vec[kGdC2 + t] = expf((float)(G[63] - Gt)) * fk[t];
         vec[kGdOq + t] = p.scale * eg * rq[t];
-        if (t == 0) vec[kGdLast] = expf((float)G[63]);
-        if (t < 32) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
+        if (t == 0) vec[kGdLast] = expf((float)G[63]), vec[kGdKn] = fmaxf(red[8], red[9]);
+        const float m = warp_max(fabsf(c2));
+        if (lane == 0) red[10 + wid] = m;
+        colf[128 + t] = c2;  // kept here until both warps' largest is known; e^(boundary 3 - G) follows
+        rowd[t] = expf(fminf((float)(Gt - Ge), kMild));
       } else {  // factors of this one
         if (t >= 16) rowf[t] = expf((float)(Gt - G[(t & ~15) - 1]));
         if (t < 16) colf[t] = expf((float)(G[15] - Gt)) * fk[t];
         if (t < 32) colf[64 + t] = expf((float)(G[31] - Gt)) * fk[t];
-        else if (t < 48) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
+        cold[t] = expf((float)(Ge - Gt)) * fk[t];
+      }
+      __syncthreads();
+      if (tid < 64) {
+        float up, down;
+        row_scale(fmaxf(red[10], red[11]), up, down);
+        vec[kGdC2 + t] = colf[128 + t] * (up * 0x1p-14f);
+        if (t == 0) vec[kGdCdn] = down * 0x1p14f;
+        if (t < 48) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
       }
     }
     __syncthreads();
@@ -370,15 +435,17 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
           }
         }
       }
-      const double Ga = G[ta], Gb = G[tb];
+      const bool mild = G[16 * wid] - G[16 * wid + 15] <= (double)kMild;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (j == 2 * wid || j == 2 * wid + 1) {
+          float d[4];
+          diag_decay(d, mild, ta, 8 * j + 2 * c, G, fk, rowd, cold);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int w = 8 * j + 2 * c + i;
-            x[j][i] = w <= ta ? qk[j][i] * ra * (fk[w] * expf((float)(Ga - G[w]))) : 0.f;
-            x[j][2 + i] = w <= tb ? qk[j][2 + i] * rb * (fk[w] * expf((float)(Gb - G[w]))) : 0.f;
+            x[j][i] = w <= ta ? qk[j][i] * ra * d[i] : 0.f;
+            x[j][2 + i] = w <= tb ? qk[j][2 + i] * rb * d[2 + i] : 0.f;
             ma = fmaxf(ma, fabsf(x[j][i]));
             mb = fmaxf(mb, fabsf(x[j][2 + i]));
           }
@@ -421,16 +488,15 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
           }
         }
       }
-      const double Ga = G[ta], Gb = G[tb];
+      const bool mild = G[16 * mk] - G[16 * mk + 15] <= (double)kMild;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (j == 2 * mk || j == 2 * mk + 1) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int w = 8 * j + 2 * c + i;
-            L[ta * kLS + w] = w < ta ? kk_[j][i] * ra * (fk[w] * expf((float)(Ga - G[w]))) : 0.f;
-            L[tb * kLS + w] = w < tb ? kk_[j][2 + i] * rb * (fk[w] * expf((float)(Gb - G[w]))) : 0.f;
-          }
+          const int w = 8 * j + 2 * c;  // only what is left of the diagonal is read
+          float d[4];
+          diag_decay(d, mild, ta, w, G, fk, rowd, cold);
+          *reinterpret_cast<float2*>(L + ta * kLS + w) = make_float2(kk_[j][0] * ra * d[0], kk_[j][1] * ra * d[1]);
+          *reinterpret_cast<float2*>(L + tb * kLS + w) = make_float2(kk_[j][2] * rb * d[2], kk_[j][3] * rb * d[3]);
         }
       }
       __syncwarp();
@@ -460,38 +526,37 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
     __syncthreads();
     corner<32>(L, X, 0, wid >> 1, wid & 1, lane);
     __syncthreads();
-    {  // the rows' scales
+    {  // the scale of T and its largest row sum
       const int t = tid >> 1, half = tid & 1;
-      float m = 0.f;
+      float m = 0.f, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 32; w += 4) {
         if (32 * half + w <= t) {
           const float4 x = *reinterpret_cast<const float4*>(X + t * kLS + 32 * half + w);
           m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+          sum += (fabsf(x.x) + fabsf(x.y)) + (fabsf(x.z) + fabsf(x.w));
         }
       }
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      float up, down;
-      row_scale(m, up, down);
-      if (half == 0) {
-        up_t[t] = up;
-        vec[kGdTs + t] = down;
-      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      m = warp_max_nonneg(m);
+      sum = warp_max_nonneg(sum);
+      if (lane == 0) red[wid] = m, red[4 + wid] = sum;
     }
     __syncthreads();
+    float t_up, t_down;
+    row_scale(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), t_up, t_down);
+    if (tid == 0) {
+      vec[kGdTdn] = t_down;
+      vec[kGdTsum] = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+    }
 #pragma unroll
     for (int f = 0; f < kGdFrags / 4; ++f) {  // fragment 4 f + wid
       const int id = 4 * f + wid;
-      int j = 0;
-#pragma unroll
-      for (int x = 1; x < 8; ++x) j += id >= gd_frag(x, 0);
-      const int kk = id - gd_frag(j, 0), t = 8 * j + g;
-      const float up = up_t[t];
-      const float2 x = *reinterpret_cast<const float2*>(X + t * kLS + 16 * kk + 2 * c);
-      const float2 y = *reinterpret_cast<const float2*>(X + t * kLS + 16 * kk + 2 * c + 8);
+      const int j = (int)(kFragRow >> (3 * id)) & 7, kk = id - gd_frag(j, 0);
+      const float* x = X + (8 * j + g) * kLS + 16 * kk + 2 * c;
       unsigned h0, l0, h1, l1;
-      split2(x.x * up, x.y * up, h0, l0);
-      split2(y.x * up, y.y * up, h1, l1);
+      split2(mul2(*reinterpret_cast<const float2*>(x), dup(t_up)), h0, l0);
+      split2(mul2(*reinterpret_cast<const float2*>(x + 8), dup(t_up)), h1, l1);
       reinterpret_cast<uint4*>(blk)[id * 32 + lane] = make_uint4(h0, h1, l0, l1);
     }
     // the next head's gates touch nothing that is still read: G and the factors were last used before
@@ -504,20 +569,23 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 // A pair of warps owns 16 rows of one head's state.  The first, the chain warp, holds S^T as MMA accumulators
 // (64 registers per thread at dk = 128) and computes what the next chunk waits for: S k, r, u, the new S.  The
 // second, the output warp, takes the operands that the first has split anyway (S and u as fp16 pairs, through
-// shared memory) and computes S q + u P^T and the rows of o; it also fetches the next chunk (cp.async).  All
-// products are taken transposed, with S, r and u as left operands: the accumulator layout of one product is
-// the left operand's layout of the next, so nothing of the chain itself passes through shared memory.
+// shared memory) and computes S q + u P^T and the rows of o; it also fetches the next chunk (cp.async): K is
+// double buffered, and Q, V, T, P and the factors are replaced as soon as they have been read, so that two
+// blocks of two pairs fit on an SM.  All products are taken transposed, with S, r and u as left operands: the
+// accumulator layout of one product is the left operand's layout of the next, so nothing of the chain itself
+// passes through shared memory.
 //   S k, S q : [16 x dk] [dk x 64]     u = r T^T, u P^T : [16 x 64] [64 x 64]     u k : [16 x 64] [64 x dk]
-// K is double buffered; Q, V, T, P and the factors of the next chunk are fetched while the products that do
-// not read them run.
+// The splits of one product's operands are written among the MMAs of the one before it or of its own earlier
+// steps, so that a single warp keeps its tensor core busy.
 //
-// Bound: the chain of a chunk is 316 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM) and
-// the splits between them, one after the other; a second pair per scheduler fills the gaps when there are
-// enough sequences and heads.
+// Bound: the chain of a chunk is 316 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM), one
+// after the other; the output warp's 188 run beside them.
 
+template <int DK>
+__host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 128; }
 template <int DK, int W>
 __host__ __device__ constexpr int gd_chunk_smem() {
-  return 3 * kGdC * DK * 2 + kGdC * 32 * W + kGdBlock + W * (DK / 16 * 1024 + 4096 + 128);
+  return 3 * kGdC * DK * 2 + kGdC * 32 * W + kGdBlock + W * gd_exchange<DK>();
 }
 
 // Byte offset of 16-byte unit u of token t in the V tile [64][16 W].
@@ -526,7 +594,7 @@ __device__ __forceinline__ uint32_t v_off(int t, int u) {
   const int f = W >= 4 ? (t & 7) : (W == 2 ? ((t >> 1) & 3) : ((t >> 2) & 1));
   return (uint32_t)(t * 32 * W + ((u ^ f) << 4));
 }
-// Named barriers: 0 the block, 1 the output warps, 2 + 3 pair + {0: S is split, 1: u is split, 2: both are read}
+// Named barriers: 0 the block, 1 the output warps, 2 + 2 pair + {0: u is split, 1: S and u have been taken}
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -534,7 +602,7 @@ __device__ __forceinline__ void bar_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// x[j] += rows of (ah + al) times the 64 x 64 triangular matrix in fragment order, for n-tiles J0 .. J0 + 3
+// x[i] += rows of (ah + al) times the 64 x 64 triangular matrix in fragment order, for n-tiles J0 + i
 template <int J0>
 __device__ __forceinline__ void tri_product(float (&x)[4][4], const unsigned (&ah)[4][4], const unsigned (&al)[4][4],
                                             const uint4* F) {
@@ -555,6 +623,25 @@ __device__ __forceinline__ void tri_product(float (&x)[4][4], const unsigned (&a
       if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk], b[i].x, b[i].y);
   }
 }
+// One k-step's left operand from two neighbouring accumulator tiles, rows scaled by f0 (rows g) and f1 (g + 8).
+__device__ __forceinline__ void split_tile(const float (&x)[4], const float (&y)[4], float f0, float f1, unsigned (&ah)[4],
+                                           unsigned (&al)[4]) {
+  split2(mul2(make_float2(x[0], x[1]), dup(f0)), ah[0], al[0]);
+  split2(mul2(make_float2(x[2], x[3]), dup(f1)), ah[1], al[1]);
+  split2(mul2(make_float2(y[0], y[1]), dup(f0)), ah[2], al[2]);
+  split2(mul2(make_float2(y[2], y[3]), dup(f1)), ah[3], al[3]);
+}
+// Largest magnitude of two pairs of 16-bit values.
+__device__ __forceinline__ float pair_max(unsigned a, unsigned b, __half) {
+  const __half2 x = __habs2(*reinterpret_cast<__half2*>(&a)), y = __habs2(*reinterpret_cast<__half2*>(&b));
+  const float2 f = __half22float2(__hmax2(x, y));
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ float pair_max(unsigned a, unsigned b, __nv_bfloat16) {
+  const __nv_bfloat162 x = __habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), y = __habs2(*reinterpret_cast<__nv_bfloat162*>(&b));
+  const float2 f = __bfloat1622float2(__hmax2(x, y));
+  return fmaxf(f.x, f.y);
+}
 
 // kq16: the fp16 tiles of K and Q for bf16 inputs; for fp16 inputs the tiles are rows of k and q themselves.
 template <typename T, int DK, int W>
@@ -563,58 +650,59 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
                          int parts, int slots_total) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int NT = 64 * W, NL = 32 * W, NK = DK / 8, UPR = DK / 8;
+  constexpr int TILE = kGdC * DK * 2, V_AT = 3 * TILE, B_AT = V_AT + kGdC * 32 * W;  // K, K, Q, V, {T, P, factors}
   extern __shared__ __align__(128) char smem[];
-  char* vt = smem + 3 * kGdC * DK * 2;
-  char* tp = vt + kGdC * 32 * W;
-  const float* vec = reinterpret_cast<const float*>(tp + 2 * kGdTri);
-  const uint32_t k_s = smem_u32(smem), q_s = k_s + 2 * kGdC * DK * 2, v_s = smem_u32(vt), tp_s = smem_u32(tp);
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   const int part = blockIdx.x % parts, h = (blockIdx.x / parts) % p.v_heads, seq = blockIdx.x / (parts * p.v_heads);
-  const int slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
-  if (slot < 0) return;
   int first, count;
   gd_range(p.cu, seq, p.tokens, first, count);
-  if (count == 0) return;
   const int base = gd_chunk_base(p.cu, seq, p.tokens);
+  // Two blocks of two pairs share an SM's four schedulers: the one in the upper warp slots swaps its roles, so that
+  // each scheduler gets a chain and an output warp and not two of a kind (only speed depends on it).
+  __shared__ int upper;
+  if (W == 2 && tid == 0) {
+    unsigned w;
+    asm volatile("mov.u32 %0, %%warpid;" : "=r"(w));
+    upper = (w >> 2) & 1;
+  }
+  const int slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
+  __syncthreads();
+  if (slot < 0 || count == 0) return;
   const int chunks = min((count + kGdC - 1) / kGdC, slots_total - base);
   const int hk = h / (p.v_heads / p.k_heads);
-  const bool chain = wid < W;
-  const int pair = chain ? wid : wid - W;
+  const bool chain = W == 2 ? (wid < W) != (upper != 0) : wid < W;
+  const int pair = wid % W;
   const int dv0 = part * 16 * W, row0 = dv0 + 16 * pair;
   const bool active = row0 < p.dv;  // dv is a multiple of 16: a pair's rows are all there or none
-  char* ex = tp + kGdBlock + pair * (DK / 16 * 1024 + 4096 + 128);
-  uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;                           // S: [dk / 16][hi, lo][32]
-  uint4* u_ex = reinterpret_cast<uint4*>(ex + DK / 16 * 1024) + lane;          // u: [4][hi, lo][32]
-  float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);            // [2][16] the rows' scales
-  const int bar = 2 + 3 * pair;
+  char* ex = smem + B_AT + kGdBlock + pair * gd_exchange<DK>();
+  uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;                   // S: [dk / 16][hi, lo][32]
+  uint4* u_ex = reinterpret_cast<uint4*>(ex + DK / 16 * 1024) + lane;  // u: [4][hi, lo][32]
+  float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);    // [2][16] the rows' scales
+  const int bar = 2 + 2 * pair;
+  const uint32_t q_s = smem_u32(smem) + 2 * TILE, v_s = smem_u32(smem) + V_AT;
+  const float* vec = reinterpret_cast<const float*>(smem + B_AT + 2 * kGdTri);
   // lane parts of the ldmatrix addresses
   const int bt = ((lane >> 4) << 3) + (lane & 7), bu = (lane >> 3) & 1;  // B from [token][dk] rows, two n-tiles
   const int tt = (((lane >> 3) & 1) << 3) + (lane & 7), tu = lane >> 4;  // the same, transposed
 
   if (!chain) {
     // ---------------------------------------------------------------- output warp
-    const int lt = tid - NL;
-    auto load_kq = [&](int ch) {  // K and Q of chunk ch
+    const int lt = tid % NL;
+    auto load_tile = [&](int ch, uint32_t dst, const void* rows, int ld, int which) {  // K (0) or Q (1) of chunk ch
       const int n = count - ch * kGdC;
-      const uint32_t kd = k_s + (ch & 1) * kGdC * DK * 2;
-      const size_t row = (size_t)first + (size_t)ch * kGdC;
+      const __half* src;
+      if constexpr (BF) src = kq16 + (((size_t)(base + ch) * p.k_heads + hk) * 2 + which) * kGdC * DK;
+      else src = static_cast<const __half*>(rows) + ((size_t)first + (size_t)ch * kGdC) * ld + hk * DK;
 #pragma unroll 4
       for (int i = lt; i < kGdC * UPR; i += NL) {
         const int t = i / UPR, u = i % UPR;
-        if constexpr (BF) {
-          const __half* src = kq16 + (((size_t)(base + ch) * p.k_heads + hk) * 2 * kGdC + t) * DK + u * 8;
-          cp16(kd + kq_off<DK>(t, u), src, true);
-          cp16(q_s + kq_off<DK>(t, u), src + kGdC * DK, true);
-        } else {
-          const bool ok = t < n;
-          const size_t r = ok ? row + t : row;
-          cp16(kd + kq_off<DK>(t, u), static_cast<const __half*>(p.k) + r * p.ld_k + hk * DK + u * 8, ok);
-          cp16(q_s + kq_off<DK>(t, u), static_cast<const __half*>(p.q) + r * p.ld_q + hk * DK + u * 8, ok);
-        }
+        if constexpr (BF) cp16(dst + kq_off<DK>(t, u), src + i * 8, true);
+        else cp16(dst + kq_off<DK>(t, u), src + (t < n ? (size_t)t * ld : 0) + u * 8, t < n);
       }
-      cp_commit();
     };
-    auto load_vtp = [&](int ch) {  // V, T, P and the factors of chunk ch
+    auto load_k = [&](int ch) { load_tile(ch, smem_u32(smem) + (ch & 1) * TILE, p.k, p.ld_k, 0); };
+    auto load_q = [&](int ch) { load_tile(ch, q_s, p.q, p.ld_q, 1); };
+    auto load_vb = [&](int ch) {  // V, T, P and the factors of chunk ch
       const int n = count - ch * kGdC;
       const size_t row = (size_t)first + (size_t)ch * kGdC;
       const int units = min(16 * W, p.dv - dv0) / 8;
@@ -626,15 +714,21 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       }
       const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock;
 #pragma unroll 4
-      for (int i = lt; i < kGdBlock / 16; i += NL) cp16(tp_s + i * 16, blk + i * 16, true);
-      cp_commit();
+      for (int i = lt; i < kGdBlock / 16; i += NL) cp16(smem_u32(smem) + B_AT + i * 16, blk + i * 16, true);
     };
-    load_kq(0);
-    load_vtp(0);
+    load_k(0);
+    load_q(0);
+    cp_commit();
+    load_vb(0);
+    cp_commit();
     for (int ch = 0; ch < chunks; ++ch) {
+      const bool more = ch + 1 < chunks;
       cp_wait<1>();
-      bar_sync(0, NT);  // K and Q are there
-      bar_sync(bar, 64);
+      bar_sync(0, NT);  // K and Q are there, and nobody reads the other K any more
+      if (more) load_k(ch + 1);
+      cp_commit();
+      cp_wait<1>();
+      bar_sync(0, NT);  // V, T, P and the factors are there, and the chains have split S
       float o[8][4];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -651,11 +745,9 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         for (int j = 0; j < 8; ++j) mma_acc(o[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
       }
       const float ds0 = sc[g], ds1 = sc[g + 8];
-      bar_sync(1, NL);  // Q is free, and the other K buffer, which the chains left before they split S
-      if (ch + 1 < chunks) load_kq(ch + 1);
-      else cp_commit();
-      cp_wait<1>();
-      bar_sync(0, NT);  // V, T and P are there
+      bar_sync(1, NL);  // Q is free
+      if (more) load_q(ch + 1);
+      cp_commit();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float2 oq = *reinterpret_cast<const float2*>(vec + kGdOq + 8 * j + 2 * c);
@@ -664,7 +756,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         o[j][2] *= oq.x * ds1;
         o[j][3] *= oq.y * ds1;
       }
-      bar_sync(bar + 1, 64);
+      bar_sync(bar, 64);
       unsigned ah[4][4], al[4][4];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
@@ -673,8 +765,8 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         al[kk][0] = lv.x, al[kk][1] = lv.y, al[kk][2] = lv.z, al[kk][3] = lv.w;
       }
       const float du0 = sc[16 + g], du1 = sc[24 + g];
-      if (ch + 1 < chunks) bar_arrive(bar + 2, 64);
-      const uint4* Pf = reinterpret_cast<const uint4*>(tp + kGdTri) + lane;
+      if (more) bar_arrive(bar + 1, 64);
+      const uint4* Pf = reinterpret_cast<const uint4*>(smem + B_AT + kGdTri) + lane;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float x[4][4] = {};
@@ -707,12 +799,12 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
           const int t = 16 * i + (lane >> 1);
           if (t < count - ch * kGdC)
             *reinterpret_cast<uint4*>(og + (size_t)t * p.ld_o + (lane & 1) * 8) =
-                *reinterpret_cast<const uint4*>(vt + v_off<W>(t, 2 * pair + (lane & 1)));
+                *reinterpret_cast<const uint4*>(smem + V_AT + v_off<W>(t, 2 * pair + (lane & 1)));
         }
       }
       bar_sync(1, NL);  // V, T, P and the factors are free: the chains left them before their u was split
-      if (ch + 1 < chunks) load_vtp(ch + 1);
-      else cp_commit();
+      if (more) load_vb(ch + 1);
+      cp_commit();
     }
     cp_wait<0>();
     return;
@@ -720,7 +812,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
 
   // ------------------------------------------------------------------ chain warp
   float* Sg = p.state + (((size_t)slot * p.v_heads + h) * p.dv + row0 + g) * DK + 2 * c;
-  float s[NK][4];
+  float s[NK][4], m0 = 0.f, m1 = 0.f;  // the state and its rows' largest magnitudes
 #pragma unroll
   for (int j = 0; j < NK; ++j) {
     float2 x = make_float2(0.f, 0.f), y = x;
@@ -729,135 +821,108 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       y = *reinterpret_cast<const float2*>(Sg + 8 * DK + 8 * j);
     }
     s[j][0] = x.x, s[j][1] = x.y, s[j][2] = y.x, s[j][3] = y.y;
+    m0 = fmaxf(m0, fmaxf(fabsf(x.x), fabsf(x.y)));
+    m1 = fmaxf(m1, fmaxf(fabsf(y.x), fabsf(y.y)));
   }
   for (int ch = 0; ch < chunks; ++ch) {
-    const uint32_t kd = k_s + (ch & 1) * kGdC * DK * 2;
-    float up0, dn0, up1, dn1, m0 = 0.f, m1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      m0 = fmaxf(m0, fmaxf(fabsf(s[j][0]), fabsf(s[j][1])));
-      m1 = fmaxf(m1, fmaxf(fabsf(s[j][2]), fabsf(s[j][3])));
-    }
-    row_scale(quad_max(m0), up0, dn0);
-    row_scale(quad_max(m1), up1, dn1);
-    if (ch) bar_sync(bar + 2, 64);  // the last chunk's S and u have been taken
+    const uint32_t k_s = smem_u32(smem) + (ch & 1) * TILE;
+    m0 = quad_max(m0);
+    m1 = quad_max(m1);
+    float up0, dn0, up1, dn1;
+    row_scale(m0, up0, dn0);
+    row_scale(m1, up1, dn1);
+    if (ch) bar_sync(bar + 1, 64);  // the last chunk's S and u have been taken
+    if (c == 0) sc[g] = dn0, sc[g + 8] = dn1;
+    unsigned sh[2][4], sl[2][4];
+    split_tile(s[0], s[1], up0, up1, sh[0], sl[0]);
+    bar_sync(0, NT);  // K and Q are there
     float ks[8][4];
 #pragma unroll
-    for (int kk = 0; kk < DK / 16; ++kk) {
-      unsigned ah[4], al[4];
-      split2(s[2 * kk][0] * up0, s[2 * kk][1] * up0, ah[0], al[0]);
-      split2(s[2 * kk][2] * up1, s[2 * kk][3] * up1, ah[1], al[1]);
-      split2(s[2 * kk + 1][0] * up0, s[2 * kk + 1][1] * up0, ah[2], al[2]);
-      split2(s[2 * kk + 1][2] * up1, s[2 * kk + 1][3] * up1, ah[3], al[3]);
-      s_ex[(2 * kk) * 32] = make_uint4(ah[0], ah[1], ah[2], ah[3]);
-      s_ex[(2 * kk + 1) * 32] = make_uint4(al[0], al[1], al[2], al[3]);
-    }
-    if (c == 0) sc[g] = dn0, sc[g + 8] = dn1;
-    bar_sync(0, NT);  // K and Q are there
-    bar_arrive(bar, 64);
-#pragma unroll
     for (int j = 0; j < 8; ++j) ks[j][0] = ks[j][1] = ks[j][2] = ks[j][3] = 0.f;
+    // S k, the next step's split between the MMAs of this one
 #pragma unroll
     for (int kk = 0; kk < DK / 16; ++kk) {
-      const uint4 hv = s_ex[(2 * kk) * 32], lv = s_ex[(2 * kk + 1) * 32];  // each lane its own
-      const unsigned ah[4] = {hv.x, hv.y, hv.z, hv.w}, al[4] = {lv.x, lv.y, lv.z, lv.w};
       unsigned b[4][4];
 #pragma unroll
-      for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], kd + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
+      for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], k_s + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
+      const int now = kk & 1;
+      s_ex[(2 * kk) * 32] = make_uint4(sh[now][0], sh[now][1], sh[now][2], sh[now][3]);
+      s_ex[(2 * kk + 1) * 32] = make_uint4(sl[now][0], sl[now][1], sl[now][2], sl[now][3]);
+      if (kk + 1 < DK / 16) split_tile(s[2 * kk + 2], s[2 * kk + 3], up0, up1, sh[now ^ 1], sl[now ^ 1]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mma_acc(ks[j], al, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+      for (int j = 0; j < 8; ++j) mma_acc(ks[j], sl[now], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mma_acc(ks[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+      for (int j = 0; j < 8; ++j) mma_acc(ks[j], sh[now], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
     }
-    bar_sync(0, NT);  // V, T and P are there
-    // r = v - e^G (S k), in ks
-    m0 = m1 = 0.f;
+    bar_sync(0, NT);  // V, T, P and the factors are there; S is split
+    // bounds of r and u, and the scales from them
+    unsigned v[4][4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
+    float v0 = 0.f, v1 = 0.f;
 #pragma unroll
     for (int jp = 0; jp < 4; ++jp) {
-      unsigned v[4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
-      ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
+      ldsm4t(v[jp], v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
+      v0 = fmaxf(v0, pair_max(v[jp][0], v[jp][1], T()));
+      v1 = fmaxf(v1, pair_max(v[jp][2], v[jp][3], T()));
+    }
+    const float root = DK == 128 ? 11.3137085f : 8.f;
+    const float r0 = fmaf(root * vec[kGdKn], m0, quad_max(v0)), r1 = fmaf(root * vec[kGdKn], m1, quad_max(v1));
+    float ur0, dr0, ur1, dr1, uu0, du0, uu1, du1;
+    row_scale(r0, ur0, dr0);
+    row_scale(r1, ur1, dr1);
+    row_scale(r0 * vec[kGdTsum], uu0, du0);
+    row_scale(r1 * vec[kGdTsum], uu1, du1);
+    const float tdn = vec[kGdTdn], el = vec[kGdLast], cdn = vec[kGdCdn];
+    // r = v - e^G (S k), in ks, split as the left operand of u = r T^T
+    unsigned ah[4][4], al[4][4];
+#pragma unroll
+    for (int jp = 0; jp < 4; ++jp) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = 2 * jp + i;
         const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + 8 * j + 2 * c);
-        const T* x = reinterpret_cast<const T*>(&v[i]);
-        const T* y = reinterpret_cast<const T*>(&v[2 + i]);
-        ks[j][0] = fmaf(bk.x * dn0, ks[j][0], to_f(x[0]));
-        ks[j][1] = fmaf(bk.y * dn0, ks[j][1], to_f(x[1]));
-        ks[j][2] = fmaf(bk.x * dn1, ks[j][2], to_f(y[0]));
-        ks[j][3] = fmaf(bk.y * dn1, ks[j][3], to_f(y[1]));
-        m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
-        m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
+        const T* x = reinterpret_cast<const T*>(&v[jp][i]);
+        const T* y = reinterpret_cast<const T*>(&v[jp][2 + i]);
+        const float2 a = fma2(mul2(bk, dup(dn0)), make_float2(ks[j][0], ks[j][1]), make_float2(to_f(x[0]), to_f(x[1])));
+        const float2 b = fma2(mul2(bk, dup(dn1)), make_float2(ks[j][2], ks[j][3]), make_float2(to_f(y[0]), to_f(y[1])));
+        ks[j][0] = a.x, ks[j][1] = a.y, ks[j][2] = b.x, ks[j][3] = b.y;
       }
+      split_tile(ks[2 * jp], ks[2 * jp + 1], ur0, ur1, ah[jp], al[jp]);
     }
-    row_scale(quad_max(m0), up0, dn0);
-    row_scale(quad_max(m1), up1, dn1);
-    unsigned ah[4][4], al[4][4];
-    auto split_rows = [&](const float (&x)[8][4]) {
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        split2(x[2 * kk][0] * up0, x[2 * kk][1] * up0, ah[kk][0], al[kk][0]);
-        split2(x[2 * kk][2] * up1, x[2 * kk][3] * up1, ah[kk][1], al[kk][1]);
-        split2(x[2 * kk + 1][0] * up0, x[2 * kk + 1][1] * up0, ah[kk][2], al[kk][2]);
-        split2(x[2 * kk + 1][2] * up1, x[2 * kk + 1][3] * up1, ah[kk][3], al[kk][3]);
-      }
+    const uint4* Tf = reinterpret_cast<const uint4*>(smem + B_AT) + lane;
+    float x0[4][4] = {}, x1[4][4] = {};  // u, scaled as r and T are
+    tri_product<0>(x0, ah, al, Tf);
+    tri_product<4>(x1, ah, al, Tf);
+    // beta e^(G_C - G) u, the left operand of the state's update
+    const float fu0 = dr0 * uu0 * tdn, fu1 = dr1 * uu1 * tdn;
+    auto weigh = [&](const float (&x)[4], int j, float (&y)[4]) {
+      const float2 c2 = *reinterpret_cast<const float2*>(vec + kGdC2 + 8 * j + 2 * c);
+      const float2 a = mul2(make_float2(x[0], x[1]), c2), b = mul2(make_float2(x[2], x[3]), c2);
+      y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
     };
-    split_rows(ks);
-    // u = r T^T, in ks
-    const uint4* Tf = reinterpret_cast<const uint4*>(tp) + lane;
-    m0 = m1 = 0.f;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float x[4][4] = {};
-      if (half == 0) tri_product<0>(x, ah, al, Tf);
-      else tri_product<4>(x, ah, al, Tf);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * half + i;
-        const float2 ts = *reinterpret_cast<const float2*>(vec + kGdTs + 8 * j + 2 * c);
-        ks[j][0] = x[i][0] * (ts.x * dn0);
-        ks[j][1] = x[i][1] * (ts.y * dn0);
-        ks[j][2] = x[i][2] * (ts.x * dn1);
-        ks[j][3] = x[i][3] * (ts.y * dn1);
-        m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
-        m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
-      }
-    }
-    row_scale(quad_max(m0), up0, dn0);
-    row_scale(quad_max(m1), up1, dn1);
-    split_rows(ks);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      u_ex[(2 * kk) * 32] = make_uint4(ah[kk][0], ah[kk][1], ah[kk][2], ah[kk][3]);
-      u_ex[(2 * kk + 1) * 32] = make_uint4(al[kk][0], al[kk][1], al[kk][2], al[kk][3]);
+      float y[2][4];
+      weigh(kk < 2 ? x0[2 * kk] : x1[2 * kk - 4], 2 * kk, y[0]);
+      weigh(kk < 2 ? x0[2 * kk + 1] : x1[2 * kk - 3], 2 * kk + 1, y[1]);
+      split_tile(y[0], y[1], fu0, fu1, ah[kk], al[kk]);
     }
-    if (c == 0) sc[16 + g] = dn0, sc[24 + g] = dn1;
-    // beta e^(G_C - G) u for the state's update
+    // S <- e^G_C S + u k, and u for the output warp between the first MMAs
+    const float ds0 = du0 * cdn, ds1 = du1 * cdn;
     m0 = m1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 c2 = *reinterpret_cast<const float2*>(vec + kGdC2 + 8 * j + 2 * c);
-      ks[j][0] *= c2.x;
-      ks[j][1] *= c2.y;
-      ks[j][2] *= c2.x;
-      ks[j][3] *= c2.y;
-      m0 = fmaxf(m0, fmaxf(fabsf(ks[j][0]), fabsf(ks[j][1])));
-      m1 = fmaxf(m1, fmaxf(fabsf(ks[j][2]), fabsf(ks[j][3])));
-    }
-    const float el = vec[kGdLast];
-    bar_arrive(bar + 1, 64);  // u is split; this warp reads V, T and the factors no more
-    row_scale(quad_max(m0), up0, dn0);
-    row_scale(quad_max(m1), up1, dn1);
-    split_rows(ks);
-    // S <- e^G_C S + u k
 #pragma unroll
     for (int jp = 0; jp < NK / 4; ++jp) {
       float x[4][4] = {};
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         unsigned b[4], d[4];
-        ldsm4t(b, kd + kq_off<DK>(16 * kk + tt, 4 * jp + tu));
-        ldsm4t(d, kd + kq_off<DK>(16 * kk + tt, 4 * jp + 2 + tu));
+        ldsm4t(b, k_s + kq_off<DK>(16 * kk + tt, 4 * jp + tu));
+        ldsm4t(d, k_s + kq_off<DK>(16 * kk + tt, 4 * jp + 2 + tu));
+        if (jp == 0) {
+          unsigned uh[4], ul[4];
+          split_tile(kk < 2 ? x0[2 * kk] : x1[2 * kk - 4], kk < 2 ? x0[2 * kk + 1] : x1[2 * kk - 3], fu0, fu1, uh, ul);
+          u_ex[(2 * kk) * 32] = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+          u_ex[(2 * kk + 1) * 32] = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+        }
         mma_acc(x[0], al[kk], b[0], b[1]);
         mma_acc(x[1], al[kk], b[2], b[3]);
         mma_acc(x[2], al[kk], d[0], d[1]);
@@ -867,13 +932,18 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         mma_acc(x[2], ah[kk], d[0], d[1]);
         mma_acc(x[3], ah[kk], d[2], d[3]);
       }
+      if (jp == 0) {
+        if (c == 0) sc[16 + g] = du0, sc[24 + g] = du1;
+        bar_arrive(bar, 64);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float(&z)[4] = s[4 * jp + i];
-        z[0] = fmaf(el, z[0], x[i][0] * dn0);
-        z[1] = fmaf(el, z[1], x[i][1] * dn0);
-        z[2] = fmaf(el, z[2], x[i][2] * dn1);
-        z[3] = fmaf(el, z[3], x[i][3] * dn1);
+        const float2 a = fma2(dup(el), make_float2(z[0], z[1]), mul2(make_float2(x[i][0], x[i][1]), dup(ds0)));
+        const float2 b = fma2(dup(el), make_float2(z[2], z[3]), mul2(make_float2(x[i][2], x[i][3]), dup(ds1)));
+        z[0] = a.x, z[1] = a.y, z[2] = b.x, z[3] = b.y;
+        m0 = fmaxf(m0, fmaxf(fabsf(a.x), fabsf(a.y)));
+        m1 = fmaxf(m1, fmaxf(fabsf(b.x), fabsf(b.y)));
       }
     }
   }
