@@ -186,11 +186,7 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
   fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, groups, per_group);
   DFSSM_CU(cudaGetLastError());
-  static const int force = getenv("DFSSM_GD_W") ? atoi(getenv("DFSSM_GD_W")) : 0;
-  switch (force ? force : 4) {
-    case 4: return launch_walk<T, DK, 4>(p, workspace, kq16, (int)n, s);
-    default: return launch_walk<T, DK, 2>(p, workspace, kq16, (int)n, s);
-  }
+  return launch_walk<T, DK, 2>(p, workspace, kq16, (int)n, s);
 }
 
 // What both entry points ask of their arguments.

@@ -90,13 +90,14 @@ __device__ __forceinline__ void mma_acc(float (&d)[4], const unsigned (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Ordered among themselves and with the barriers (volatile), free to move among ordinary loads.
 __device__ __forceinline__ void ldsm4(unsigned (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void ldsm4t(unsigned (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void stsm4t(uint32_t addr, const unsigned (&r)[4]) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
@@ -582,7 +583,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 // after the other; the output warp's 188 run beside them.
 
 template <int DK>
-__host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 128; }
+__host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 192; }
 template <int DK, int W>
 __host__ __device__ constexpr int gd_chunk_smem() {
   return 3 * kGdC * DK * 2 + kGdC * 32 * W + kGdBlock + W * gd_exchange<DK>();
@@ -677,7 +678,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   char* ex = smem + B_AT + kGdBlock + pair * gd_exchange<DK>();
   uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;                   // S: [dk / 16][hi, lo][32]
   uint4* u_ex = reinterpret_cast<uint4*>(ex + DK / 16 * 1024) + lane;  // u: [4][hi, lo][32]
-  float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);    // [2][16] the rows' scales
+  float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);    // [3][16] the rows' scales of S and u, and max |v|
   const int bar = 2 + 2 * pair;
   const uint32_t q_s = smem_u32(smem) + 2 * TILE, v_s = smem_u32(smem) + V_AT;
   const float* vec = reinterpret_cast<const float*>(smem + B_AT + 2 * kGdTri);
@@ -687,34 +688,52 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
 
   if (!chain) {
     // ---------------------------------------------------------------- output warp
+    // A lane copies one 16-byte column of every RP-th row (K, Q), so that a copy costs a pointer step; rows past
+    // the sequence's end are zeros.
     const int lt = tid % NL;
+    constexpr int RP = NL / UPR;  // rows per pass: 4 to 16
+    const uint32_t sm0 = smem_u32(smem);
+    const int kt = lt / UPR, ku = lt % UPR;
+    const uint32_t off0 = kq_off<DK>(kt, ku), off1 = kq_off<DK>(kt + RP, ku) - RP * DK * 2;  // even and odd passes
     auto load_tile = [&](int ch, uint32_t dst, const void* rows, int ld, int which) {  // K (0) or Q (1) of chunk ch
       const int n = count - ch * kGdC;
       const __half* src;
-      if constexpr (BF) src = kq16 + (((size_t)(base + ch) * p.k_heads + hk) * 2 + which) * kGdC * DK;
-      else src = static_cast<const __half*>(rows) + ((size_t)first + (size_t)ch * kGdC) * ld + hk * DK;
-#pragma unroll 4
-      for (int i = lt; i < kGdC * UPR; i += NL) {
-        const int t = i / UPR, u = i % UPR;
-        if constexpr (BF) cp16(dst + kq_off<DK>(t, u), src + i * 8, true);
-        else cp16(dst + kq_off<DK>(t, u), src + (t < n ? (size_t)t * ld : 0) + u * 8, t < n);
+      size_t step;
+      if constexpr (BF) {
+        src = kq16 + ((((size_t)(base + ch) * p.k_heads + hk) * 2 + which) * kGdC + kt) * DK + ku * 8;
+        step = RP * DK;
+      } else {
+        src = static_cast<const __half*>(rows) + ((size_t)first + (size_t)ch * kGdC + kt) * ld + hk * DK + ku * 8;
+        step = (size_t)RP * ld;
+      }
+      if (BF || n >= kGdC) {
+#pragma unroll
+        for (int i = 0; i < kGdC / RP; ++i, src += step) cp16(dst + i * (RP * DK * 2) + ((i & 1) ? off1 : off0), src, true);
+      } else {
+        for (int i = 0; i < kGdC / RP; ++i, src += step) {
+          const bool ok = kt + i * RP < n;
+          cp16(dst + i * (RP * DK * 2) + ((i & 1) ? off1 : off0), ok ? src : static_cast<const __half*>(rows), ok);
+        }
       }
     };
-    auto load_k = [&](int ch) { load_tile(ch, smem_u32(smem) + (ch & 1) * TILE, p.k, p.ld_k, 0); };
+    auto load_k = [&](int ch) { load_tile(ch, sm0 + (ch & 1) * TILE, p.k, p.ld_k, 0); };
     auto load_q = [&](int ch) { load_tile(ch, q_s, p.q, p.ld_q, 1); };
+    const int vu = lt % (2 * W), vt = lt / (2 * W);  // 16 rows of V per pass
+    const bool v_there = dv0 + vu * 8 < p.dv;
     auto load_vb = [&](int ch) {  // V, T, P and the factors of chunk ch
       const int n = count - ch * kGdC;
-      const size_t row = (size_t)first + (size_t)ch * kGdC;
-      const int units = min(16 * W, p.dv - dv0) / 8;
+      const T* src = static_cast<const T*>(p.v) + ((size_t)first + (size_t)ch * kGdC + vt) * p.ld_v + h * p.dv + dv0 + vu * 8;
 #pragma unroll
-      for (int i = lt; i < kGdC * 2 * W; i += NL) {
-        const int t = i / (2 * W), u = i % (2 * W);
-        const bool ok = t < n && u < units;
-        cp16(v_s + v_off<W>(t, u), static_cast<const T*>(p.v) + (ok ? (row + t) * p.ld_v + h * p.dv + dv0 + u * 8 : 0), ok);
+      for (int i = 0; i < 4; ++i, src += (size_t)16 * p.ld_v) {
+        const bool ok = v_there && vt + 16 * i < n;
+        cp16(v_s + v_off<W>(vt + 16 * i, vu), ok ? src : static_cast<const T*>(p.v), ok);
       }
-      const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock;
-#pragma unroll 4
-      for (int i = lt; i < kGdBlock / 16; i += NL) cp16(smem_u32(smem) + B_AT + i * 16, blk + i * 16, true);
+      const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock + lt * 16;
+      const uint32_t dst = sm0 + B_AT + lt * 16;
+#pragma unroll
+      for (int i = 0; i < kGdBlock / 16 / NL; ++i) cp16(dst + i * NL * 16, blk + i * NL * 16, true);
+      constexpr int REST = kGdBlock / 16 % NL;
+      if (lt < REST) cp16(dst + kGdBlock / 16 / NL * NL * 16, blk + kGdBlock / 16 / NL * NL * 16, true);
     };
     load_k(0);
     load_q(0);
@@ -728,7 +747,21 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       if (more) load_k(ch + 1);
       cp_commit();
       cp_wait<1>();
-      bar_sync(0, NT);  // V, T, P and the factors are there, and the chains have split S
+      bar_sync(1, NL);  // V, T, P and the factors are there
+      {  // the largest |v| of each row, for the chain's bound of r
+        float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+        for (int jp = 0; jp < 4; ++jp) {
+          unsigned v[4];
+          ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
+          v0 = fmaxf(v0, pair_max(v[0], v[1], T()));
+          v1 = fmaxf(v1, pair_max(v[2], v[3], T()));
+        }
+        v0 = quad_max(v0);
+        v1 = quad_max(v1);
+        if (c == 0) sc[32 + g] = v0, sc[40 + g] = v1;
+      }
+      bar_sync(0, NT);  // the chains have split S; V, T, P and the factors are there for them too
       float o[8][4];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -856,16 +889,8 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     }
     bar_sync(0, NT);  // V, T, P and the factors are there; S is split
     // bounds of r and u, and the scales from them
-    unsigned v[4][4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
-    float v0 = 0.f, v1 = 0.f;
-#pragma unroll
-    for (int jp = 0; jp < 4; ++jp) {
-      ldsm4t(v[jp], v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
-      v0 = fmaxf(v0, pair_max(v[jp][0], v[jp][1], T()));
-      v1 = fmaxf(v1, pair_max(v[jp][2], v[jp][3], T()));
-    }
     const float root = DK == 128 ? 11.3137085f : 8.f;
-    const float r0 = fmaf(root * vec[kGdKn], m0, quad_max(v0)), r1 = fmaf(root * vec[kGdKn], m1, quad_max(v1));
+    const float r0 = fmaf(root * vec[kGdKn], m0, sc[32 + g]), r1 = fmaf(root * vec[kGdKn], m1, sc[40 + g]);
     float ur0, dr0, ur1, dr1, uu0, du0, uu1, du1;
     row_scale(r0, ur0, dr0);
     row_scale(r1, ur1, dr1);
@@ -876,12 +901,14 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     unsigned ah[4][4], al[4][4];
 #pragma unroll
     for (int jp = 0; jp < 4; ++jp) {
+      unsigned v[4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
+      ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = 2 * jp + i;
         const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + 8 * j + 2 * c);
-        const T* x = reinterpret_cast<const T*>(&v[jp][i]);
-        const T* y = reinterpret_cast<const T*>(&v[jp][2 + i]);
+        const T* x = reinterpret_cast<const T*>(&v[i]);
+        const T* y = reinterpret_cast<const T*>(&v[2 + i]);
         const float2 a = fma2(mul2(bk, dup(dn0)), make_float2(ks[j][0], ks[j][1]), make_float2(to_f(x[0]), to_f(x[1])));
         const float2 b = fma2(mul2(bk, dup(dn1)), make_float2(ks[j][2], ks[j][3]), make_float2(to_f(y[0]), to_f(y[1])));
         ks[j][0] = a.x, ks[j][1] = a.y, ks[j][2] = b.x, ks[j][3] = b.y;
