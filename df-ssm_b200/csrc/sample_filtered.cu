@@ -8,9 +8,22 @@
 // T <= 0 takes the first token.  NaN and -inf logits are never taken; tokens at +inf share the row.
 //
 // Which token is drawn must not depend on how the sums were split, so weights are 64-bit integers: exp in
-// double precision times 2^S with S = 62 - ceil(log2 V), rounded.  Their sums are exact in any order, and
-// the rounding moves a boundary by about sqrt(V) 2^-S of the largest weight, some 1e-12, where fp32 sums
+// double precision times 2^S with S = min(50, 62 - ceil(log2 V)), rounded.  Their sums are exact in any order,
+// and the rounding moves a boundary by about sqrt(V) 2^-S of the largest weight, some 1e-12, where fp32 sums
 // would move it by 1e-7 and pick other tokens once in a thousand rows.
+//
+// One block of 1024 threads per row, the row's x in shared memory where it fits (V up to about 50,000; else
+// every pass reads the logits again, from L2).  No pass sorts or selects over the whole row:
+//   - with top-k, the k-th largest of the threads' own largest values bounds the k-th largest x from below;
+//     the few tokens above it go to a list that is sorted, and the rest of the row is not looked at again;
+//   - with top-p alone, tokens of weight below (1 - top_p) sum / V together weigh too little to hold the
+//     boundary; a histogram over the others (1024 bins of x) finds its bin, whose tokens are sorted;
+//   - the result of either is a cut {x, how many of the tokens equal to it stay}.
+// Rows where the list would overflow (thousands of equal logits at the cut, top_k in the thousands) select the
+// cut by four rounds over 8 bits of x's order-preserving key instead.
+//
+// Bound: 64-bit floating point where a whole row needs its weights (10 operations a token), else the first
+// pass over the logits.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -20,6 +33,9 @@ namespace dfssm {
 
 constexpr int kSfThreads = 1024;
 constexpr int kSfWarps = kSfThreads / 32;
+constexpr int kSfList = 2048;  // tokens that are sorted
+constexpr int kSfBins = 1024;  // one per thread
+constexpr int kSfAll = 0x7fffffff;
 
 typedef unsigned long long u64;
 
@@ -33,82 +49,338 @@ struct SampleArgs {
   float rep;
   int *next, *kept;
   float* prob;
-  double unit;  // 2^S
+  int shift;      // S
+  int in_shared;  // x of the row in shared memory
 };
 
 __device__ __forceinline__ float sf_logit(const float* p) { return *p; }
 __device__ __forceinline__ float sf_logit(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float sf_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// Order-preserving key of x; 0 for NaN and -inf, which are never taken.
+// Order-preserving key of x; 0 for -inf (and NaN), which is never taken.
 __device__ __forceinline__ uint32_t sf_key(float x) {
   if (!(x > -INFINITY)) return 0u;
   const uint32_t u = __float_as_uint(x + 0.0f);  // -0 counts as 0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float sf_unkey(uint32_t k) {
+  if (k == 0u) return -INFINITY;
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
+// A row's x.  from4 computes four of them from the logits: divided by T with the rounding of an IEEE division
+// (two corrections bring q within an ulp of l / T and then, Markstein, to the rounded quotient, as long as
+// nothing under- or overflows; -inf, NaN and large negative logits end as NaN on the way, which fmaxf turns
+// into -inf; zero, tiny and large positive ones take the division itself).  -inf stands for every token
+// that cannot be taken.
 template <typename T>
 struct Row {
   const T* l;
   const uint32_t* seen;
-  float temp, rep;
-  __device__ __forceinline__ uint32_t key(int i) const {
-    float x = __fdiv_rn(sf_logit(l + i), temp);
-    if (seen && ((seen[i >> 5] >> (i & 31)) & 1u)) x = __fdiv_rn(x, rep);
-    return sf_key(x);
+  const float* xs;  // the row's x in shared memory, or NULL: every pass computes them again
+  int V;
+  float temp, rtemp, rep;
+  bool divide, mild, aligned;  // aligned: four logits at a time
+  bool lift;                   // the row's largest x is +inf: tokens there count as 0, all others as -inf
+  __device__ __forceinline__ float4 from4(float4 v, int i) const {
+    float* e = reinterpret_cast<float*>(&v);
+    if (divide) {
+      bool odd = !mild;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd |= e[j] > 0x1p100f || fabsf(e[j]) < 0x1p-79f;
+      if (odd) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = __fdiv_rn(e[j], temp);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float q = __fmul_rn(e[j], rtemp);
+          q = __fmaf_rn(__fmaf_rn(-q, temp, e[j]), rtemp, q);
+          e[j] = __fmaf_rn(__fmaf_rn(-q, temp, e[j]), rtemp, q);
+        }
+      }
+    }
+    if (seen) {
+      const uint32_t bits = seen[i >> 5] >> (i & 31);  // i is a multiple of 4
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((bits >> j) & 1u) e[j] = __fdiv_rn(e[j], rep);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = fmaxf(e[j], -INFINITY);
+    return v;
+  }
+  // logits i .. i + 3 (i a multiple of 4, i < V), -inf behind the row's end
+  __device__ __forceinline__ float4 logits4(int i) const {
+    float4 v;
+    if (aligned && i + 4 <= V) {
+      if constexpr (sizeof(T) == 4) {
+        v = *reinterpret_cast<const float4*>(l + i);
+      } else {
+        const uint2 raw = *reinterpret_cast<const uint2*>(l + i);
+        const T* e = reinterpret_cast<const T*>(&raw);
+        v = make_float4(sf_logit(e), sf_logit(e + 1), sf_logit(e + 2), sf_logit(e + 3));
+      }
+    } else {
+      v.x = sf_logit(l + i);
+      v.y = i + 1 < V ? sf_logit(l + i + 1) : -INFINITY;
+      v.z = i + 2 < V ? sf_logit(l + i + 2) : -INFINITY;
+      v.w = i + 3 < V ? sf_logit(l + i + 3) : -INFINITY;
+    }
+    return v;
+  }
+  __device__ __forceinline__ float4 x4(int i) const {
+    float4 v = xs ? *reinterpret_cast<const float4*>(xs + i) : from4(logits4(i), i);
+    if (lift) {
+      v.x = v.x == INFINITY ? 0.f : -INFINITY;
+      v.y = v.y == INFINITY ? 0.f : -INFINITY;
+      v.z = v.z == INFINITY ? 0.f : -INFINITY;
+      v.w = v.w == INFINITY ? 0.f : -INFINITY;
+    }
+    return v;
+  }
+  // f(x, index) for four tokens at a time
+  template <typename F>
+  __device__ __forceinline__ void each4(F f) const {
+    for (int i = 4 * threadIdx.x; i < V; i += 4 * kSfThreads) {
+      const float4 v = x4(i);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      f(x, i);
+    }
+  }
+  // f(x, index) for every token; behind the row's end x is -inf
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = 4 * threadIdx.x; i < V; i += 4 * kSfThreads) {
+      const float4 v = x4(i);
+      f(v.x, i);
+      f(v.y, i + 1);
+      f(v.z, i + 2);
+      f(v.w, i + 3);
+    }
   }
 };
 
-// w of a key as a double in [0, 1]
-__device__ __forceinline__ double sf_weight(uint32_t key, uint32_t top) {
-  if (key == top) return 1.0;
-  return key == 0u ? 0.0 : exp((double)sf_unkey(key) - (double)sf_unkey(top));
-}
-__device__ __forceinline__ u64 sf_fix(double w, double unit) { return (u64)__double2ll_rn(w * unit); }
+// Weights: exp(x - m) by table and polynomial (Tang's scheme): x - m = n ln2 / 64 + r, |r| <= ln2 / 128,
+// exp = 2^(n / 64) (1 + r + r^2/2 + r^3/6 + r^4/24), off by 4e-14; the table holds 2^(S + j / 64).  No branches:
+// tokens beyond `far`, whose weight rounds to 0, are computed and dropped.  A row whose largest x is
+// +inf comes lifted: its tokens there as 0 and the others as -inf.
+struct Weigh {
+  const double* table;
+  double m;
+  float top, far;  // the largest x, and the distance from it beyond which a weight rounds to 0
+  __device__ __forceinline__ double scaled(float x) const {  // w 2^S
+    const double magic = 6755399441055744.0;  // 1.5 2^52: the sum's low word is the rounded integer
+    const double t = (double)x - m, z = fma(t, 92.33248261689366, magic);
+    const int n = __double2loint(z);
+    const double r = fma(z - magic, -0.010830424696249145, t);
+    double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    p *= table[n & 63];
+    const double w = __hiloint2double(__double2hiint(p) + (n & ~63) * (1 << 14), __double2loint(p));
+    return top - x < far ? w : 0.0;
+  }
+  // v rounded to an integer, as the low bits of a double in [2^52, 2^53): sums of these patterns are sums of the
+  // integers plus kBias each (modulo 2^64).
+  static constexpr u64 kBias = 0x4330000000000000ull;
+  static __device__ __forceinline__ u64 biased(double v) { return (u64)__double_as_longlong(v + 4503599627370496.0); }
+  static __device__ __forceinline__ u64 fix(double v) { return biased(v) - kBias; }  // v < 2^51
+  __device__ __forceinline__ u64 of(float x) const { return fix(scaled(x)); }
+};
 
-__device__ __forceinline__ u64 sf_block_sum(u64 v, u64* red) {
+// Adds a weight to a bin's two words in shared memory (64-bit shared atomics are loops).
+__device__ __forceinline__ void add_weight(unsigned* lo, unsigned* hi, u64 w) {
+  const unsigned wl = (unsigned)w, old = atomicAdd(lo, wl);
+  const unsigned wh = (unsigned)(w >> 32) + (old + wl < old ? 1u : 0u);
+  if (wh) atomicAdd(hi, wh);
+}
+
+// The last kept token of the order: its x, and how many of the tokens with that x stay (lowest indices first).
+struct Cut {
+  float x;
+  int ties;
+};
+
+struct Shared {
+  u64 red[kSfWarps];
+  int ired[kSfWarps];
+  float fred[kSfWarps];
+  double table[64];
+  u64 found;
+  int count, pick;
+};
+
+// Block-wide reductions and an exclusive scan, the same value in every thread.
+template <typename V>
+__device__ __forceinline__ V sf_sum(V v, V* red) {
   v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  u64 s = 0;
-  for (int j = 0; j < kSfWarps; ++j) s += red[j];
-  return s;
+  return warp_sum(red[threadIdx.x & 31]);
+}
+__device__ __forceinline__ float sf_max(float v, float* red) {
+  v = warp_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_max(red[threadIdx.x & 31]);
+}
+__device__ __forceinline__ u64 sf_scan(u64 v, u64* red, u64& total) {  // sum over the threads before this one
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  u64 upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  __syncthreads();
+  if (lane == 31) red[wid] = upto;
+  __syncthreads();
+  u64 w = red[lane], wupto = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, wupto, o);
+    if (lane >= o) wupto += x;
+  }
+  total = __shfl_sync(0xffffffffu, wupto, 31);
+  return __shfl_sync(0xffffffffu, wupto - w, wid) + upto - v;
 }
 
-// The last kept token of the order, as (key, how many of the tokens with that key stay).
-struct Cut {
-  uint32_t key;
-  int ties;
-};
+// From one value per warp in red[]: the sum over the warps before `wid`, and over all.
+template <typename V>
+__device__ __forceinline__ V sf_warps(const V* red, int wid, V& total) {
+  const int lane = threadIdx.x & 31;
+  const V own = red[lane];
+  V upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  total = __shfl_sync(0xffffffffu, upto, 31);
+  return __shfl_sync(0xffffffffu, upto - own, wid);
+}
 
-// Finds the group of equal keys in which the budget (a count, or a weight) runs out, among the keys >= floor:
-// four rounds over 8 bits of the key, each a histogram of the keys that share the digits found so far.
-// by_weight: a token stays while the weight before it is <= budget; else `budget` tokens stay.
-// Returns {floor_key, floor_ties} when the budget outlasts all of them.
+// Adds the tokens of a warp's tile that `take` accepts to the warp's pool (64 floats, `have` in use) and runs
+// use(x) whenever 32 are there.
+template <typename F, typename G>
+__device__ __forceinline__ void sf_pool(float* pool, int& have, const float4& v, F take, G use) {
+  const int lane = threadIdx.x & 31;
+  const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool in = take(x[j]);
+    const unsigned all = __ballot_sync(0xffffffffu, in);
+    if (all) {
+      if (in) pool[have + __popc(all & ((1u << lane) - 1))] = x[j];
+      have += __popc(all);
+      if (have >= 32) {
+        __syncwarp();
+        use(pool[lane]);
+        have -= 32;
+        const float rest = pool[32 + lane];
+        __syncwarp();
+        pool[lane] = rest;
+        __syncwarp();
+      }
+    }
+  }
+}
+
+// Runs `use(x)` on every token that `take` accepts, 32 at a time: a warp collects what its lanes' tiles have in
+// its pool, so that a few tokens among many cost few warp-wide evaluations.  use() is called by
+// whole warps, with -inf in the lanes of a last, partly filled round.
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void sf_dense(const Row<T>& row, float* pool, F take, G use) {
+  const int lane = threadIdx.x & 31;
+  int have = 0;
+  for (int i0 = 4 * (threadIdx.x - lane); i0 < row.V; i0 += 4 * kSfThreads) {
+    const int i = i0 + 4 * lane;
+    sf_pool(pool, have, i < row.V ? row.x4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), take, use);
+  }
+  __syncwarp();
+  if (have) use(lane < have ? pool[lane] : -INFINITY);
+}
+
+// Descending bitonic sort of list[0..n), n <= kSfList, padded with zeros to a power of two, by half as many
+// threads as there are entries; begins and ends with a block barrier.
+__device__ void sf_sort(u64* list, int n) {
+  int size = 64;
+  while (size < n) size <<= 1;
+  __syncthreads();
+  const int t = threadIdx.x, workers = size / 2;
+  if (t < workers) {
+    for (int i = n + t; i < size; i += workers) list[i] = 0ull;
+    auto meet = [&] {
+      if (workers == 32) __syncwarp();
+      else asm volatile("bar.sync 1, %0;" ::"r"(workers) : "memory");
+    };
+    meet();
+    for (int k = 2; k <= size; k <<= 1) {
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const int i = 2 * t - (t & (j - 1)), o = i + j;  // pairs at distance j
+        const u64 a = list[i], b = list[o];
+        if ((a < b) == ((i & k) == 0)) list[i] = b, list[o] = a;
+        if (j > 32 || (j == 1 && k >= 64)) meet();  // pairs at distances up to 32 stay within a warp's 64 entries
+        else __syncwarp();
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// Appends the tokens that `take` accepts (none at -inf) to the list as {key of x, complement of the index};
+// returns how many there are, which may be more than were stored.
+template <typename T, typename F>
+__device__ int sf_gather(const Row<T>& row, u64* list, int* count, F take) {
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int i0 = 4 * (threadIdx.x - lane); i0 < row.V; i0 += 4 * kSfThreads) {
+    const int i = i0 + 4 * lane;
+    const float4 v = i < row.V ? row.x4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    bool in[4], any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) any |= in[j] = take(x[j]);
+    if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned all = __ballot_sync(0xffffffffu, in[j]);
+      if (!all) continue;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(count, __popc(all));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
+      if (in[j] && at < kSfList) list[at] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
+    }
+  }
+  __syncthreads();
+  return *count;
+}
+
+// The cut by four rounds over 8 bits of the key, for what does not fit the list.  by_weight: a token stays while
+// the weight before it is <= budget; else `budget` tokens stay.  Looks at the tokens that `floor` keeps and
+// returns it when the budget outlasts them.
 template <typename T>
-__device__ Cut sf_cut(const Row<T>& row, int V, uint32_t top, Cut fl, bool by_weight, u64 budget, double unit,
-                      unsigned* cnt, unsigned* lo, unsigned* hi) {
+__device__ __noinline__ Cut sf_radix_cut(const Row<T>& row, const Weigh& weigh, Cut floor, bool by_weight, u64 budget,
+                                         unsigned* cnt, unsigned* lo, unsigned* hi) {
+  const uint32_t least = max(sf_key(floor.x), 1u);
   uint32_t prefix = 0;
   u64 used = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
     for (int i = threadIdx.x; i < 256; i += kSfThreads) cnt[i] = lo[i] = hi[i] = 0u;
     __syncthreads();
-    for (int i = threadIdx.x; i < V; i += kSfThreads) {
-      const uint32_t k = row.key(i);
-      if (k == 0u || k < fl.key || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
+    row.each([&](float x, int) {
+      const uint32_t k = sf_key(x);
+      if (k < least || (shift < 24 && (k >> (shift + 8)) != prefix)) return;
       const int d = (k >> shift) & 255;
       atomicAdd(cnt + d, 1u);
-      if (by_weight) {
-        const u64 w = sf_fix(sf_weight(k, top), unit);
-        const unsigned wl = (unsigned)w, old = atomicAdd(lo + d, wl);
-        const unsigned wh = (unsigned)(w >> 32) + (old + wl < old ? 1u : 0u);
-        if (wh) atomicAdd(hi + d, wh);
-      }
-    }
+      if (by_weight) add_weight(lo + d, hi + d, weigh.of(x));
+    });
     __syncthreads();
     int d = 255;  // every thread walks the digits from the top; all come to the same one
     for (; d >= 0; --d) {
@@ -116,49 +388,75 @@ __device__ Cut sf_cut(const Row<T>& row, int V, uint32_t top, Cut fl, bool by_we
       if (cnt[d] && (by_weight ? used + m > budget : used + m >= budget)) break;
       used += m;
     }
+    const int here = d < 0 ? 0 : (int)cnt[d];
     __syncthreads();
-    if (d < 0) return fl;
+    if (d < 0) return floor;
     prefix = (prefix << 8) | (uint32_t)d;
     if (shift == 0) {
-      const int n = prefix == fl.key ? fl.ties : (int)cnt[d];
-      int stay;
-      if (by_weight) {
-        const u64 w = sf_fix(sf_weight(prefix, top), unit);
-        stay = w == 0 ? n : (int)min((u64)n, (budget - used) / w + 1);
-      } else {
-        stay = (int)(budget - used);
-      }
-      __syncthreads();
-      return Cut{prefix, min(stay, n)};
+      const float x = sf_unkey(prefix);
+      const int n = x == floor.x ? min(floor.ties, here) : here;
+      if (!by_weight) return Cut{x, min(n, (int)(budget - used))};
+      const u64 w = weigh.of(x);
+      return Cut{x, w == 0 ? n : (int)min((u64)n, (budget - used) / w + 1)};
     }
   }
-  return fl;
+  return floor;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const SampleArgs p) {
-  __shared__ unsigned cnt[256], lo[256], hi[256];
-  __shared__ u64 red[kSfWarps];
-  __shared__ int ties_of[kSfWarps];
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ Shared sh;
+  u64* list = reinterpret_cast<u64*>(dyn);  // [kSfList]; the histogram's counts and weights before it is filled
+  unsigned* cnt = reinterpret_cast<unsigned*>(dyn);
+  unsigned *lo = cnt + kSfBins, *hi = lo + kSfBins;
+  float* pool = reinterpret_cast<float*>(list + kSfList) + (threadIdx.x >> 5) * 64;  // one per warp
+  float* xs = reinterpret_cast<float*>(list + kSfList) + kSfWarps * 64;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, V = p.vocab;
   Row<T> row;
   row.l = static_cast<const T*>(p.logits) + (long long)b * p.ld;
   row.seen = p.seen ? p.seen + (size_t)b * ((V + 31) / 32) : nullptr;
-  row.rep = p.rep;
+  row.xs = nullptr;
+  row.V = V;
+  row.lift = false;
+  row.aligned = (reinterpret_cast<uintptr_t>(row.l) & (4 * sizeof(T) - 1)) == 0;
   const float temp = p.temperature ? p.temperature[b] : 1.0f;
   const bool greedy = !(temp > 0.f);
   row.temp = greedy ? 1.0f : temp;
+  row.rep = p.rep;
+  row.rtemp = __frcp_rn(row.temp);
+  row.divide = row.temp != 1.f;
+  row.mild = row.temp > 0x1p-20f && row.temp < 0x1p20f;
   const int k = greedy ? 1 : (p.top_k ? p.top_k[b] : 0);
   const float top_p = p.top_p ? p.top_p[b] : 1.0f, min_p = p.min_p ? p.min_p[b] : 0.f;
-  // the largest key
-  uint32_t top = 0;
-  for (int i = tid; i < V; i += kSfThreads) top = max(top, row.key(i));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) cnt[wid] = top;
-  __syncthreads();
-  for (int j = 0; j < kSfWarps; ++j) top = max(top, cnt[j]);
-  __syncthreads();
-  if (top == 0u) {  // nothing to take in this row
+  float u = p.uniform[b];
+  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+
+  // ---- x of the row, each thread's largest, the row's largest
+  float mine2[2] = {-INFINITY, -INFINITY};  // of the thread's tokens, split in two
+  constexpr int kAhead = 4;
+  for (int i0 = 4 * tid; i0 < V; i0 += kAhead * 4 * kSfThreads) {
+    float4 v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * 4 * kSfThreads;
+      if (i < V) v[j] = row.logits4(i);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * 4 * kSfThreads;
+      if (i < V) {
+        const float4 x = row.from4(v[j], i);
+        if (p.in_shared) *reinterpret_cast<float4*>(xs + i) = x;
+        mine2[j & 1] = fmaxf(mine2[j & 1], fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+      }
+    }
+  }
+  if (p.in_shared) row.xs = xs;
+  const float mine = fmaxf(mine2[0], mine2[1]);
+  if (tid < 64) sh.table[tid] = ldexp(exp2(tid / 64.0), p.shift);
+  float top = sf_max(mine, sh.fred);
+  if (top == -INFINITY) {  // nothing to take in this row
     if (tid == 0) {
       p.next[b] = -1;
       if (p.kept) p.kept[b] = 0;
@@ -166,84 +464,366 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
     }
     return;
   }
-  Cut cut{1u, 0x7fffffff};
-  if (k > 0 && k < V) cut = sf_cut(row, V, top, cut, false, (u64)k, p.unit, cnt, lo, hi);
-  if (top_p < 1.f) {
-    u64 m = 0;
-    for (int i = tid; i < V; i += kSfThreads) {
-      const uint32_t key = row.key(i);
-      if (key > cut.key) m += sf_fix(sf_weight(key, top), p.unit);
+  if (k == 1) {  // the first token of the order
+    if (tid == 0) sh.pick = V;
+    __syncthreads();
+    if (mine == top) row.each([&](float x, int i) { if (x == top) atomicMin(&sh.pick, i); });
+    __syncthreads();
+    if (tid == 0) {
+      p.next[b] = sh.pick;
+      if (p.kept) p.kept[b] = 1;
+      if (p.prob) p.prob[b] = 1.f;
     }
-    m = sf_block_sum(m, red);
-    if (cut.ties != 0x7fffffff) m += (u64)cut.ties * sf_fix(sf_weight(cut.key, top), p.unit);
-    const u64 budget = (u64)(fmax((double)top_p, 0.0) * (double)m);
-    cut = sf_cut(row, V, top, cut, true, budget, p.unit, cnt, lo, hi);
+    return;
   }
-  // the draw: every warp owns a run of the vocabulary
-  const int run = (V + kSfThreads - 1) / kSfThreads * 32, i0 = min(V, wid * run), i1 = min(V, i0 + run);
-  auto weight = [&](uint32_t key) -> double {  // negative: not kept by key and min_p
-    if (key < cut.key || key == 0u) return -1.0;
-    const double w = sf_weight(key, top);
-    return (key == top || w >= (double)min_p) ? w : -1.0;
+  if (top == INFINITY) {
+    row.lift = true;
+    top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) mine2[e] = mine2[e] == INFINITY ? 0.f : -INFINITY;
+  }
+  const Weigh weigh{sh.table, (double)top, top, (p.shift + 1) * 0.69314718f + 0.5f};
+  const double unit = sh.table[0], least = (double)min_p * unit;
+  Cut cut{-INFINITY, kSfAll};
+  bool open_p = top_p < 1.f;  // top-p is still to be applied
+
+  if (k > 0 && k < V) {
+    // ---- top-k: a lower bound of the k-th largest x, the tokens from there on sorted
+    const uint32_t key0 = sf_key(mine2[0]), key1 = sf_key(mine2[1]), keys = max(key0, key1);
+    uint32_t low = 0u, high = sf_key(top);
+    if (k <= 2 * kSfThreads) {
+      // the largest key that at least k of the threads' largest reach (for larger k of both their halves), or
+      // one that few more do
+      const bool halves = k > kSfThreads / 4;
+      const uint32_t all = __reduce_min_sync(0xffffffffu, halves ? min(key0, key1) : keys);
+      if (lane == 0) sh.ired[wid] = (int)all;
+      __syncthreads();
+      low = __reduce_min_sync(0xffffffffu, (unsigned)sh.ired[lane]);
+      while (low < high) {
+        const uint32_t mid = low + (high - low + 1) / 2;
+        const int n = halves ? __syncthreads_count(key0 >= mid) + __syncthreads_count(key1 >= mid) : __syncthreads_count(keys >= mid);
+        if (n >= k) low = mid;
+        else high = mid - 1;
+        if (n >= k && n <= k + k / 16) break;
+      }
+      high = sf_key(top);
+    }
+    const int most = min(kSfList, 2 * kSfThreads);
+    float bound = sf_unkey(low);
+    int n = k > most ? most + 1 : sf_gather(row, list, &sh.count, [&](float x) { return x >= bound && x > -INFINITY; });
+    if (n > most && k <= most) {
+      // too many: halve the keys between by counting tokens, until at least k and no more than fit are left
+      while (low < high) {
+        const uint32_t mid = low + (high - low + 1) / 2;
+        const float at = sf_unkey(mid);
+        int c = 0;
+        row.each([&](float x, int) { c += x >= at; });
+        c = sf_sum(c, sh.ired);
+        if (c >= k) low = mid, n = c;
+        else high = mid - 1;
+        if (n <= most) break;
+      }
+      bound = sf_unkey(low);
+      if (n <= most) n = sf_gather(row, list, &sh.count, [&](float x) { return x >= bound && x > -INFINITY; });
+    }
+    if (n <= most) {
+      sf_sort(list, n);
+      // weights in order: thread t has the tokens 2t and 2t + 1
+      const int n_k = min(n, k);
+      float x[2];
+      u64 w[2], total;
+      double exact[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        x[e] = i < n_k ? sf_unkey((uint32_t)(list[i] >> 32)) : -INFINITY;
+        exact[e] = i < n_k ? weigh.scaled(x[e]) : 0.0;
+        w[e] = Weigh::fix(exact[e]);
+      }
+      const u64 before = sf_scan(w[0] + w[1], sh.red, total);
+      const u64 budget = top_p < 1.f ? (u64)(fmax((double)top_p, 0.0) * (double)total) : ~0ull;
+      int stay = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        stay += 2 * tid + e < n_k && before + (e ? w[0] : 0) <= budget && (x[e] == top || exact[e] >= least);
+      const int kept = sf_sum(stay, sh.ired);  // the first `kept` tokens: every condition falls along the order
+      if (kept <= 64) {
+        // back in vocabulary order (the list's low words are the complements of the indices), by one warp
+        if (wid == 0) {
+          u64 key[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int i = 2 * lane + e;
+            key[e] = i < kept ? (list[i] << 32) | (unsigned)(list[i] >> 32) : 0ull;
+          }
+          __syncwarp();
+          list[2 * lane] = key[0];
+          list[2 * lane + 1] = key[1];
+        }
+        sf_sort(list, 64);
+        if (wid == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int i = 2 * lane + e;
+            exact[e] = i < kept ? weigh.scaled(sf_unkey((uint32_t)list[i])) : 0.0;
+            w[e] = Weigh::fix(exact[e]);
+          }
+          u64 upto = w[0] + w[1];
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+          }
+          total = __shfl_sync(0xffffffffu, upto, 31);
+          const u64 target = min((u64)((double)u * (double)total), total - 1);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const u64 at = upto - w[1] - (e ? 0 : w[0]);
+            if (target >= at && target < at + w[e]) {
+              p.next[b] = (int)(0xffffffffu - (unsigned)(list[2 * lane + e] >> 32));
+              if (p.kept) p.kept[b] = kept;
+              if (p.prob) p.prob[b] = (float)(exact[e] / (double)total);
+            }
+          }
+        }
+        return;
+      }
+      // more: the draw below finds them again in vocabulary order
+      const float last = sf_unkey((uint32_t)(list[kept - 1] >> 32));
+      int equal = 0, ties = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        const bool same = i < n && (uint32_t)(list[i] >> 32) == sf_key(last);
+        equal += same;
+        ties += same && i < kept;
+      }
+      equal = sf_sum(equal, sh.ired);
+      ties = sf_sum(ties, sh.ired);
+      cut = Cut{last, ties == equal ? kSfAll : ties};
+      open_p = false;
+    } else {
+      cut = sf_radix_cut(row, weigh, cut, false, (u64)k, cnt, lo, hi);
+    }
+  }
+
+  if (open_p) {
+    // ---- top-p over what top-k keeps (here: everything, or more tokens than the list holds)
+    u64 m = 0;
+    row.each4([&](const float(&x)[4], int) {
+      if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > cut.x) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m += Weigh::biased(x[j] > cut.x ? weigh.scaled(x[j]) : 0.0);
+        m -= 4 * Weigh::kBias;
+      }
+    });
+    m = sf_sum(m, sh.red);
+    if (cut.ties != kSfAll) m += (u64)cut.ties * weigh.of(cut.x);
+    const u64 budget = (u64)(fmax((double)top_p, 0.0) * (double)m);
+    bool found = false;
+    if (cut.x == -INFINITY) {
+      // tokens further than `reach` below the top weigh under (m - budget) / V each: the boundary is above them
+      const double tail = (double)(m - budget) / V / unit;
+      const float reach = tail > 0 ? fminf((float)-log(tail) + 0.01f, weigh.far) : weigh.far;
+      const float scale = kSfBins / fmaxf(reach, 0.01f);
+      auto bin = [&](float x) { return (int)fminf((top - x) * scale, (float)kSfBins); };
+      cnt[tid] = lo[tid] = hi[tid] = 0u;
+      __syncthreads();
+      sf_dense(row, pool, [&](float x) { return bin(x) < kSfBins; }, [&](float x) {
+        const int d = bin(x);
+        const u64 w = weigh.of(x);
+        if (d < kSfBins) {
+          add_weight(lo + d, hi + d, w);
+          atomicAdd(cnt + d, 1u);
+        }
+      });
+      __syncthreads();
+      u64 total;
+      const u64 w = ((u64)hi[tid] << 32) + lo[tid], before = sf_scan(w, sh.red, total);
+      if (tid == 0) sh.pick = -1;
+      __syncthreads();
+      if (before <= budget && before + w > budget) {
+        sh.pick = cnt[tid] <= kSfList ? tid : -1;
+        sh.found = before;
+      }
+      __syncthreads();
+      const int d = sh.pick;
+      const u64 above = sh.found;
+      if (d >= 0) {
+        const int n = sf_gather(row, list, &sh.count, [&](float x) { return x > -INFINITY && bin(x) == d; });
+        sf_sort(list, n);
+        float x[2];
+        u64 v[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * tid + e;
+          x[e] = i < n ? sf_unkey((uint32_t)(list[i] >> 32)) : -INFINITY;
+          v[e] = i < n ? weigh.of(x[e]) : 0;
+        }
+        const u64 start = above + sf_scan(v[0] + v[1], sh.red, total);
+        int stay = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) stay += 2 * tid + e < n && start + (e ? v[0] : 0) <= budget;
+        stay = sf_sum(stay, sh.ired);  // at least 1: the bin's first token has `above` <= budget before it
+        const float last = sf_unkey((uint32_t)(list[stay - 1] >> 32));
+        int equal = 0, ties = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool same = 2 * tid + e < n && x[e] == last;
+          equal += same;
+          ties += same && 2 * tid + e < stay;
+        }
+        equal = sf_sum(equal, sh.ired);
+        ties = sf_sum(ties, sh.ired);
+        cut = Cut{last, ties == equal ? kSfAll : ties};
+        found = true;
+      }
+    }
+    if (!found) cut = sf_radix_cut(row, weigh, cut, true, budget, cnt, lo, hi);
+  }
+
+  // ---- the draw over the row: every warp owns a run of the vocabulary, a lane four neighbouring tokens at a time
+  const int run = (V + kSfWarps * 128 - 1) / (kSfWarps * 128) * 128, i0 = min(V, wid * run), i1 = min(V, i0 + run);
+  const bool count_ties = cut.ties != kSfAll;
+  // tokens below this are not kept: the cut, and a bound of min_p's that leaves the comparison to the weights
+  const float floor_p = min_p > 0.f ? fminf(top + logf(min_p) - 0.01f - 1e-5f * fabsf(top), top) : -INFINITY;
+  const float floor_x = fmaxf(cut.x, floor_p);
+  auto kept_by_x = [&](float x) { return x >= floor_x && x > -INFINITY; };
+  auto weight = [&](float x) -> double {  // negative: not kept by x and min_p
+    const double w = weigh.scaled(x);
+    return kept_by_x(x) && (x == top || w >= least) ? w : -1.0;
   };
-  int ties = 0;
-  for (int i = i0 + lane; i < i1; i += 32) ties += row.key(i) == cut.key;
-  ties = warp_sum(ties);
-  if (lane == 0) ties_of[wid] = ties;
-  __syncthreads();
-  int tie0 = 0;  // equal keys in the runs before this one
-  for (int j = 0; j < wid; ++j) tie0 += ties_of[j];
   u64 mass = 0;
-  int count = 0, tie = tie0;
-  for (int i = i0; i < i1; i += 32) {
-    const uint32_t key = i + lane < i1 ? row.key(i + lane) : 0u;
-    const unsigned eq = __ballot_sync(0xffffffffu, key == cut.key);
-    const double w = weight(key);
-    const bool stay = w >= 0.0 && (key != cut.key || tie + __popc(eq & ((1u << lane) - 1)) < cut.ties);
-    if (stay) mass += sf_fix(w, p.unit), ++count;
-    tie += __popc(eq);
+  int count = 0, tie0 = 0;  // tie0: tokens equal to the cut before this warp's run
+  if (!count_ties) {
+    // the weights of the runs do not depend on the order within them
+    auto add = [&](float x) {
+      const double w = weight(x);
+      mass += Weigh::fix(fmax(w, 0.0));
+      count += w >= 0.0;
+    };
+    if (floor_x == -INFINITY) {
+      for (int i = i0 + 4 * lane; i < i1; i += 128) {
+        const float4 v = row.x4(i);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mass += Weigh::biased(weigh.scaled(x[j]));
+          count += x[j] > -INFINITY;
+        }
+        mass -= 4 * Weigh::kBias;
+      }
+    } else {
+      int have = 0;
+      for (int i = i0; i < i1; i += 128) {
+        const float4 v = i + 4 * lane < i1 ? row.x4(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        sf_pool(pool, have, v, kept_by_x, add);
+      }
+      __syncwarp();
+      if (have) add(lane < have ? pool[lane] : -INFINITY);
+    }
+  } else {
+    int ties = 0;
+    for (int i = i0 + 4 * lane; i < i1; i += 128) {
+      const float4 v = row.x4(i);
+      ties += (v.x == cut.x) + (v.y == cut.x) + (v.z == cut.x) + (v.w == cut.x);
+    }
+    ties = warp_sum(ties);
+    __syncthreads();
+    if (lane == 0) sh.ired[wid] = ties;
+    __syncthreads();
+    int all;
+    tie0 = sf_warps(sh.ired, wid, all);
+    int tie = tie0;
+    for (int i = i0; i < i1; i += 128) {
+      const float4 v = i + 4 * lane < i1 ? row.x4(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      int before = tie;  // equal tokens before this lane's next one
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned eq = __ballot_sync(0xffffffffu, x[j] == cut.x);
+        before += __popc(eq & ((1u << lane) - 1));
+        tie += __popc(eq);
+      }
+      if (!kept_by_x(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])))) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double w = weight(x[j]);
+        const bool same = x[j] == cut.x, stay = w >= 0.0 && !(same && before >= cut.ties);
+        mass += Weigh::fix(stay ? w : 0.0);
+        count += stay;
+        before += same;
+      }
+    }
   }
   mass = warp_sum(mass);
   count = warp_sum(count);
   __syncthreads();
-  if (lane == 0) red[wid] = mass, ties_of[wid] = count;
+  if (lane == 0) sh.red[wid] = mass, sh.ired[wid] = count;
   __syncthreads();
-  u64 total = 0, before = 0;
-  int kept = 0;
-  for (int j = 0; j < kSfWarps; ++j) {
-    if (j < wid) before += red[j];
-    total += red[j];
-    kept += ties_of[j];
-  }
-  float u = p.uniform[b];
-  u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  u64 total;
+  int kept;
+  u64 before = sf_warps(sh.red, wid, total);
+  sf_warps(sh.ired, wid, kept);
   const u64 target = min((u64)((double)u * (double)total), total - 1);  // total >= 2^S: the first token is kept
-  if (target < before || target >= before + mass) return;
-  tie = tie0;
-  for (int i = i0; i < i1; i += 32) {
-    const uint32_t key = i + lane < i1 ? row.key(i + lane) : 0u;
-    const unsigned eq = __ballot_sync(0xffffffffu, key == cut.key);
-    const double w = weight(key);
-    const bool stay = w >= 0.0 && (key != cut.key || tie + __popc(eq & ((1u << lane) - 1)) < cut.ties);
-    const u64 mine = stay ? sf_fix(w, p.unit) : 0;
-    u64 upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > target);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        p.next[b] = i + lane;
-        if (p.kept) p.kept[b] = kept;
-        if (p.prob) p.prob[b] = (float)((double)mine / (double)total);
-      }
-      return;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-    tie += __popc(eq);
+  if (lane == 0 && target >= before && target < before + mass) {
+    sh.pick = wid;
+    sh.found = before;
+    sh.count = tie0;
   }
+  __syncthreads();
+  // ... and the whole block walks the run that holds the target
+  before = sh.found;
+  int tie = sh.count;
+  const int first = sh.pick * run, end = min(V, first + run);
+  for (int i = first; i < end; i += 4 * kSfThreads) {
+    const int at = i + 4 * tid;
+    const float4 v = at < end ? row.x4(at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    int rank = 0;
+    if (count_ties) {
+      u64 ties, own = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) own += x[j] == cut.x;
+      rank = tie + (int)sf_scan(own, sh.red, ties);
+      tie += (int)ties;
+    }
+    double w[4];
+    u64 fixed[4], sum = 0, all;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = weight(x[j]);
+      const bool same = count_ties && x[j] == cut.x;
+      fixed[j] = w[j] >= 0.0 && !(same && rank >= cut.ties) ? Weigh::fix(w[j]) : 0;
+      rank += same;
+      sum += fixed[j];
+    }
+    u64 from = before + sf_scan(sum, sh.red, all);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (target >= from && target < from + fixed[j]) {
+        p.next[b] = at + j;
+        if (p.kept) p.kept[b] = kept;
+        if (p.prob) p.prob[b] = (float)(w[j] / (double)total);
+      }
+      from += fixed[j];
+    }
+    before += all;
+    if (before > target) return;
+  }
+}
+
+template <typename T>
+int launch_sample(SampleArgs p, int batch, cudaStream_t s) {
+  static SmemLimit limit;
+  const auto fn = sample_filtered_kernel<T>;
+  const int list = kSfList * 8 + kSfWarps * 64 * 4, most = 232448 - 2048;  // 227 KB per block less the static part
+  p.in_shared = p.vocab <= (most - list) / 16 * 4;
+  const int bytes = list + (p.in_shared ? (p.vocab * 4 + 15) / 16 * 16 : 0);
+  DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
+  fn<<<batch, kSfThreads, bytes, s>>>(p);
+  DFSSM_CU(cudaGetLastError());
+  return DFSSM_OK;
 }
 
 }  // namespace dfssm
@@ -263,15 +843,10 @@ extern "C" int dfssm_sample_filtered(const void* logits, int64_t ld, int dtype, 
   if (batch == 0) return DFSSM_OK;
   int bits = 0;
   while ((1 << bits) < vocab) ++bits;
-  const SampleArgs p{logits,    ld,  vocab,       temperature, top_p,      min_p, uniform,
-                     top_k, seen_bits, rep_penalty, next,        kept_count, prob,  (double)(1ull << (62 - bits))};
+  SampleArgs p{logits,      ld,   vocab,      temperature, top_p,     min_p, uniform, top_k,
+               seen_bits, rep_penalty, next, kept_count, prob,        62 - bits > 50 ? 50 : 62 - bits, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == DFSSM_F32)
-    sample_filtered_kernel<float><<<batch, kSfThreads, 0, s>>>(p);
-  else if (dtype == DFSSM_F16)
-    sample_filtered_kernel<__half><<<batch, kSfThreads, 0, s>>>(p);
-  else
-    sample_filtered_kernel<__nv_bfloat16><<<batch, kSfThreads, 0, s>>>(p);
-  DFSSM_CU(cudaGetLastError());
-  return DFSSM_OK;
+  if (dtype == DFSSM_F32) return launch_sample<float>(p, batch, s);
+  if (dtype == DFSSM_F16) return launch_sample<__half>(p, batch, s);
+  return launch_sample<__nv_bfloat16>(p, batch, s);
 }
