@@ -12,18 +12,22 @@
 // and the rounding moves a boundary by about sqrt(V) 2^-S of the largest weight, some 1e-12, where fp32 sums
 // would move it by 1e-7 and pick other tokens once in a thousand rows.
 //
-// One block of 1024 threads per row, the row's x in shared memory where it fits (V up to about 50,000; else
-// every pass reads the logits again, from L2).  No pass sorts or selects over the whole row:
+// A cluster of 1 to 8 blocks of 1024 threads per row, each with a slice of the vocabulary and its x in shared memory
+// where it fits (about 51,000 tokens; else every pass reads the logits again, from L2).  No pass sorts or selects
+// over the whole row:
 //   - with top-k, the k-th largest of the threads' own largest values bounds the k-th largest x from below;
-//     the few tokens above it go to a list that is sorted, and the rest of the row is not looked at again;
-//   - with top-p alone, tokens of weight below (1 - top_p) sum / V together weigh too little to hold the
-//     boundary; a histogram over the others (1024 bins of x) finds its bin, whose tokens are sorted;
-//   - the result of either is a cut {x, how many of the tokens equal to it stay}.
+//     the few tokens above it go to a list that the cluster's first block sorts, and the rest of the row is not
+//     looked at again;
+//   - with top-p alone, a histogram of the weights (1024 bins of x, one pass) finds the bin that holds the
+//     boundary, whose tokens are sorted;
+//   - the result of either is a cut {x, how many of the tokens equal to it stay}, and the draw is one more pass
+//     that weighs what the cut keeps.
 // Rows where the list would overflow (thousands of equal logits at the cut, top_k in the thousands) select the
 // cut by four rounds over 8 bits of x's order-preserving key instead.
 //
-// Bound: 64-bit floating point where a whole row needs its weights (10 operations a token), else the first
-// pass over the logits.
+// Bound: instructions.  A weight is 25 of them, 10 in 64-bit floating point, and a row without top-k needs one
+// for every token; with top-k the first pass over the logits (a division each) is most of it.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -36,6 +40,7 @@ constexpr int kSfWarps = kSfThreads / 32;
 constexpr int kSfList = 2048;  // tokens that are sorted
 constexpr int kSfBins = 1024;  // one per thread
 constexpr int kSfAll = 0x7fffffff;
+constexpr int kSfBlocks = 8;   // of a row, at most
 
 typedef unsigned long long u64;
 
@@ -50,7 +55,8 @@ struct SampleArgs {
   int *next, *kept;
   float* prob;
   int shift;      // S
-  int in_shared;  // x of the row in shared memory
+  int slice;      // tokens per block of a row's cluster, a multiple of 128
+  int in_shared;  // x of the slice in shared memory
 };
 
 __device__ __forceinline__ float sf_logit(const float* p) { return *p; }
@@ -77,8 +83,9 @@ template <typename T>
 struct Row {
   const T* l;
   const uint32_t* seen;
-  const float* xs;  // the row's x in shared memory, or NULL: every pass computes them again
-  int V;
+  const float* xs;  // the slice's x in shared memory (token i at xs[i - from]), or NULL: every pass computes them again
+  int V;            // the row's tokens
+  int from, to;     // the block's slice of them
   float temp, rtemp, rep;
   bool divide, mild, aligned;  // aligned: four logits at a time
   bool lift;                   // the row's largest x is +inf: tokens there count as 0, all others as -inf
@@ -110,7 +117,7 @@ struct Row {
     for (int j = 0; j < 4; ++j) e[j] = fmaxf(e[j], -INFINITY);
     return v;
   }
-  // logits i .. i + 3 (i a multiple of 4, i < V), -inf behind the row's end
+  // logits i .. i + 3 (i a multiple of 4, i < V), -inf behind the row's end (a slice ends at a multiple of 4 or there)
   __device__ __forceinline__ float4 logits4(int i) const {
     float4 v;
     if (aligned && i + 4 <= V) {
@@ -130,7 +137,7 @@ struct Row {
     return v;
   }
   __device__ __forceinline__ float4 x4(int i) const {
-    float4 v = xs ? *reinterpret_cast<const float4*>(xs + i) : from4(logits4(i), i);
+    float4 v = xs ? *reinterpret_cast<const float4*>(xs + (i - from)) : from4(logits4(i), i);
     if (lift) {
       v.x = v.x == INFINITY ? 0.f : -INFINITY;
       v.y = v.y == INFINITY ? 0.f : -INFINITY;
@@ -142,7 +149,7 @@ struct Row {
   // f(x, index) for four tokens at a time
   template <typename F>
   __device__ __forceinline__ void each4(F f) const {
-    for (int i = 4 * threadIdx.x; i < V; i += 4 * kSfThreads) {
+    for (int i = from + 4 * threadIdx.x; i < to; i += 4 * kSfThreads) {
       const float4 v = x4(i);
       const float x[4] = {v.x, v.y, v.z, v.w};
       f(x, i);
@@ -151,7 +158,7 @@ struct Row {
   // f(x, index) for every token; behind the row's end x is -inf
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (int i = 4 * threadIdx.x; i < V; i += 4 * kSfThreads) {
+    for (int i = from + 4 * threadIdx.x; i < to; i += 4 * kSfThreads) {
       const float4 v = x4(i);
       f(v.x, i);
       f(v.y, i + 1);
@@ -210,6 +217,36 @@ struct Shared {
   double table[64];
   u64 found;
   int count, pick;
+  // written by the cluster's blocks in one another's copy, a slot for each; two sets, used in turn
+  float bmax[2][kSfBlocks];
+  u64 bmass[2][kSfBlocks];
+  int bcount[2][kSfBlocks];
+  // written by the first block in everybody's
+  Cut cut;
+  u64 budget, above;
+  float scale;
+  int state;
+};
+
+// The blocks of one row.
+struct Group {
+  int rank, blocks, turn;
+  __device__ __forceinline__ void sync() const {
+    if (blocks == 1) __syncthreads();
+    else cooperative_groups::this_cluster().sync();
+  }
+  template <typename V>
+  __device__ __forceinline__ V* at(V* p, int block) const {  // that block's copy of a shared variable
+    return blocks == 1 ? p : cooperative_groups::this_cluster().map_shared_rank(p, block);
+  }
+  // Every block's value, the same in all its threads, to every block: read slots[turn][...] after the sync in it.
+  template <typename V>
+  __device__ __forceinline__ const V* share(V (&slots)[2][kSfBlocks], V v) {
+    turn ^= 1;
+    if (threadIdx.x < blocks) *at(&slots[turn][rank], threadIdx.x) = v;
+    sync();
+    return slots[turn];
+  }
 };
 
 // Block-wide reductions and an exclusive scan, the same value in every thread.
@@ -290,58 +327,130 @@ __device__ __forceinline__ void sf_pool(float* pool, int& have, const float4& v,
   }
 }
 
-// Runs `use(x)` on every token that `take` accepts, 32 at a time: a warp collects what its lanes' tiles have in
-// its pool, so that a few tokens among many cost few warp-wide evaluations.  use() is called by
-// whole warps, with -inf in the lanes of a last, partly filled round.
-template <typename T, typename F, typename G>
-__device__ __forceinline__ void sf_dense(const Row<T>& row, float* pool, F take, G use) {
+// Compare-exchange steps of a bitonic sort at distances 32 .. 1 among the 64 keys of a warp, for the merges of length
+// k: lane l holds the keys base + l and base + l + 32.
+__device__ __forceinline__ void sf_merge64(u64 (&e)[2], int base, int k) {
   const int lane = threadIdx.x & 31;
-  int have = 0;
-  for (int i0 = 4 * (threadIdx.x - lane); i0 < row.V; i0 += 4 * kSfThreads) {
-    const int i = i0 + 4 * lane;
-    sf_pool(pool, have, i < row.V ? row.x4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), take, use);
+#pragma unroll
+  for (int j = 32; j > 0; j >>= 1) {
+    if (j >= k) continue;
+    if (j == 32) {
+      const u64 a = max(e[0], e[1]), b = min(e[0], e[1]);
+      const bool falling = (base & k) == 0;
+      e[0] = falling ? a : b, e[1] = falling ? b : a;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u64 o = __shfl_xor_sync(0xffffffffu, e[h], j);
+        const bool falling = ((base + lane + 32 * h) & k) == 0;
+        e[h] = falling == ((lane & j) == 0) ? max(e[h], o) : min(e[h], o);
+      }
+    }
   }
-  __syncwarp();
-  if (have) use(lane < have ? pool[lane] : -INFINITY);
+}
+// Descending sort of 64 keys by one warp.
+__device__ __forceinline__ void sf_sort64(u64 (&e)[2], int base = 0) {
+#pragma unroll 1
+  for (int k = 2; k <= 64; k <<= 1) sf_merge64(e, base, k);
+}
+// Sum over the keys before each of two: e = 0 stands before e = 1 of every lane (positions l and l + 32).
+__device__ __forceinline__ void sf_scan64(const u64 (&v)[2], u64 (&before)[2], u64& total) {
+  const int lane = threadIdx.x & 31;
+  u64 a = v[0], b = v[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += x, b += y;
+  }
+  const u64 first = __shfl_sync(0xffffffffu, a, 31);
+  before[0] = a - v[0];
+  before[1] = first + b - v[1];
+  total = first + __shfl_sync(0xffffffffu, b, 31);
 }
 
-// Descending bitonic sort of list[0..n), n <= kSfList, padded with zeros to a power of two, by half as many
-// threads as there are entries; begins and ends with a block barrier.
+// The draw among up to 64 kept tokens {key of x, complement of the index}, zeros behind them, by one warp.
+__device__ __forceinline__ void sf_draw64(const SampleArgs& p, int b, float u, const Weigh& weigh, u64 (&key)[2], int kept) {
+  u64 w[2], before[2], total;
+  double exact[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) key[e] = (key[e] << 32) | (key[e] >> 32);
+  sf_sort64(key);  // in vocabulary order
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    exact[e] = key[e] ? weigh.scaled(sf_unkey((uint32_t)key[e])) : 0.0;
+    w[e] = Weigh::fix(exact[e]);
+  }
+  sf_scan64(w, before, total);
+  const u64 target = min((u64)((double)u * (double)total), total - 1);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (target >= before[e] && target < before[e] + w[e]) {
+      p.next[b] = (int)(0xffffffffu - (unsigned)(key[e] >> 32));
+      if (p.kept) p.kept[b] = kept;
+      if (p.prob) p.prob[b] = (float)(exact[e] / (double)total);
+    }
+  }
+}
+
+// Descending sort of list[0..n), n <= kSfList, all different: up to 256 by counting, more by a bitonic sort, padded with
+// zeros to a power of two, by half as many threads as entries: distances below 64 in registers, the others
+// through the list.  Begins and ends with a block barrier.
 __device__ void sf_sort(u64* list, int n) {
   int size = 64;
   while (size < n) size <<= 1;
   __syncthreads();
-  const int t = threadIdx.x, workers = size / 2;
-  if (t < workers) {
-    for (int i = n + t; i < size; i += workers) list[i] = 0ull;
-    auto meet = [&] {
-      if (workers == 32) __syncwarp();
-      else asm volatile("bar.sync 1, %0;" ::"r"(workers) : "memory");
-    };
-    meet();
-    for (int k = 2; k <= size; k <<= 1) {
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        const int i = 2 * t - (t & (j - 1)), o = i + j;  // pairs at distance j
-        const u64 a = list[i], b = list[o];
-        if ((a < b) == ((i & k) == 0)) list[i] = b, list[o] = a;
-        if (j > 32 || (j == 1 && k >= 64)) meet();  // pairs at distances up to 32 stay within a warp's 64 entries
-        else __syncwarp();
+  if (size <= 256) {
+    // few: every key's place is the number of larger ones, counted by several threads
+    const int per = kSfThreads / size, i = threadIdx.x / per, part = threadIdx.x % per;
+    const u64 key = i < n ? list[i] : 0ull;
+    int place = 0;
+    for (int j = part; j < n; j += per) place += list[j] > key;
+    for (int o = per / 2; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    __syncthreads();
+    if (part == 0 && i < n) list[place] = key;
+    __syncthreads();
+    return;
+  }
+  const int workers = size / 2;
+  if (threadIdx.x < workers) {
+    const int base = (threadIdx.x >> 5) * 64, i0 = base + (threadIdx.x & 31), i1 = i0 + 32;
+    u64 e[2] = {i0 < n ? list[i0] : 0ull, i1 < n ? list[i1] : 0ull};
+    auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"r"(workers) : "memory"); };
+    sf_sort64(e, base);
+    for (int k = 128; k <= size; k <<= 1) {
+      for (int j = k >> 1; j >= 64; j >>= 1) {
+        meet();
+        list[i0] = e[0];
+        list[i1] = e[1];
+        meet();
+        const bool upper = (base & j) != 0, falling = (base & k) == 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u64 o = list[(h ? i1 : i0) ^ j];
+          e[h] = falling != upper ? max(e[h], o) : min(e[h], o);
+        }
       }
+      sf_merge64(e, base, k);
     }
+    meet();
+    list[i0] = e[0];
+    list[i1] = e[1];
   }
   __syncthreads();
 }
 
-// Appends the tokens that `take` accepts (none at -inf) to the list as {key of x, complement of the index};
-// returns how many there are, which may be more than were stored.
+// Appends the cluster's tokens that `take` accepts (none at -inf) to the first block's list, as {key of x,
+// complement of the index}; returns how many there are, which may be more than were stored.
 template <typename T, typename F>
-__device__ int sf_gather(const Row<T>& row, u64* list, int* count, F take) {
-  if (threadIdx.x == 0) *count = 0;
-  __syncthreads();
+__device__ int sf_gather(const Row<T>& row, Group& grp, u64* list, Shared& sh, F take) {
+  if (grp.rank == 0 && threadIdx.x == 0) sh.count = 0;
+  grp.sync();
+  u64* const to = grp.at(list, 0);
+  int* const count = grp.at(&sh.count, 0);
   const int lane = threadIdx.x & 31;
-  for (int i0 = 4 * (threadIdx.x - lane); i0 < row.V; i0 += 4 * kSfThreads) {
+  for (int i0 = row.from + 4 * (threadIdx.x - lane); i0 < row.to; i0 += 4 * kSfThreads) {
     const int i = i0 + 4 * lane;
-    const float4 v = i < row.V ? row.x4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const float4 v = i < row.to ? row.x4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     const float x[4] = {v.x, v.y, v.z, v.w};
     bool in[4], any = false;
 #pragma unroll
@@ -354,24 +463,26 @@ __device__ int sf_gather(const Row<T>& row, u64* list, int* count, F take) {
       int at = 0;
       if (lane == 0) at = atomicAdd(count, __popc(all));
       at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
-      if (in[j] && at < kSfList) list[at] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
+      if (in[j] && at < kSfList) to[at] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
     }
   }
-  __syncthreads();
-  return *count;
+  grp.sync();
+  const int n = *count;
+  grp.sync();  // everybody has read it: the list may be used again
+  return n;
 }
 
 // The cut by four rounds over 8 bits of the key, for what does not fit the list.  by_weight: a token stays while
 // the weight before it is <= budget; else `budget` tokens stay.  Looks at the tokens that `floor` keeps and
 // returns it when the budget outlasts them.
 template <typename T>
-__device__ __noinline__ Cut sf_radix_cut(const Row<T>& row, const Weigh& weigh, Cut floor, bool by_weight, u64 budget,
-                                         unsigned* cnt, unsigned* lo, unsigned* hi) {
+__device__ __noinline__ Cut sf_radix_cut(const Row<T>& row, Group& grp, const Weigh& weigh, Cut floor, bool by_weight,
+                                         u64 budget, unsigned* cnt, unsigned* lo, unsigned* hi) {
   const uint32_t least = max(sf_key(floor.x), 1u);
   uint32_t prefix = 0;
   u64 used = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
+    grp.sync();
     for (int i = threadIdx.x; i < 256; i += kSfThreads) cnt[i] = lo[i] = hi[i] = 0u;
     __syncthreads();
     row.each([&](float x, int) {
@@ -381,7 +492,20 @@ __device__ __noinline__ Cut sf_radix_cut(const Row<T>& row, const Weigh& weigh, 
       atomicAdd(cnt + d, 1u);
       if (by_weight) add_weight(lo + d, hi + d, weigh.of(x));
     });
-    __syncthreads();
+    grp.sync();
+    if (grp.blocks > 1) {  // every block adds up everybody's
+      unsigned c = 0;
+      u64 m = 0;
+      if (threadIdx.x < 256) {
+        for (int r = 0; r < grp.blocks; ++r) {
+          c += grp.at(cnt, r)[threadIdx.x];
+          m += ((u64)grp.at(hi, r)[threadIdx.x] << 32) + grp.at(lo, r)[threadIdx.x];
+        }
+      }
+      grp.sync();
+      if (threadIdx.x < 256) cnt[threadIdx.x] = c, lo[threadIdx.x] = (unsigned)m, hi[threadIdx.x] = (unsigned)(m >> 32);
+      __syncthreads();
+    }
     int d = 255;  // every thread walks the digits from the top; all come to the same one
     for (; d >= 0; --d) {
       const u64 m = by_weight ? ((u64)hi[d] << 32) + lo[d] : cnt[d];
@@ -389,7 +513,7 @@ __device__ __noinline__ Cut sf_radix_cut(const Row<T>& row, const Weigh& weigh, 
       used += m;
     }
     const int here = d < 0 ? 0 : (int)cnt[d];
-    __syncthreads();
+    grp.sync();
     if (d < 0) return floor;
     prefix = (prefix << 8) | (uint32_t)d;
     if (shift == 0) {
@@ -407,17 +531,27 @@ template <typename T>
 __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
-  u64* list = reinterpret_cast<u64*>(dyn);  // [kSfList]; the histogram's counts and weights before it is filled
+  u64* list = reinterpret_cast<u64*>(dyn);  // [kSfList]; before it is filled, the histograms' words
   unsigned* cnt = reinterpret_cast<unsigned*>(dyn);
-  unsigned *lo = cnt + kSfBins, *hi = lo + kSfBins;
+  unsigned *lo = cnt + 256, *hi = lo + kSfBins;
   float* pool = reinterpret_cast<float*>(list + kSfList) + (threadIdx.x >> 5) * 64;  // one per warp
   float* xs = reinterpret_cast<float*>(list + kSfList) + kSfWarps * 64;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, V = p.vocab;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, V = p.vocab;
+  Group grp{0, 1, 0};
+  if (gridDim.y > 1) {  // a cluster is the blocks of one row
+    grp.blocks = gridDim.y;
+    grp.rank = blockIdx.y;
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // this block runs: the wait is below
+  }
+  const int b = blockIdx.x;
+  const bool chief = grp.rank == 0;
   Row<T> row;
   row.l = static_cast<const T*>(p.logits) + (long long)b * p.ld;
   row.seen = p.seen ? p.seen + (size_t)b * ((V + 31) / 32) : nullptr;
   row.xs = nullptr;
   row.V = V;
+  row.from = min(V, grp.rank * p.slice);
+  row.to = min(V, row.from + p.slice);
   row.lift = false;
   row.aligned = (reinterpret_cast<uintptr_t>(row.l) & (4 * sizeof(T) - 1)) == 0;
   const float temp = p.temperature ? p.temperature[b] : 1.0f;
@@ -432,22 +566,22 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   float u = p.uniform[b];
   u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
 
-  // ---- x of the row, each thread's largest, the row's largest
+  // ---- x of the slice, each thread's largest, the row's largest
   float mine2[2] = {-INFINITY, -INFINITY};  // of the thread's tokens, split in two
   constexpr int kAhead = 4;
-  for (int i0 = 4 * tid; i0 < V; i0 += kAhead * 4 * kSfThreads) {
+  for (int i0 = row.from + 4 * tid; i0 < row.to; i0 += kAhead * 4 * kSfThreads) {
     float4 v[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int i = i0 + j * 4 * kSfThreads;
-      if (i < V) v[j] = row.logits4(i);
+      if (i < row.to) v[j] = row.logits4(i);
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int i = i0 + j * 4 * kSfThreads;
-      if (i < V) {
+      if (i < row.to) {
         const float4 x = row.from4(v[j], i);
-        if (p.in_shared) *reinterpret_cast<float4*>(xs + i) = x;
+        if (p.in_shared) *reinterpret_cast<float4*>(xs + (i - row.from)) = x;
         mine2[j & 1] = fmaxf(mine2[j & 1], fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
       }
     }
@@ -455,21 +589,27 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   if (p.in_shared) row.xs = xs;
   const float mine = fmaxf(mine2[0], mine2[1]);
   if (tid < 64) sh.table[tid] = ldexp(exp2(tid / 64.0), p.shift);
+  if (tid == 0) sh.pick = V;
   float top = sf_max(mine, sh.fred);
+  if (grp.blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all run: their memory can be written
+  {
+    const float* all = grp.share(sh.bmax, top);
+    for (int r = 0; r < grp.blocks; ++r) top = fmaxf(top, all[r]);
+  }
   if (top == -INFINITY) {  // nothing to take in this row
-    if (tid == 0) {
+    if (chief && tid == 0) {
       p.next[b] = -1;
       if (p.kept) p.kept[b] = 0;
       if (p.prob) p.prob[b] = 0.f;
     }
+    grp.sync();
     return;
   }
   if (k == 1) {  // the first token of the order
-    if (tid == 0) sh.pick = V;
-    __syncthreads();
-    if (mine == top) row.each([&](float x, int i) { if (x == top) atomicMin(&sh.pick, i); });
-    __syncthreads();
-    if (tid == 0) {
+    int* const pick = grp.at(&sh.pick, 0);
+    if (mine == top) row.each([&](float x, int i) { if (x == top) atomicMin(pick, i); });
+    grp.sync();
+    if (chief && tid == 0) {
       p.next[b] = sh.pick;
       if (p.kept) p.kept[b] = 1;
       if (p.prob) p.prob[b] = 1.f;
@@ -489,201 +629,242 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
 
   if (k > 0 && k < V) {
     // ---- top-k: a lower bound of the k-th largest x, the tokens from there on sorted
-    const uint32_t key0 = sf_key(mine2[0]), key1 = sf_key(mine2[1]), keys = max(key0, key1);
-    uint32_t low = 0u, high = sf_key(top);
+    float bound = -INFINITY;
     if (k <= 2 * kSfThreads) {
-      // the largest key that at least k of the threads' largest reach (for larger k of both their halves), or
-      // one that few more do
-      const bool halves = k > kSfThreads / 4;
-      const uint32_t all = __reduce_min_sync(0xffffffffu, halves ? min(key0, key1) : keys);
-      if (lane == 0) sh.ired[wid] = (int)all;
-      __syncthreads();
-      low = __reduce_min_sync(0xffffffffu, (unsigned)sh.ired[lane]);
-      while (low < high) {
-        const uint32_t mid = low + (high - low + 1) / 2;
-        const int n = halves ? __syncthreads_count(key0 >= mid) + __syncthreads_count(key1 >= mid) : __syncthreads_count(keys >= mid);
-        if (n >= k) low = mid;
-        else high = mid - 1;
-        if (n >= k && n <= k + k / 16) break;
+      // The c-th largest of the block's threads' largest (for larger c of both their halves), rounded down to a bin of a
+      // histogram: at least c of the block's tokens are there or above.  With c = k / blocks in every block, the
+      // least of the blocks' bounds bounds the row's k-th largest; where that is nothing (a block holds too few
+      // tokens), with c = k, each one's does.
+      auto reach = [&](int c) -> float {
+        const bool halves = c > kSfThreads / 4;
+        const float m0 = halves ? mine2[0] : fmaxf(mine2[0], mine2[1]), m1 = halves ? mine2[1] : -INFINITY;
+        const float low = fminf(m0 > -INFINITY ? m0 : top, m1 > -INFINITY ? m1 : top);
+        const float width = fmaxf(top + sf_max(-low, sh.fred), 1e-6f * fabsf(top) + 1e-30f), scale = (kSfBins - 1) / width;
+        lo[tid] = 0u;
+        __syncthreads();
+        if (m0 > -INFINITY) atomicAdd(lo + min(kSfBins - 1, (int)((top - m0) * scale)), 1u);
+        if (m1 > -INFINITY) atomicAdd(lo + min(kSfBins - 1, (int)((top - m1) * scale)), 1u);
+        __syncthreads();
+        u64 total;
+        const int n = (int)lo[tid], before = (int)sf_scan((u64)n, sh.red, total);
+        if (tid == 0) sh.scale = -INFINITY;
+        __syncthreads();
+        // a margin for the roundings of the bin's number
+        if (before < c && before + n >= c) sh.scale = top - (tid + 1.01f) / scale - 1e-6f * fabsf(top);
+        __syncthreads();
+        return sh.scale;
+      };
+      bound = reach((k + grp.blocks - 1) / grp.blocks);
+      if (grp.blocks > 1) {
+        const float* bounds = grp.share(sh.bmax, bound);
+        for (int r = 0; r < grp.blocks; ++r) bound = fminf(bound, bounds[r]);
+        if (bound == -INFINITY) {
+          bounds = grp.share(sh.bmax, reach(k));
+          for (int r = 0; r < grp.blocks; ++r) bound = fmaxf(bound, bounds[r]);
+        }
       }
-      high = sf_key(top);
     }
-    const int most = min(kSfList, 2 * kSfThreads);
-    float bound = sf_unkey(low);
-    int n = k > most ? most + 1 : sf_gather(row, list, &sh.count, [&](float x) { return x >= bound && x > -INFINITY; });
-    if (n > most && k <= most) {
+    int n = k > kSfList ? kSfList + 1
+                        : sf_gather(row, grp, list, sh, [&](float x) { return x >= bound && x > -INFINITY; });
+    if (n > kSfList && k <= kSfList) {
       // too many: halve the keys between by counting tokens, until at least k and no more than fit are left
+      uint32_t low = sf_key(bound), high = sf_key(top);
       while (low < high) {
         const uint32_t mid = low + (high - low + 1) / 2;
         const float at = sf_unkey(mid);
         int c = 0;
         row.each([&](float x, int) { c += x >= at; });
-        c = sf_sum(c, sh.ired);
+        const int* all = grp.share(sh.bcount, sf_sum(c, sh.ired));
+        c = 0;
+        for (int r = 0; r < grp.blocks; ++r) c += all[r];
         if (c >= k) low = mid, n = c;
         else high = mid - 1;
-        if (n <= most) break;
+        if (n <= kSfList) break;
       }
       bound = sf_unkey(low);
-      if (n <= most) n = sf_gather(row, list, &sh.count, [&](float x) { return x >= bound && x > -INFINITY; });
+      if (n <= kSfList) n = sf_gather(row, grp, list, sh, [&](float x) { return x >= bound && x > -INFINITY; });
     }
-    if (n <= most) {
-      sf_sort(list, n);
-      // weights in order: thread t has the tokens 2t and 2t + 1
-      const int n_k = min(n, k);
-      float x[2];
-      u64 w[2], total;
-      double exact[2];
+    if (n <= kSfList) {
+      if (chief) {
+        const int n_k = min(n, k);
+        if (n <= 64) {
+          // one warp: order, weights, what stays; then the draw
+          if (wid == 0) {
+            u64 key[2], w[2], before[2], total;
+            double exact[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        x[e] = i < n_k ? sf_unkey((uint32_t)(list[i] >> 32)) : -INFINITY;
-        exact[e] = i < n_k ? weigh.scaled(x[e]) : 0.0;
-        w[e] = Weigh::fix(exact[e]);
-      }
-      const u64 before = sf_scan(w[0] + w[1], sh.red, total);
-      const u64 budget = top_p < 1.f ? (u64)(fmax((double)top_p, 0.0) * (double)total) : ~0ull;
-      int stay = 0;
+            for (int e = 0; e < 2; ++e) key[e] = lane + 32 * e < n ? list[lane + 32 * e] : 0ull;
+            sf_sort64(key);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        stay += 2 * tid + e < n_k && before + (e ? w[0] : 0) <= budget && (x[e] == top || exact[e] >= least);
-      const int kept = sf_sum(stay, sh.ired);  // the first `kept` tokens: every condition falls along the order
-      if (kept <= 64) {
-        // back in vocabulary order (the list's low words are the complements of the indices), by one warp
-        if (wid == 0) {
-          u64 key[2];
+            for (int e = 0; e < 2; ++e) {
+              exact[e] = lane + 32 * e < n_k ? weigh.scaled(sf_unkey((uint32_t)(key[e] >> 32))) : 0.0;
+              w[e] = Weigh::fix(exact[e]);
+            }
+            sf_scan64(w, before, total);
+            const u64 budget = top_p < 1.f ? (u64)(fmax((double)top_p, 0.0) * (double)total) : ~0ull;
+            int kept = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = 2 * lane + e;
-            key[e] = i < kept ? (list[i] << 32) | (unsigned)(list[i] >> 32) : 0ull;
+            for (int e = 0; e < 2; ++e) {
+              const bool stay = lane + 32 * e < n_k && before[e] <= budget &&
+                                (sf_unkey((uint32_t)(key[e] >> 32)) == top || exact[e] >= least);
+              kept += __popc(__ballot_sync(0xffffffffu, stay));
+              if (!stay) key[e] = 0ull;
+            }
+            sf_draw64(p, b, u, weigh, key, kept);
           }
-          __syncwarp();
-          list[2 * lane] = key[0];
-          list[2 * lane + 1] = key[1];
-        }
-        sf_sort(list, 64);
-        if (wid == 0) {
+        } else {
+          sf_sort(list, n);
+          // weights in order: thread t has the tokens 2t and 2t + 1
+          float x[2];
+          u64 w[2], total;
+          double exact[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int i = 2 * lane + e;
-            exact[e] = i < kept ? weigh.scaled(sf_unkey((uint32_t)list[i])) : 0.0;
+            const int i = 2 * tid + e;
+            x[e] = i < n_k ? sf_unkey((uint32_t)(list[i] >> 32)) : -INFINITY;
+            exact[e] = i < n_k ? weigh.scaled(x[e]) : 0.0;
             w[e] = Weigh::fix(exact[e]);
           }
-          u64 upto = w[0] + w[1];
+          const u64 before = sf_scan(w[0] + w[1], sh.red, total);
+          const u64 budget = top_p < 1.f ? (u64)(fmax((double)top_p, 0.0) * (double)total) : ~0ull;
+          int stay = 0;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
+          for (int e = 0; e < 2; ++e)
+            stay += 2 * tid + e < n_k && before + (e ? w[0] : 0) <= budget && (x[e] == top || exact[e] >= least);
+          const int kept = sf_sum(stay, sh.ired);  // the first `kept` tokens: every condition falls along the order
+          if (kept <= 64 && wid == 0) {
+            u64 key[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) key[e] = lane + 32 * e < kept ? list[lane + 32 * e] : 0ull;
+            sf_draw64(p, b, u, weigh, key, kept);
           }
-          total = __shfl_sync(0xffffffffu, upto, 31);
-          const u64 target = min((u64)((double)u * (double)total), total - 1);
+          // more than 64: the draw below finds them again in vocabulary order
+          const uint32_t last = (uint32_t)(list[kept - 1] >> 32);
+          int equal = 0, ties = 0;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const u64 at = upto - w[1] - (e ? 0 : w[0]);
-            if (target >= at && target < at + w[e]) {
-              p.next[b] = (int)(0xffffffffu - (unsigned)(list[2 * lane + e] >> 32));
-              if (p.kept) p.kept[b] = kept;
-              if (p.prob) p.prob[b] = (float)(exact[e] / (double)total);
-            }
+            const int i = 2 * tid + e;
+            const bool same = i < n && (uint32_t)(list[i] >> 32) == last;
+            equal += same;
+            ties += same && i < kept;
           }
+          equal = sf_sum(equal, sh.ired);
+          ties = sf_sum(ties, sh.ired);
+          if (tid < grp.blocks)
+            *grp.at(&sh.cut, tid) = kept <= 64 ? Cut{INFINITY, 0} : Cut{sf_unkey(last), ties == equal ? kSfAll : ties};
         }
-        return;
       }
-      // more: the draw below finds them again in vocabulary order
-      const float last = sf_unkey((uint32_t)(list[kept - 1] >> 32));
-      int equal = 0, ties = 0;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        const bool same = i < n && (uint32_t)(list[i] >> 32) == sf_key(last);
-        equal += same;
-        ties += same && i < kept;
-      }
-      equal = sf_sum(equal, sh.ired);
-      ties = sf_sum(ties, sh.ired);
-      cut = Cut{last, ties == equal ? kSfAll : ties};
+      if (n <= 64) return;  // after the gather no block reaches into another's memory
+      grp.sync();
+      cut = sh.cut;
+      if (cut.ties == 0) return;  // drawn
       open_p = false;
     } else {
-      cut = sf_radix_cut(row, weigh, cut, false, (u64)k, cnt, lo, hi);
+      cut = sf_radix_cut(row, grp, weigh, cut, false, (u64)k, cnt, lo, hi);
     }
   }
 
   if (open_p) {
     // ---- top-p over what top-k keeps (here: everything, or more tokens than the list holds)
-    u64 m = 0;
-    row.each4([&](const float(&x)[4], int) {
-      if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > cut.x) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) m += Weigh::biased(x[j] > cut.x ? weigh.scaled(x[j]) : 0.0);
-        m -= 4 * Weigh::kBias;
-      }
-    });
-    m = sf_sum(m, sh.red);
-    if (cut.ties != kSfAll) m += (u64)cut.ties * weigh.of(cut.x);
-    const u64 budget = (u64)(fmax((double)top_p, 0.0) * (double)m);
     bool found = false;
+    u64 budget = 0;
     if (cut.x == -INFINITY) {
-      // tokens further than `reach` below the top weigh under (m - budget) / V each: the boundary is above them
-      const double tail = (double)(m - budget) / V / unit;
-      const float reach = tail > 0 ? fminf((float)-log(tail) + 0.01f, weigh.far) : weigh.far;
-      const float scale = kSfBins / fmaxf(reach, 0.01f);
-      auto bin = [&](float x) { return (int)fminf((top - x) * scale, (float)kSfBins); };
-      cnt[tid] = lo[tid] = hi[tid] = 0u;
+      // Weights by x, in bins; even and odd warps have a copy each (fewer collide).  Tokens further below the top than
+      // `range` weigh less than (1 - top_p) / V of it each, so together too little to hold the boundary: they are
+      // only added up.  One thread per bin then adds up the copies and the blocks.
+      const float range = fminf(weigh.far, logf(V / (1.f - fmaxf(top_p, 0.f))) + 0.01f), scale = kSfBins / range;
+      unsigned *lo0 = cnt, *hi0 = cnt + 2 * kSfBins, *lo1 = lo0 + (wid & 1) * kSfBins, *hi1 = hi0 + (wid & 1) * kSfBins;
+      lo0[tid] = lo0[kSfBins + tid] = hi0[tid] = hi0[kSfBins + tid] = 0u;
       __syncthreads();
-      sf_dense(row, pool, [&](float x) { return bin(x) < kSfBins; }, [&](float x) {
-        const int d = bin(x);
-        const u64 w = weigh.of(x);
-        if (d < kSfBins) {
-          add_weight(lo + d, hi + d, w);
-          atomicAdd(cnt + d, 1u);
+      u64 rest = 0;
+      row.each4([&](const float(&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float d = (top - x[j]) * scale;
+          const u64 w = weigh.of(x[j]);
+          if (d < (float)kSfBins) add_weight(lo1 + (int)d, hi1 + (int)d, w);
+          else rest += w;
         }
       });
-      __syncthreads();
-      u64 total;
-      const u64 w = ((u64)hi[tid] << 32) + lo[tid], before = sf_scan(w, sh.red, total);
-      if (tid == 0) sh.pick = -1;
-      __syncthreads();
-      if (before <= budget && before + w > budget) {
-        sh.pick = cnt[tid] <= kSfList ? tid : -1;
-        sh.found = before;
+      rest = sf_sum(rest, sh.red);
+      const u64* rests = grp.share(sh.bmass, rest);
+      if (chief) {
+        u64 w = 0, total;
+#pragma unroll
+        for (int r = 0; r < kSfBlocks; ++r) {
+          if (r < grp.blocks) {
+            const unsigned *l = grp.at(lo0, r), *h = grp.at(hi0, r);
+            w += ((u64)h[tid] << 32) + l[tid] + ((u64)h[kSfBins + tid] << 32) + l[kSfBins + tid];
+          }
+        }
+        const u64 before = sf_scan(w, sh.red, total);
+        for (int r = 0; r < grp.blocks; ++r) total += rests[r];
+        budget = (u64)(fmax((double)top_p, 0.0) * (double)total);
+        if (tid < grp.blocks) *grp.at(&sh.budget, tid) = budget, *grp.at(&sh.state, tid) = -1;
+        __syncthreads();
+        if (before <= budget && before + w > budget) {
+          for (int r = 0; r < grp.blocks; ++r) *grp.at(&sh.state, r) = tid;
+          sh.above = before;
+        }
       }
-      __syncthreads();
-      const int d = sh.pick;
-      const u64 above = sh.found;
-      if (d >= 0) {
-        const int n = sf_gather(row, list, &sh.count, [&](float x) { return x > -INFINITY && bin(x) == d; });
-        sf_sort(list, n);
-        float x[2];
-        u64 v[2];
+      grp.sync();
+      budget = sh.budget;
+      const float d0 = (float)sh.state, d1 = d0 + 1.f;
+      int n = kSfList + 1;
+      if (sh.state >= 0)
+        n = sf_gather(row, grp, list, sh, [&](float x) {
+          const float d = (top - x) * scale;
+          return d >= d0 && d < d1;
+        });
+      if (n <= kSfList) {
+        if (chief) {
+          sf_sort(list, n);
+          float x[2];
+          u64 v[2], total;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * tid + e;
-          x[e] = i < n ? sf_unkey((uint32_t)(list[i] >> 32)) : -INFINITY;
-          v[e] = i < n ? weigh.of(x[e]) : 0;
+          for (int e = 0; e < 2; ++e) {
+            const int i = 2 * tid + e;
+            x[e] = i < n ? sf_unkey((uint32_t)(list[i] >> 32)) : -INFINITY;
+            v[e] = i < n ? weigh.of(x[e]) : 0;
+          }
+          const u64 start = sh.above + sf_scan(v[0] + v[1], sh.red, total);
+          int stay = 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) stay += 2 * tid + e < n && start + (e ? v[0] : 0) <= budget;
+          stay = sf_sum(stay, sh.ired);  // at least 1: the bin's first token has `above` <= budget before it
+          const float last = sf_unkey((uint32_t)(list[stay - 1] >> 32));
+          int equal = 0, ties = 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool same = 2 * tid + e < n && x[e] == last;
+            equal += same;
+            ties += same && 2 * tid + e < stay;
+          }
+          equal = sf_sum(equal, sh.ired);
+          ties = sf_sum(ties, sh.ired);
+          if (tid < grp.blocks) *grp.at(&sh.cut, tid) = Cut{last, ties == equal ? kSfAll : ties};
         }
-        const u64 start = above + sf_scan(v[0] + v[1], sh.red, total);
-        int stay = 0;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) stay += 2 * tid + e < n && start + (e ? v[0] : 0) <= budget;
-        stay = sf_sum(stay, sh.ired);  // at least 1: the bin's first token has `above` <= budget before it
-        const float last = sf_unkey((uint32_t)(list[stay - 1] >> 32));
-        int equal = 0, ties = 0;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool same = 2 * tid + e < n && x[e] == last;
-          equal += same;
-          ties += same && 2 * tid + e < stay;
-        }
-        equal = sf_sum(equal, sh.ired);
-        ties = sf_sum(ties, sh.ired);
-        cut = Cut{last, ties == equal ? kSfAll : ties};
+        grp.sync();
+        cut = sh.cut;
         found = true;
       }
+    } else {
+      u64 m = 0;
+      row.each4([&](const float(&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m += x[j] > cut.x ? weigh.of(x[j]) : 0;
+      });
+      const u64* all = grp.share(sh.bmass, sf_sum(m, sh.red));
+      m = (u64)cut.ties * weigh.of(cut.x);
+      for (int r = 0; r < grp.blocks; ++r) m += all[r];
+      budget = (u64)(fmax((double)top_p, 0.0) * (double)m);
     }
-    if (!found) cut = sf_radix_cut(row, weigh, cut, true, budget, cnt, lo, hi);
+    if (!found) cut = sf_radix_cut(row, grp, weigh, cut, true, budget, cnt, lo, hi);
   }
 
-  // ---- the draw over the row: every warp owns a run of the vocabulary, a lane four neighbouring tokens at a time
-  const int run = (V + kSfWarps * 128 - 1) / (kSfWarps * 128) * 128, i0 = min(V, wid * run), i1 = min(V, i0 + run);
+  // ---- the draw: every warp owns a run of the slice, a lane four neighbouring tokens at a time
+  const int run = (p.slice + kSfWarps * 128 - 1) / (kSfWarps * 128) * 128;
+  const int i0 = min(row.to, row.from + wid * run), i1 = min(row.to, i0 + run);
   const bool count_ties = cut.ties != kSfAll;
   // tokens below this are not kept: the cut, and a bound of min_p's that leaves the comparison to the weights
   const float floor_p = min_p > 0.f ? fminf(top + logf(min_p) - 0.01f - 1e-5f * fabsf(top), top) : -INFINITY;
@@ -734,6 +915,8 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
     __syncthreads();
     int all;
     tie0 = sf_warps(sh.ired, wid, all);
+    const int* theirs = grp.share(sh.bcount, all);
+    for (int r = 0; r < grp.rank; ++r) tie0 += theirs[r];
     int tie = tie0;
     for (int i = i0; i < i1; i += 128) {
       const float4 v = i + 4 * lane < i1 ? row.x4(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -761,10 +944,24 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   __syncthreads();
   if (lane == 0) sh.red[wid] = mass, sh.ired[wid] = count;
   __syncthreads();
-  u64 total;
+  u64 total, before = sf_warps(sh.red, wid, total);
   int kept;
-  u64 before = sf_warps(sh.red, wid, total);
   sf_warps(sh.ired, wid, kept);
+  const u64 here = total;
+  if (grp.blocks > 1) {
+    const u64* masses = grp.share(sh.bmass, total);
+    const int* counts = grp.share(sh.bcount, kept);  // the last use of another block's memory
+    total = 0, kept = 0;
+    u64 ahead = 0;
+    for (int r = 0; r < grp.blocks; ++r) {
+      if (r < grp.rank) ahead += masses[r];
+      total += masses[r];
+      kept += counts[r];
+    }
+    before += ahead;
+    const u64 target = min((u64)((double)u * (double)total), total - 1);
+    if (target < ahead || target >= ahead + here) return;
+  }
   const u64 target = min((u64)((double)u * (double)total), total - 1);  // total >= 2^S: the first token is kept
   if (lane == 0 && target >= before && target < before + mass) {
     sh.pick = wid;
@@ -775,7 +972,7 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   // ... and the whole block walks the run that holds the target
   before = sh.found;
   int tie = sh.count;
-  const int first = sh.pick * run, end = min(V, first + run);
+  const int first = row.from + sh.pick * run, end = min(row.to, first + run);
   for (int i = first; i < end; i += 4 * kSfThreads) {
     const int at = i + 4 * tid;
     const float4 v = at < end ? row.x4(at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -818,11 +1015,46 @@ int launch_sample(SampleArgs p, int batch, cudaStream_t s) {
   static SmemLimit limit;
   const auto fn = sample_filtered_kernel<T>;
   const int list = kSfList * 8 + kSfWarps * 64 * 4, most = 232448 - 2048;  // 227 KB per block less the static part
-  p.in_shared = p.vocab <= (most - list) / 16 * 4;
-  const int bytes = list + (p.in_shared ? (p.vocab * 4 + 15) / 16 * 16 : 0);
-  DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  fn<<<batch, kSfThreads, bytes, s>>>(p);
-  DFSSM_CU(cudaGetLastError());
+  const int capacity = (most - list) / 512 * 128;
+  DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), list + capacity * 4));
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(kSfThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  // Blocks per row: the number that takes the fewest waves x (tokens per block + what a block costs apart from its
+  // tokens), in tokens.  Measured at 50,280 logits: a pass over a block's tokens costs 0.2 to 0.6 cycles a token, the
+  // rest of a block about 12,000 cycles; tokens that do not fit shared memory cost about half as much again.
+  // rows_at_once: the clusters of that size that run together with a full block per SM (B200: 148, 74, 45, 33, ...).
+  static std::atomic<int> rows_at_once[kSfBlocks + 1];
+  int blocks = 1;
+  long long least = 0;
+  for (int n = 1; n <= kSfBlocks && (n == 1 || p.vocab >= 4096 * n); ++n) {
+    int rows = rows_at_once[n].load(std::memory_order_relaxed);
+    if (rows == 0) {
+      cfg.gridDim = dim3(1, n);
+      cfg.dynamicSmemBytes = list + capacity * 4;
+      cluster.val.clusterDim.y = n;
+      cfg.numAttrs = 1;
+      DFSSM_CU(cudaOccupancyMaxActiveClusters(&rows, fn, &cfg));
+      if (rows < 1) rows = 1;
+      rows_at_once[n].store(rows, std::memory_order_relaxed);
+    }
+    const long long slice = (p.vocab + n - 1) / n, waves = (batch + rows - 1) / rows;
+    const long long cost = waves * ((slice <= capacity ? slice : slice + slice / 2) + 12000);
+    if (n == 1 || cost < least) blocks = n, least = cost;
+    if (batch >= 2 * rows) break;  // more blocks per row only add waves
+  }
+  p.slice = ((p.vocab + blocks - 1) / blocks + 127) / 128 * 128;
+  p.in_shared = p.slice <= capacity;
+  const int bytes = list + (p.in_shared ? p.slice * 4 : 0);
+  cfg.gridDim = dim3(batch, blocks);
+  cfg.dynamicSmemBytes = bytes;
+  cluster.val.clusterDim.y = blocks;
+  cfg.numAttrs = blocks > 1 ? 1 : 0;
+  DFSSM_CU(cudaLaunchKernelEx(&cfg, fn, p));
   return DFSSM_OK;
 }
 
@@ -844,7 +1076,7 @@ extern "C" int dfssm_sample_filtered(const void* logits, int64_t ld, int dtype, 
   int bits = 0;
   while ((1 << bits) < vocab) ++bits;
   SampleArgs p{logits,      ld,   vocab,      temperature, top_p,     min_p, uniform, top_k,
-               seen_bits, rep_penalty, next, kept_count, prob,        62 - bits > 50 ? 50 : 62 - bits, 0};
+               seen_bits, rep_penalty, next, kept_count, prob,        62 - bits > 50 ? 50 : 62 - bits, 0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == DFSSM_F32) return launch_sample<float>(p, batch, s);
   if (dtype == DFSSM_F16) return launch_sample<__half>(p, batch, s);
