@@ -14,6 +14,9 @@ import torch
 
 from . import _lib
 
+# The handle of a device's current stream; torch.cuda.current_stream() also makes a Stream object, 2 us a call.
+_stream_of = torch._C._cuda_getCurrentRawStream
+
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
@@ -37,10 +40,9 @@ def _on(t, name: str, device=None):
 
 def _vector(t, name: str, n: int, dtype, device):
     """Pointer of a contiguous [n]."""
-    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != (n,)
-            or (n > 1 and t.stride(0) != 1)):
-        _refuse(t, name, f"a contiguous {dtype} vector of {n}", device)
-    return t.data_ptr()
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(t, name, f"a contiguous {dtype} vector of {n}", device)
 
 
 def _heads(t, name: str, shape, dtype, device):
@@ -68,11 +70,12 @@ def _gates(t, name: str, shape, dtype, device):
 
 def _call(device, fn, *args):
     """Runs a C entry on `device`, on its current stream (the last argument)."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.check(fn(*args, _stream_of(index)))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            _lib.check(fn(*args, _stream_of(index)))
 
 
 def _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale):
@@ -90,7 +93,7 @@ def _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale):
             or state.shape[1:] != (hv, dv, dk) or not state.is_contiguous()):
         _refuse(state, "state", f"contiguous fp32 [slots, {hv}, {dv}, {dk}]", dev)
     if out is None:
-        out = torch.empty(values, dtype=dtype, device=dev)
+        out = v.new_empty(values)
     head = (*_heads(q, "q", keys, dtype, dev), *_heads(k, "k", keys, dtype, dev), *_heads(v, "v", values, dtype, dev),
             *_gates(a, "a", (n, hv), dtype, dev), *_gates(b, "b", (n, hv), dtype, dev),
             _vector(A_log, "A_log", hv, torch.float32, dev), _vector(dt_bias, "dt_bias", hv, torch.float32, dev),
@@ -136,7 +139,7 @@ def gated_delta_prefill(q, k, v, a, b, A_log, dt_bias, state, cu_seqlens, *, slo
     lib = _lib.load()
     need = lib.dfssm_gated_delta_workspace(dims[0], n_seq, *dims[1:])
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = v.new_empty(need, dtype=torch.uint8)
     elif (not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.device != dev
           or not workspace.is_contiguous() or workspace.numel() < need):
         _refuse(workspace, "workspace", f"contiguous uint8 of at least {need} bytes", dev)
@@ -184,8 +187,7 @@ def sample_filtered(logits, uniform, *, temperature=None, top_k=None, top_p=None
                 or seen_bits.shape != (B, (V + 31) // 32) or not seen_bits.is_contiguous()):
             _refuse(seen_bits, "seen_bits", f"contiguous int32 [{B}, {(V + 31) // 32}]", dev)
     if out is None:
-        out = (torch.empty(B, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev),
-               torch.empty(B, dtype=torch.float32, device=dev))
+        out = (uniform.new_empty(B, dtype=torch.int32), uniform.new_empty(B, dtype=torch.int32), uniform.new_empty(B))
     token, kept, prob = out
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     _call(dev, _lib.load().dfssm_sample_filtered, logits.data_ptr(), ld, _DTYPES[logits.dtype], B, V, ptr(temperature),
