@@ -150,19 +150,20 @@ int launch_loop(const GatedDeltaArgs& p, int dk, int dtype, cudaStream_t s) {
 
 size_t gd_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dtype) {
   const size_t n = (size_t)gd_chunk_slots(tokens, n_seq);
-  return n * v_heads * kGdBlock + (dtype == DFSSM_BF16 ? n * k_heads * 2 * kGdC * dk * 2 : 0);
+  return n * v_heads * kGdBlock + (dtype == DFSSM_BF16 ? n * k_heads * 2 * kGdC * dk * 2 : 0) + (size_t)n_seq * 16;
 }
 
-template <typename T, int DK, int W>
-int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16, int slots_total, cudaStream_t s) {
+template <typename T, int DK, int W, bool DEEP>
+int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16, const int4* order, int slots_total,
+                cudaStream_t s) {
   static SmemLimit limit;
-  constexpr int bytes = gd_chunk_smem<DK, W>();
-  const auto fn = gated_delta_chunk_kernel<T, DK, W>;
+  constexpr int bytes = gd_chunk_smem<DK, W, DEEP>();
+  const auto fn = gated_delta_chunk_kernel<T, DK, W, DEEP>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
   const int parts = (p.dv + 16 * W - 1) / (16 * W);
   const long long grid = (long long)p.n_seq * p.v_heads * parts;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
-  fn<<<(unsigned)grid, 64 * W, bytes, s>>>(p, blocks, kq16, parts, slots_total);
+  fn<<<(unsigned)grid, 64 * W, bytes, s>>>(p, blocks, kq16, order, parts, slots_total);
   DFSSM_CU(cudaGetLastError());
   return DFSSM_OK;
 }
@@ -182,11 +183,23 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
+  int dev = 0, sms = 0;
+  DFSSM_CU(cudaGetDevice(&dev));
+  DFSSM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const long long walks = (long long)p.n_seq * p.v_heads * ((p.dv + 31) / 32);
+  // The sequences by falling length (a long one that starts last runs alone), with their slots looked up.  It costs
+  // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself.
+  int4* order = p.n_seq <= 512 ? reinterpret_cast<int4*>(workspace + gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK,
+                                                                                 std::is_same<T, __half>::value ? DFSSM_F16 : DFSSM_BF16) -
+                                                         (size_t)p.n_seq * 16)
+                               : nullptr;
   const auto fn = gated_delta_prep_kernel<T, DK>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, groups, per_group);
+  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group);
   DFSSM_CU(cudaGetLastError());
-  return launch_walk<T, DK, 2>(p, workspace, kq16, (int)n, s);
+  static const int deep = getenv("DFSSM_GD_DEEP") ? atoi(getenv("DFSSM_GD_DEEP")) : 0;
+  return walks <= sms || deep ? launch_walk<T, DK, 2, true>(p, workspace, kq16, order, (int)n, s)  // every block has an SM
+                      : launch_walk<T, DK, 2, false>(p, workspace, kq16, order, (int)n, s);
 }
 
 // What both entry points ask of their arguments.

@@ -235,11 +235,12 @@ constexpr unsigned long long frag_rows() {
 }
 constexpr unsigned long long kFragRow = frag_rows();
 
-// kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.
+// kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.  walks, if not
+// NULL: [n_seq], for the chunk kernel: {first token, tokens, slot or -1, number} of the sequences by falling length.
 template <typename T, int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4)
-gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __half* __restrict__ kq16, int groups,
-                        int per_group) {
+gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __half* __restrict__ kq16,
+                        int4* __restrict__ walks, int groups, int per_group) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int UPR = DK / 8;  // 16-byte units per row
   extern __shared__ __align__(128) char smem[];
@@ -259,6 +260,21 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   const int rep = p.v_heads / p.k_heads;
   const int grp = blockIdx.x % groups, hk = (blockIdx.x / groups) % p.k_heads, num = blockIdx.x / (groups * p.k_heads);
+  if (walks && blockIdx.x == 0) {
+    for (int i = tid; i < p.n_seq; i += kPrepThreads) {
+      int first, count, place = 0;
+      gd_range(p.cu, i, p.tokens, first, count);
+      const int slot = p.slots ? p.slots[i] : i;
+      bool mine = slot >= 0 && slot < p.n_slots;
+      for (int j = 0; j < p.n_seq; ++j) {
+        int f, n;
+        gd_range(p.cu, j, p.tokens, f, n);
+        place += n > count || (n == count && j < i);
+        if (p.slots && j < i && p.slots[j] == slot) mine = false;
+      }
+      walks[place] = make_int4(first, count, mine ? slot : -1, i);
+    }
+  }
   // the sequence of chunk `num`: the last one whose first chunk is not behind it
   int lo = 0, hi = p.n_seq - 1;
   while (lo < hi) {
@@ -572,7 +588,8 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 // second, the output warp, takes the operands that the first has split anyway (S and u as fp16 pairs, through
 // shared memory) and computes S q + u P^T and the rows of o; it also fetches the next chunk (cp.async): K is
 // double buffered, and Q, V, T, P and the factors are replaced as soon as they have been read, so that two
-// blocks of two pairs fit on an SM.  All products are taken transposed, with S, r and u as left operands: the
+// blocks of two pairs fit on an SM.  DEEP, for grids that give every block an SM of its own, has two of all of them and
+// fetches a chunk ahead: XXX us a chunk instead of YYY.  All products are taken transposed, with S, r and u as left operands: the
 // accumulator layout of one product is the left operand's layout of the next, so nothing of the chain itself
 // passes through shared memory.
 //   S k, S q : [16 x dk] [dk x 64]     u = r T^T, u P^T : [16 x 64] [64 x 64]     u k : [16 x 64] [64 x dk]
@@ -584,9 +601,9 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 
 template <int DK>
 __host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 192; }
-template <int DK, int W>
+template <int DK, int W, bool DEEP>
 __host__ __device__ constexpr int gd_chunk_smem() {
-  return 3 * kGdC * DK * 2 + kGdC * 32 * W + kGdBlock + W * gd_exchange<DK>();
+  return (DEEP ? 4 : 3) * kGdC * DK * 2 + (DEEP ? 2 : 1) * (kGdC * 32 * W + kGdBlock) + W * gd_exchange<DK>();
 }
 
 // Byte offset of 16-byte unit u of token t in the V tile [64][16 W].
@@ -595,7 +612,8 @@ __device__ __forceinline__ uint32_t v_off(int t, int u) {
   const int f = W >= 4 ? (t & 7) : (W == 2 ? ((t >> 1) & 3) : ((t >> 2) & 1));
   return (uint32_t)(t * 32 * W + ((u ^ f) << 4));
 }
-// Named barriers: 0 the block, 1 the output warps, 2 + 2 pair + {0: u is split, 1: S and u have been taken}
+// Named barriers: 0 the block, 1 the output warps, 2 + 4 pair + {0: u is split, 1: S and u have been taken, 2: the
+// first half of S is split, 3: all of it}
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -645,43 +663,52 @@ __device__ __forceinline__ float pair_max(unsigned a, unsigned b, __nv_bfloat16)
 }
 
 // kq16: the fp16 tiles of K and Q for bf16 inputs; for fp16 inputs the tiles are rows of k and q themselves.
-template <typename T, int DK, int W>
-__global__ void __launch_bounds__(64 * W, W == 2 ? 2 : 1)
+template <typename T, int DK, int W, bool DEEP>
+__global__ void __launch_bounds__(64 * W, DEEP ? 1 : 2)
 gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
-                         int parts, int slots_total) {
+                         const int4* __restrict__ walks, int parts, int slots_total) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int NT = 64 * W, NL = 32 * W, NK = DK / 8, UPR = DK / 8;
-  constexpr int TILE = kGdC * DK * 2, V_AT = 3 * TILE, B_AT = V_AT + kGdC * 32 * W;  // K, K, Q, V, {T, P, factors}
+  constexpr int TILE = kGdC * DK * 2;
+  constexpr int V_AT = (DEEP ? 4 : 3) * TILE, B_AT = V_AT + kGdC * 32 * W;  // K, K, Q (DEEP: twice), V, {T, P, factors}
+  constexpr int STAGE = kGdC * 32 * W + kGdBlock;  // V and the rest (DEEP: two of them)
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int part = blockIdx.x % parts, h = (blockIdx.x / parts) % p.v_heads, seq = blockIdx.x / (parts * p.v_heads);
-  int first, count;
-  gd_range(p.cu, seq, p.tokens, first, count);
-  const int base = gd_chunk_base(p.cu, seq, p.tokens);
-  // Two blocks of two pairs share an SM's four schedulers: the one in the upper warp slots swaps its roles, so that
-  // each scheduler gets a chain and an output warp and not two of a kind (only speed depends on it).
-  __shared__ int upper;
-  if (W == 2 && tid == 0) {
-    unsigned w;
-    asm volatile("mov.u32 %0, %%warpid;" : "=r"(w));
-    upper = (w >> 2) & 1;
+  const int part = blockIdx.x % parts, h = (blockIdx.x / parts) % p.v_heads, nth = blockIdx.x / (parts * p.v_heads);
+  int first, count, slot, seq;
+  if (walks) {
+    const int4 w = walks[nth];
+    first = w.x, count = w.y, slot = w.z, seq = w.w;
+  } else {
+    seq = nth;
+    gd_range(p.cu, seq, p.tokens, first, count);
+    slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
   }
-  const int slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
+  // Roles by scheduler.  A block's four warps sit on the SM's four schedulers in an order of the hardware's own (warp slot
+  // modulo 4), and two blocks share an SM, one in slots 0-3 and one in 4-7: the first has its chain warps on
+  // schedulers 0 and 1, the other on 2 and 3, so that no scheduler gets two chains.  Only speed depends on it: where
+  // the slots are not as described the warps' numbers serve.
+  static_assert(W == 2, "four warps");
+  __shared__ unsigned place[2 * W];
+  if (lane == 0) asm volatile("mov.u32 %0, %%warpid;" : "=r"(place[wid]));
   __syncthreads();
   if (slot < 0 || count == 0) return;
+  const int base = first / kGdC + seq;  // gd_chunk_base
   const int chunks = min((count + kGdC - 1) / kGdC, slots_total - base);
   const int hk = h / (p.v_heads / p.k_heads);
-  const bool chain = W == 2 ? (wid < W) != (upper != 0) : wid < W;
-  const int pair = wid % W;
+  unsigned seen = 0;
+#pragma unroll
+  for (int i = 0; i < 2 * W; ++i) seen |= 1u << (place[i] & 3);
+  const int at = seen == 15u ? (int)(place[wid] & 3) : wid;
+  const bool chain = (at < W) != (((place[0] >> 2) & 1) != 0);
+  const int pair = at % W;
   const int dv0 = part * 16 * W, row0 = dv0 + 16 * pair;
   const bool active = row0 < p.dv;  // dv is a multiple of 16: a pair's rows are all there or none
-  char* ex = smem + B_AT + kGdBlock + pair * gd_exchange<DK>();
+  char* ex = smem + V_AT + (DEEP ? 2 : 1) * STAGE + pair * gd_exchange<DK>();
   uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;                   // S: [dk / 16][hi, lo][32]
   uint4* u_ex = reinterpret_cast<uint4*>(ex + DK / 16 * 1024) + lane;  // u: [4][hi, lo][32]
   float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);    // [3][16] the rows' scales of S and u, and max |v|
-  const int bar = 2 + 2 * pair;
-  const uint32_t q_s = smem_u32(smem) + 2 * TILE, v_s = smem_u32(smem) + V_AT;
-  const float* vec = reinterpret_cast<const float*>(smem + B_AT + 2 * kGdTri);
+  const int bar = 2 + 4 * pair;
   // lane parts of the ldmatrix addresses
   const int bt = ((lane >> 4) << 3) + (lane & 7), bu = (lane >> 3) & 1;  // B from [token][dk] rows, two n-tiles
   const int tt = (((lane >> 3) & 1) << 3) + (lane & 7), tu = lane >> 4;  // the same, transposed
@@ -690,7 +717,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     // ---------------------------------------------------------------- output warp
     // A lane copies one 16-byte column of every RP-th row (K, Q), so that a copy costs a pointer step; rows past
     // the sequence's end are zeros.
-    const int lt = tid % NL;
+    const int lt = pair * 32 + lane;
     constexpr int RP = NL / UPR;  // rows per pass: 4 to 16
     const uint32_t sm0 = smem_u32(smem);
     const int kt = lt / UPR, ku = lt % UPR;
@@ -717,11 +744,12 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       }
     };
     auto load_k = [&](int ch) { load_tile(ch, sm0 + (ch & 1) * TILE, p.k, p.ld_k, 0); };
-    auto load_q = [&](int ch) { load_tile(ch, q_s, p.q, p.ld_q, 1); };
+    auto load_q = [&](int ch) { load_tile(ch, sm0 + (2 + (DEEP ? ch & 1 : 0)) * TILE, p.q, p.ld_q, 1); };
     const int vu = lt % (2 * W), vt = lt / (2 * W);  // 16 rows of V per pass
     const bool v_there = dv0 + vu * 8 < p.dv;
     auto load_vb = [&](int ch) {  // V, T, P and the factors of chunk ch
-      const int n = count - ch * kGdC;
+      const int n = count - ch * kGdC, stage = DEEP ? (ch & 1) * STAGE : 0;
+      const uint32_t v_s = sm0 + V_AT + stage;
       const T* src = static_cast<const T*>(p.v) + ((size_t)first + (size_t)ch * kGdC + vt) * p.ld_v + h * p.dv + dv0 + vu * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i, src += (size_t)16 * p.ld_v) {
@@ -729,44 +757,68 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         cp16(v_s + v_off<W>(vt + 16 * i, vu), ok ? src : static_cast<const T*>(p.v), ok);
       }
       const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock + lt * 16;
-      const uint32_t dst = sm0 + B_AT + lt * 16;
+      const uint32_t dst = sm0 + B_AT + stage + lt * 16;
 #pragma unroll
       for (int i = 0; i < kGdBlock / 16 / NL; ++i) cp16(dst + i * NL * 16, blk + i * NL * 16, true);
       constexpr int REST = kGdBlock / 16 % NL;
       if (lt < REST) cp16(dst + kGdBlock / 16 / NL * NL * 16, blk + kGdBlock / 16 / NL * NL * 16, true);
     };
+    // the largest |v| of each row of chunk ch, for the chain's bound of r
+    auto largest_v = [&](int ch) {
+      const uint32_t v_s = sm0 + (DEEP ? (ch & 1) * STAGE : 0) + V_AT;
+      float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int jp = 0; jp < 4; ++jp) {
+        unsigned v[4];
+        ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
+        v0 = fmaxf(v0, pair_max(v[0], v[1], T()));
+        v1 = fmaxf(v1, pair_max(v[2], v[3], T()));
+      }
+      v0 = quad_max(v0);
+      v1 = quad_max(v1);
+      if (c == 0) sc[32 + g] = v0, sc[40 + g] = v1;
+    };
     load_k(0);
     load_q(0);
-    cp_commit();
+    if (!DEEP) cp_commit();
     load_vb(0);
     cp_commit();
+    if constexpr (DEEP) {
+      cp_wait<0>();
+      bar_sync(1, NL);
+      largest_v(0);
+      bar_arrive(0, NT);  // the chunk is there
+    }
     for (int ch = 0; ch < chunks; ++ch) {
       const bool more = ch + 1 < chunks;
-      cp_wait<1>();
-      bar_sync(0, NT);  // K and Q are there, and nobody reads the other K any more
-      if (more) load_k(ch + 1);
-      cp_commit();
-      cp_wait<1>();
-      bar_sync(1, NL);  // V, T, P and the factors are there
-      {  // the largest |v| of each row, for the chain's bound of r
-        float v0 = 0.f, v1 = 0.f;
-#pragma unroll
-        for (int jp = 0; jp < 4; ++jp) {
-          unsigned v[4];
-          ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
-          v0 = fmaxf(v0, pair_max(v[0], v[1], T()));
-          v1 = fmaxf(v1, pair_max(v[2], v[3], T()));
-        }
-        v0 = quad_max(v0);
-        v1 = quad_max(v1);
-        if (c == 0) sc[32 + g] = v0, sc[40 + g] = v1;
+      const char* st = smem + (DEEP ? (ch & 1) * STAGE : 0);
+      const uint32_t v_s = smem_u32(st) + V_AT;
+      const float* vec = reinterpret_cast<const float*>(st + B_AT + 2 * kGdTri);
+      if constexpr (!DEEP) {
+        cp_wait<1>();
+        bar_sync(0, NT);  // K and Q are there, and nobody reads the other K any more
+        if (more) load_k(ch + 1);
+        cp_commit();
+        cp_wait<1>();
+        bar_sync(1, NL);  // V, T, P and the factors are there
+        largest_v(ch);
       }
-      bar_sync(0, NT);  // the chains have split S; V, T, P and the factors are there for them too
+      const uint32_t q_s = smem_u32(smem) + (2 + (DEEP ? ch & 1 : 0)) * TILE;
       float o[8][4];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      bar_sync(bar + 2, 64);  // half of S is split
+      if constexpr (DEEP) {
+        bar_sync(1, NL);  // every chain is past the last chunk, and so are the output warps: the other stage is free
+        if (more) load_k(ch + 1), load_q(ch + 1), load_vb(ch + 1);
+        cp_commit();
+      }
 #pragma unroll
       for (int kk = 0; kk < DK / 16; ++kk) {
+        if (kk == DK / 32) {
+          if constexpr (DEEP) bar_sync(bar + 3, 64);  // all of S is split
+          else bar_sync(0, NT);  // the same of all chains; V, T, P and the factors are there for them too
+        }
         const uint4 hv = s_ex[(2 * kk) * 32], lv = s_ex[(2 * kk + 1) * 32];
         const unsigned ah[4] = {hv.x, hv.y, hv.z, hv.w}, al[4] = {lv.x, lv.y, lv.z, lv.w};
         unsigned b[4][4];
@@ -778,9 +830,11 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         for (int j = 0; j < 8; ++j) mma_acc(o[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
       }
       const float ds0 = sc[g], ds1 = sc[g + 8];
-      bar_sync(1, NL);  // Q is free
-      if (more) load_q(ch + 1);
-      cp_commit();
+      if constexpr (!DEEP) {
+        bar_sync(1, NL);  // Q is free
+        if (more) load_q(ch + 1);
+        cp_commit();
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float2 oq = *reinterpret_cast<const float2*>(vec + kGdOq + 8 * j + 2 * c);
@@ -799,12 +853,19 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       }
       const float du0 = sc[16 + g], du1 = sc[24 + g];
       if (more) bar_arrive(bar + 1, 64);
-      const uint4* Pf = reinterpret_cast<const uint4*>(smem + B_AT + kGdTri) + lane;
+      if (DEEP && more) {
+        cp_wait<0>();
+        bar_sync(1, NL);
+        largest_v(ch + 1);
+        bar_arrive(0, NT);  // the next chunk is there
+      }
+      const uint4* Pf = reinterpret_cast<const uint4*>(st + B_AT + kGdTri) + lane;
+      float x0[4][4] = {}, x1[4][4] = {};
+      tri_product<0>(x0, ah, al, Pf);
+      tri_product<4>(x1, ah, al, Pf);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float x[4][4] = {};
-        if (half == 0) tri_product<0>(x, ah, al, Pf);
-        else tri_product<4>(x, ah, al, Pf);
+        float(&x)[4][4] = half ? x1 : x0;
 #pragma unroll
         for (int jp = 0; jp < 2; ++jp) {
           unsigned out[4];
@@ -832,12 +893,14 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
           const int t = 16 * i + (lane >> 1);
           if (t < count - ch * kGdC)
             *reinterpret_cast<uint4*>(og + (size_t)t * p.ld_o + (lane & 1) * 8) =
-                *reinterpret_cast<const uint4*>(smem + V_AT + v_off<W>(t, 2 * pair + (lane & 1)));
+                *reinterpret_cast<const uint4*>(st + V_AT + v_off<W>(t, 2 * pair + (lane & 1)));
         }
       }
-      bar_sync(1, NL);  // V, T, P and the factors are free: the chains left them before their u was split
-      if (more) load_vb(ch + 1);
-      cp_commit();
+      if constexpr (!DEEP) {
+        bar_sync(1, NL);  // V, T, P and the factors are free: the chains left them before their u was split
+        if (more) load_vb(ch + 1);
+        cp_commit();
+      }
     }
     cp_wait<0>();
     return;
@@ -859,6 +922,9 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   }
   for (int ch = 0; ch < chunks; ++ch) {
     const uint32_t k_s = smem_u32(smem) + (ch & 1) * TILE;
+    const char* st = smem + (DEEP ? (ch & 1) * STAGE : 0);
+    const uint32_t v_s = smem_u32(st) + V_AT;
+    const float* vec = reinterpret_cast<const float*>(st + B_AT + 2 * kGdTri);
     m0 = quad_max(m0);
     m1 = quad_max(m1);
     float up0, dn0, up1, dn1;
@@ -868,7 +934,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     if (c == 0) sc[g] = dn0, sc[g + 8] = dn1;
     unsigned sh[2][4], sl[2][4];
     split_tile(s[0], s[1], up0, up1, sh[0], sl[0]);
-    bar_sync(0, NT);  // K and Q are there
+    bar_sync(0, NT);  // K and Q are there (DEEP: the whole chunk)
     float ks[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) ks[j][0] = ks[j][1] = ks[j][2] = ks[j][3] = 0.f;
@@ -882,12 +948,14 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       s_ex[(2 * kk) * 32] = make_uint4(sh[now][0], sh[now][1], sh[now][2], sh[now][3]);
       s_ex[(2 * kk + 1) * 32] = make_uint4(sl[now][0], sl[now][1], sl[now][2], sl[now][3]);
       if (kk + 1 < DK / 16) split_tile(s[2 * kk + 2], s[2 * kk + 3], up0, up1, sh[now ^ 1], sl[now ^ 1]);
+      if (kk == DK / 32 - 1) bar_arrive(bar + 2, 64);  // half of S is split
 #pragma unroll
       for (int j = 0; j < 8; ++j) mma_acc(ks[j], sl[now], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) mma_acc(ks[j], sh[now], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
     }
-    bar_sync(0, NT);  // V, T, P and the factors are there; S is split
+    if constexpr (DEEP) bar_arrive(bar + 3, 64);  // S is split
+    else bar_sync(0, NT);                         // ... and V, T, P and the factors are there
     // bounds of r and u, and the scales from them
     const float root = DK == 128 ? 11.3137085f : 8.f;
     const float r0 = fmaf(root * vec[kGdKn], m0, sc[32 + g]), r1 = fmaf(root * vec[kGdKn], m1, sc[40 + g]);
@@ -915,7 +983,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       }
       split_tile(ks[2 * jp], ks[2 * jp + 1], ur0, ur1, ah[jp], al[jp]);
     }
-    const uint4* Tf = reinterpret_cast<const uint4*>(smem + B_AT) + lane;
+    const uint4* Tf = reinterpret_cast<const uint4*>(st + B_AT) + lane;
     float x0[4][4] = {}, x1[4][4] = {};  // u, scaled as r and T are
     tri_product<0>(x0, ah, al, Tf);
     tri_product<4>(x1, ah, al, Tf);
