@@ -2,7 +2,6 @@
 #include "gated_delta_chunk.cuh"
 
 #include <cmath>
-#include <cstdlib>
 
 #include "op_host.h"
 
@@ -153,17 +152,17 @@ size_t gd_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int
   return n * v_heads * kGdBlock + (dtype == DFSSM_BF16 ? n * k_heads * 2 * kGdC * dk * 2 : 0) + (size_t)n_seq * 16;
 }
 
-template <typename T, int DK, int W, bool DEEP>
+template <typename T, int DK, bool DEEP>
 int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16, const int4* order, int slots_total,
                 cudaStream_t s) {
   static SmemLimit limit;
-  constexpr int bytes = gd_chunk_smem<DK, W, DEEP>();
-  const auto fn = gated_delta_chunk_kernel<T, DK, W, DEEP>;
+  constexpr int bytes = gd_chunk_smem<DK, DEEP>();
+  const auto fn = gated_delta_chunk_kernel<T, DK, DEEP>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  const int parts = (p.dv + 16 * W - 1) / (16 * W);
+  const int parts = (p.dv + 16 * kGdPairs - 1) / (16 * kGdPairs);
   const long long grid = (long long)p.n_seq * p.v_heads * parts;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
-  fn<<<(unsigned)grid, 64 * W, bytes, s>>>(p, blocks, kq16, order, parts, slots_total);
+  fn<<<(unsigned)grid, 64 * kGdPairs, bytes, s>>>(p, blocks, kq16, order, parts, slots_total);
   DFSSM_CU(cudaGetLastError());
   return DFSSM_OK;
 }
@@ -174,18 +173,18 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   constexpr int bytes = gd_prep_smem<DK>();
   const long long n = gd_chunk_slots(p.tokens, p.n_seq);
   const int rep = p.v_heads / p.k_heads;
-  static const int pg = getenv("DFSSM_GD_PG") ? atoi(getenv("DFSSM_GD_PG")) : 0;
-  int per_group = pg ? pg : 4;
-  if (per_group > rep) per_group = rep;
-  while (per_group > 1 && n * p.k_heads * ((rep + per_group - 1) / per_group) < 600) per_group /= 2;
+  int dev = 0, sms = 0;
+  DFSSM_CU(cudaGetDevice(&dev));
+  DFSSM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  // Heads of one key per prep block: the more, the less is computed twice, as long as there are blocks for every SM
+  // (64 heads on one key, 64 prompts of 64 tokens, whole call: 265 us with 2, 254 with 4, 247 with 8, 246 with 16).
+  int per_group = rep < 8 ? rep : 8;
+  while (per_group > 1 && n * p.k_heads * ((rep + per_group - 1) / per_group) < 4 * sms) per_group /= 2;
   const int groups = (rep + per_group - 1) / per_group;
   const long long grid = n * p.k_heads * groups;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
-  int dev = 0, sms = 0;
-  DFSSM_CU(cudaGetDevice(&dev));
-  DFSSM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const long long walks = (long long)p.n_seq * p.v_heads * ((p.dv + 31) / 32);
   // The sequences by falling length (a long one that starts last runs alone), with their slots looked up.  It costs
   // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself.
@@ -197,9 +196,8 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
   fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group);
   DFSSM_CU(cudaGetLastError());
-  static const int deep = getenv("DFSSM_GD_DEEP") ? atoi(getenv("DFSSM_GD_DEEP")) : 0;
-  return walks <= sms || deep ? launch_walk<T, DK, 2, true>(p, workspace, kq16, order, (int)n, s)  // every block has an SM
-                      : launch_walk<T, DK, 2, false>(p, workspace, kq16, order, (int)n, s);
+  return walks <= sms ? launch_walk<T, DK, true>(p, workspace, kq16, order, (int)n, s)  // every block has an SM
+                      : launch_walk<T, DK, false>(p, workspace, kq16, order, (int)n, s);
 }
 
 // What both entry points ask of their arguments.
@@ -265,8 +263,11 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
     return dfssm_fail(DFSSM_ERR_ARG, "the workspace must be %zu bytes, 256-byte aligned", need);
   if (n_seq == 0 || tokens == 0) return DFSSM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  static const int loop = getenv("DFSSM_GD_LOOP") ? atoi(getenv("DFSSM_GD_LOOP")) : 4;
-  if (tokens <= (long long)loop * n_seq) return launch_loop(p, dk, dtype, s);
+  // The token loop for sequences of few tokens: it takes about 1 us a token of the longest one, the chunked kernels 16 us
+  // and more whatever the length up to 64 (64 heads, one sequence of 12 / 16 tokens: 14.7 / 18.5 us against 17;
+  // 64 sequences of 4 / 16: 83 / 256 us against 252 / 255).  The lengths are not known here, so the average decides,
+  // well below the crossover, since one of the sequences may hold most of the tokens.
+  if (tokens <= 15 || tokens <= 4LL * n_seq) return launch_loop(p, dk, dtype, s);
   char* w = static_cast<char*>(workspace);
   if (dtype == DFSSM_F16) return dk == 128 ? launch_chunked<__half, 128>(p, w, s) : launch_chunked<__half, 64>(p, w, s);
   return dk == 128 ? launch_chunked<__nv_bfloat16, 128>(p, w, s) : launch_chunked<__nv_bfloat16, 64>(p, w, s);

@@ -589,29 +589,30 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 // shared memory) and computes S q + u P^T and the rows of o; it also fetches the next chunk (cp.async): K is
 // double buffered, and Q, V, T, P and the factors are replaced as soon as they have been read, so that two
 // blocks of two pairs fit on an SM.  DEEP, for grids that give every block an SM of its own, has two of all of them and
-// fetches a chunk ahead: XXX us a chunk instead of YYY.  All products are taken transposed, with S, r and u as left operands: the
+// fetches a chunk ahead: 2.35 us a chunk (dk = 128) instead of 2.7.  All products are taken transposed, with S, r and u as left operands: the
 // accumulator layout of one product is the left operand's layout of the next, so nothing of the chain itself
 // passes through shared memory.
 //   S k, S q : [16 x dk] [dk x 64]     u = r T^T, u P^T : [16 x 64] [64 x 64]     u k : [16 x 64] [64 x dk]
 // The splits of one product's operands are written among the MMAs of the one before it or of its own earlier
 // steps, so that a single warp keeps its tensor core busy.
 //
-// Bound: the chain of a chunk is 316 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM), one
-// after the other; the output warp's 188 run beside them.
+// Bound: the chain of a chunk, at dk = 128 316 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM)
+// and the splits between them, one after the other: 3900 cycles when it runs alone, 4350 with the output warp and
+// the copies beside it.  Where two blocks share an SM the tensor cores are 55% busy.  Measured: 512 chunks of
+// 32 heads in 1.20 ms (128 blocks), 268 chunks of 24 sequences and 32 heads in 0.46 ms.
+
+constexpr int kGdPairs = 2;  // of warps per block: 32 rows of a head (four measured the same or slower)
 
 template <int DK>
 __host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 192; }
-template <int DK, int W, bool DEEP>
+template <int DK, bool DEEP>
 __host__ __device__ constexpr int gd_chunk_smem() {
-  return (DEEP ? 4 : 3) * kGdC * DK * 2 + (DEEP ? 2 : 1) * (kGdC * 32 * W + kGdBlock) + W * gd_exchange<DK>();
+  return (DEEP ? 4 : 3) * kGdC * DK * 2 + (DEEP ? 2 : 1) * (kGdC * 32 * kGdPairs + kGdBlock) + kGdPairs * gd_exchange<DK>();
 }
 
-// Byte offset of 16-byte unit u of token t in the V tile [64][16 W].
-template <int W>
-__device__ __forceinline__ uint32_t v_off(int t, int u) {
-  const int f = W >= 4 ? (t & 7) : (W == 2 ? ((t >> 1) & 3) : ((t >> 2) & 1));
-  return (uint32_t)(t * 32 * W + ((u ^ f) << 4));
-}
+// Byte offset of 16-byte unit u of token t in the V tile [64][32]: two rows per 128 bytes, the units of four
+// neighbouring pairs of rows permuted.
+__device__ __forceinline__ uint32_t v_off(int t, int u) { return (uint32_t)(t * 64 + ((u ^ ((t >> 1) & 3)) << 4)); }
 // Named barriers: 0 the block, 1 the output warps, 2 + 4 pair + {0: u is split, 1: S and u have been taken, 2: the
 // first half of S is split, 3: all of it}
 __device__ __forceinline__ void bar_sync(int id, int threads) {
@@ -663,12 +664,12 @@ __device__ __forceinline__ float pair_max(unsigned a, unsigned b, __nv_bfloat16)
 }
 
 // kq16: the fp16 tiles of K and Q for bf16 inputs; for fp16 inputs the tiles are rows of k and q themselves.
-template <typename T, int DK, int W, bool DEEP>
-__global__ void __launch_bounds__(64 * W, DEEP ? 1 : 2)
+template <typename T, int DK, bool DEEP>
+__global__ void __launch_bounds__(64 * kGdPairs, DEEP ? 1 : 2)
 gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
                          const int4* __restrict__ walks, int parts, int slots_total) {
   constexpr bool BF = !std::is_same<T, __half>::value;
-  constexpr int NT = 64 * W, NL = 32 * W, NK = DK / 8, UPR = DK / 8;
+  constexpr int W = kGdPairs, NT = 64 * W, NL = 32 * W, NK = DK / 8, UPR = DK / 8;
   constexpr int TILE = kGdC * DK * 2;
   constexpr int V_AT = (DEEP ? 4 : 3) * TILE, B_AT = V_AT + kGdC * 32 * W;  // K, K, Q (DEEP: twice), V, {T, P, factors}
   constexpr int STAGE = kGdC * 32 * W + kGdBlock;  // V and the rest (DEEP: two of them)
@@ -688,7 +689,6 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   // modulo 4), and two blocks share an SM, one in slots 0-3 and one in 4-7: the first has its chain warps on
   // schedulers 0 and 1, the other on 2 and 3, so that no scheduler gets two chains.  Only speed depends on it: where
   // the slots are not as described the warps' numbers serve.
-  static_assert(W == 2, "four warps");
   __shared__ unsigned place[2 * W];
   if (lane == 0) asm volatile("mov.u32 %0, %%warpid;" : "=r"(place[wid]));
   __syncthreads();
@@ -754,7 +754,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
 #pragma unroll
       for (int i = 0; i < 4; ++i, src += (size_t)16 * p.ld_v) {
         const bool ok = v_there && vt + 16 * i < n;
-        cp16(v_s + v_off<W>(vt + 16 * i, vu), ok ? src : static_cast<const T*>(p.v), ok);
+        cp16(v_s + v_off(vt + 16 * i, vu), ok ? src : static_cast<const T*>(p.v), ok);
       }
       const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock + lt * 16;
       const uint32_t dst = sm0 + B_AT + stage + lt * 16;
@@ -770,7 +770,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
 #pragma unroll
       for (int jp = 0; jp < 4; ++jp) {
         unsigned v[4];
-        ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
+        ldsm4t(v, v_s + v_off(16 * jp + tt, 2 * pair + tu));
         v0 = fmaxf(v0, pair_max(v[0], v[1], T()));
         v1 = fmaxf(v1, pair_max(v[2], v[3], T()));
       }
@@ -882,7 +882,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
             out[2 + i] = (unsigned)__builtin_bit_cast(unsigned short, r[2]) | (unsigned)__builtin_bit_cast(unsigned short, r[3]) << 16;
           }
           // into the pair's own columns of V, which its chain warp has read
-          stsm4t(v_s + v_off<W>(32 * half + 16 * jp + tt, 2 * pair + tu), out);
+          stsm4t(v_s + v_off(32 * half + 16 * jp + tt, 2 * pair + tu), out);
         }
       }
       __syncwarp();
@@ -893,7 +893,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
           const int t = 16 * i + (lane >> 1);
           if (t < count - ch * kGdC)
             *reinterpret_cast<uint4*>(og + (size_t)t * p.ld_o + (lane & 1) * 8) =
-                *reinterpret_cast<const uint4*>(st + V_AT + v_off<W>(t, 2 * pair + (lane & 1)));
+                *reinterpret_cast<const uint4*>(st + V_AT + v_off(t, 2 * pair + (lane & 1)));
         }
       }
       if constexpr (!DEEP) {
@@ -970,7 +970,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
 #pragma unroll
     for (int jp = 0; jp < 4; ++jp) {
       unsigned v[4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
-      ldsm4t(v, v_s + v_off<W>(16 * jp + tt, 2 * pair + tu));
+      ldsm4t(v, v_s + v_off(16 * jp + tt, 2 * pair + tu));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = 2 * jp + i;

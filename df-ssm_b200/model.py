@@ -255,6 +255,15 @@ class DFSSMModel:
         _lib.check(self.lib.dfssm_set_sampling(self._h, float(temperature), float(top_p), float(rep_penalty),
                                                int(seed) & (2**64 - 1)))
 
+    def sample(self, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None):
+        """Tokens from the logits that the last forward(), step() or prefill(logits=True) left in self.logits,
+        by ops.sample_filtered: per-sequence temperature, top_k, top_p and min_p (None, a number, or a device
+        tensor [B]) and given uniform numbers (fp32 [B] on the device).  Returns int32 [B] on the device, to be fed
+        to the next step(); the engine's own choice (set_sampling) is not touched."""
+        from . import ops
+        return ops.sample_filtered(self.logits[:self.batch_size], uniform, temperature=temperature, top_k=top_k,
+                                   top_p=top_p, min_p=min_p)[0]
+
     def generate(self, n_tokens: int = 128, prompt=None, verbose: bool = True, logits: bool = False,
                  temperature: float = 0.0, top_p: float = 0.9, rep_penalty: float = 1.2, seed: int = 0):
         """Decode: reset, consume `prompt` ([B, T]; token 0 if None), then n_tokens steps.  Greedy

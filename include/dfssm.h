@@ -278,7 +278,8 @@ size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_hea
  * tokens changes nothing; rows of o outside every sequence are left as they were.  `workspace` is device
  * memory of dfssm_gated_delta_workspace bytes, 256-byte aligned, used by this call alone until it has run:
  * calls that may overlap (other streams, graphs replayed at once) need one each.  Neither call allocates or
- * synchronises, and both can be captured into a graph. */
+ * synchronises, and both can be captured into a graph.  A NaN or infinite input spoils the rows of o and the
+ * state of its own sequence, from the start of its 64 tokens on, and nothing else. */
 int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, const void* v, int ld_v, const void* a,
                               int ld_a, const void* b, int ld_b, const float* A_log, const float* dt_bias,
                               float* state, int n_slots, const int32_t* slots, const int32_t* cu_seqlens, int n_seq,
