@@ -45,61 +45,91 @@ def _vector(t, name: str, n: int, dtype, device):
     _refuse(t, name, f"a contiguous {dtype} vector of {n}", device)
 
 
-def _heads(t, name: str, shape, dtype, device):
-    """Pointer and row stride of [rows, heads, width] whose rows are contiguous."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape:
-        n, h, d = shape
-        ld, sh, sd = t.stride()
-        if n < 2:
-            ld = h * d
-        if sd == 1 and (sh == d or h == 1) and h * d <= ld < 2**31:
-            return t.data_ptr(), ld
-    _refuse(t, name, f"{dtype} {tuple(shape)} with contiguous rows", device)
-
-
-def _gates(t, name: str, shape, dtype, device):
-    """Pointer and row stride of [rows, heads] whose rows are contiguous."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape:
-        ld, sh = t.stride()
-        if shape[0] < 2:
-            ld = shape[1]
-        if (sh == 1 or shape[1] == 1) and shape[1] <= ld < 2**31:
-            return t.data_ptr(), ld
-    _refuse(t, name, f"{dtype} {tuple(shape)} with contiguous rows", device)
-
-
-def _call(device, fn, *args):
-    """Runs a C entry on `device`, on its current stream (the last argument)."""
-    index = device.index
+def _call(index, fn, *args):
+    """Runs a C entry on that device, on its current stream (the last argument)."""
     if index == torch.cuda.current_device():
-        _lib.check(fn(*args, _stream_of(index)))
+        rc = fn(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream_of(index)))
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream_of(index))
+    if rc:
+        _lib.check(rc)
 
 
-def _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale):
+def _explain(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out):
+    """Finds out what _delta's checks did not like, and says so."""
     _on(q, "q")
     dev, dtype = q.device, q.dtype
     if dtype not in (torch.float16, torch.bfloat16) or q.dim() != 3:
         _refuse(q, "q", "fp16 or bf16 [tokens, k_heads, dk]")
     if not isinstance(v, torch.Tensor) or v.dim() != 3:
-        _refuse(v, "v", "[tokens, v_heads, dv]")
-    keys, values = q.shape, v.shape
-    n, hk, dk = keys
-    hv, dv = values[1:]
-    values = (n, hv, dv)
+        _refuse(v, "v", "[tokens, v_heads, dv]", dev)
+    (n, hk, dk), (hv, dv) = q.shape, v.shape[1:]
     if (not isinstance(state, torch.Tensor) or state.dtype is not torch.float32 or state.device != dev or state.dim() != 4
             or state.shape[1:] != (hv, dv, dk) or not state.is_contiguous()):
         _refuse(state, "state", f"contiguous fp32 [slots, {hv}, {dv}, {dk}]", dev)
-    if out is None:
-        out = v.new_empty(values)
-    head = (*_heads(q, "q", keys, dtype, dev), *_heads(k, "k", keys, dtype, dev), *_heads(v, "v", values, dtype, dev),
-            *_gates(a, "a", (n, hv), dtype, dev), *_gates(b, "b", (n, hv), dtype, dev),
-            _vector(A_log, "A_log", hv, torch.float32, dev), _vector(dt_bias, "dt_bias", hv, torch.float32, dev),
-            state.data_ptr(), state.shape[0], None if slots is None else _vector(slots, "slots", n_seq, torch.int32, dev))
-    tail = (*_heads(out, "out", values, dtype, dev), hk, hv, dk, dv, dk ** -0.5 if scale is None else float(scale))
-    return dev, head, tail, out, (n, hk, hv, dk, dv, _DTYPES[dtype])
+    for t, name, shape in ((q, "q", (n, hk, dk)), (k, "k", (n, hk, dk)), (v, "v", (n, hv, dv)), (out, "out", (n, hv, dv)),
+                           (a, "a", (n, hv)), (b, "b", (n, hv))):
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev or t.shape != shape or _row(t) is None:
+            _refuse(t, name, f"{dtype} {shape} with contiguous rows", dev)
+    _vector(A_log, "A_log", hv, torch.float32, dev)
+    _vector(dt_bias, "dt_bias", hv, torch.float32, dev)
+    if slots is not None:
+        _vector(slots, "slots", n_seq, torch.int32, dev)
+    raise ValueError("arguments do not fit together")
+
+
+def _row(t):
+    """Row stride of [rows, heads, width] or [rows, heads] whose rows are contiguous, else None."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        n, h, d = shape
+        ld, sh, sd = stride
+        width, ok = h * d, (sd == 1 or d == 1) and (sh == d or h == 1)
+    else:
+        n, width = shape
+        ld, sh = stride
+        ok = sh == 1 or width == 1
+    if n < 2:
+        ld = width
+    return ld if ok and width <= ld < 2**31 else None
+
+
+def _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale):
+    # One straight run of checks: a one-token call is over in less time than they take.
+    try:
+        dtype, index = q.dtype, q.get_device()
+        keys, values, heads = q.shape, v.shape, a.shape
+        n, hk, dk = keys
+        hv, dv = values[1:]
+        if out is None:
+            out = torch.empty_like(v) if v.is_contiguous() else v.new_empty(values)
+        f32, outputs = torch.float32, out.shape
+        ok = (index >= 0 and (dtype is torch.float16 or dtype is torch.bfloat16) and k.shape == keys and outputs == values
+              and values[0] == n and heads == (n, hv) and b.shape == heads and state.shape[1:] == (hv, dv, dk)
+              and k.dtype is dtype and v.dtype is dtype and a.dtype is dtype and b.dtype is dtype and out.dtype is dtype
+              and state.dtype is f32 and A_log.dtype is f32 and dt_bias.dtype is f32
+              and A_log.shape == (hv,) and dt_bias.shape == (hv,)
+              and k.get_device() == index and v.get_device() == index and a.get_device() == index
+              and b.get_device() == index and state.get_device() == index and out.get_device() == index
+              and A_log.get_device() == index and dt_bias.get_device() == index
+              and state.is_contiguous() and A_log.is_contiguous() and dt_bias.is_contiguous())
+        if slots is None:
+            slot = None
+        else:
+            slot = slots.data_ptr()
+            ok = (ok and slots.dtype is torch.int32 and slots.shape == (n_seq,) and slots.get_device() == index
+                  and slots.is_contiguous())
+        if ok:
+            lq, lk, lv, la, lb, lo = _row(q), _row(k), _row(v), _row(a), _row(b), _row(out)
+            if None not in (lq, lk, lv, la, lb, lo):
+                return (index, (q.data_ptr(), lq, k.data_ptr(), lk, v.data_ptr(), lv, a.data_ptr(), la, b.data_ptr(), lb,
+                                A_log.data_ptr(), dt_bias.data_ptr(), state.data_ptr(), state.shape[0], slot),
+                        (out.data_ptr(), lo, hk, hv, dk, dv, dk ** -0.5 if scale is None else float(scale)),
+                        out, (n, hk, hv, dk, dv, _DTYPES[dtype]))
+    except (AttributeError, TypeError, ValueError):  # not a tensor, or not of that rank
+        pass
+    _explain(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, v if out is None else out)
 
 
 def gated_delta_step(q, k, v, a, b, A_log, dt_bias, state, *, slots=None, scale: Optional[float] = None,
@@ -111,8 +141,8 @@ def gated_delta_step(q, k, v, a, b, A_log, dt_bias, state, *, slots=None, scale:
     updated in place; slots int32 [B] on the device (None: sequence i is in slot i).  scale defaults to
     dk ** -0.5.  Returns o [B, v_heads, dv] (`out` if given)."""
     n_seq = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
-    dev, head, tail, out, dims = _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale)
-    _call(dev, _lib.load().dfssm_gated_delta_step, *head, n_seq, *tail, int(bool(qk_norm)), dims[-1])
+    index, head, tail, out, dims = _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale)
+    _call(index, _lib.load().dfssm_gated_delta_step, *head, n_seq, *tail, int(bool(qk_norm)), dims[-1])
     return out
 
 
@@ -135,15 +165,15 @@ def gated_delta_prefill(q, k, v, a, b, A_log, dt_bias, state, cu_seqlens, *, slo
         _refuse(cu_seqlens, "cu_seqlens", "int32 [sequences + 1]")
     n_seq = cu_seqlens.shape[0] - 1
     cu = _vector(cu_seqlens, "cu_seqlens", n_seq + 1, torch.int32, q.device)
-    dev, head, tail, out, dims = _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale)
+    index, head, tail, out, dims = _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale)
     lib = _lib.load()
     need = lib.dfssm_gated_delta_workspace(dims[0], n_seq, *dims[1:])
     if workspace is None:
         workspace = v.new_empty(need, dtype=torch.uint8)
-    elif (not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.device != dev
+    elif (not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.get_device() != index
           or not workspace.is_contiguous() or workspace.numel() < need):
-        _refuse(workspace, "workspace", f"contiguous uint8 of at least {need} bytes", dev)
-    _call(dev, lib.dfssm_gated_delta_prefill, *head, cu, n_seq, dims[0], *tail, int(bool(qk_norm)), dims[-1],
+        _refuse(workspace, "workspace", f"contiguous uint8 of at least {need} bytes", q.device)
+    _call(index, lib.dfssm_gated_delta_prefill, *head, cu, n_seq, dims[0], *tail, int(bool(qk_norm)), dims[-1],
           workspace.data_ptr(), workspace.numel())
     return out
 
@@ -187,11 +217,14 @@ def sample_filtered(logits, uniform, *, temperature=None, top_k=None, top_p=None
                 or seen_bits.shape != (B, (V + 31) // 32) or not seen_bits.is_contiguous()):
             _refuse(seen_bits, "seen_bits", f"contiguous int32 [{B}, {(V + 31) // 32}]", dev)
     if out is None:
-        out = (uniform.new_empty(B, dtype=torch.int32), uniform.new_empty(B, dtype=torch.int32), uniform.new_empty(B))
-    token, kept, prob = out
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _call(dev, _lib.load().dfssm_sample_filtered, logits.data_ptr(), ld, _DTYPES[logits.dtype], B, V, ptr(temperature),
-          ptr(top_k), ptr(top_p), ptr(min_p), ptr(seen_bits), float(rep_penalty), u,
-          _vector(token, "out[0]", B, torch.int32, dev), _vector(kept, "out[1]", B, torch.int32, dev),
-          _vector(prob, "out[2]", B, torch.float32, dev))
+        out = (torch.empty_like(uniform, dtype=torch.int32), torch.empty_like(uniform, dtype=torch.int32), torch.empty_like(uniform))
+        tp, kp, pp = (t.data_ptr() for t in out)
+    else:
+        token, kept, prob = out
+        tp, kp = _vector(token, "out[0]", B, torch.int32, dev), _vector(kept, "out[1]", B, torch.int32, dev)
+        pp = _vector(prob, "out[2]", B, torch.float32, dev)
+    _call(dev.index, _lib.load().dfssm_sample_filtered, logits.data_ptr(), ld, _DTYPES[logits.dtype], B, V,
+          None if temperature is None else temperature.data_ptr(), None if top_k is None else top_k.data_ptr(),
+          None if top_p is None else top_p.data_ptr(), None if min_p is None else min_p.data_ptr(),
+          None if seen_bits is None else seen_bits.data_ptr(), float(rep_penalty), u, tp, kp, pp)
     return out
