@@ -159,10 +159,10 @@ int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16,
   constexpr int bytes = gd_chunk_smem<DK, DEEP>();
   const auto fn = gated_delta_chunk_kernel<T, DK, DEEP>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  const int parts = (p.dv + 16 * kGdPairs - 1) / (16 * kGdPairs);
+  const int parts = (p.dv + 16 * kGdGroups - 1) / (16 * kGdGroups);
   const long long grid = (long long)p.n_seq * p.v_heads * parts;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
-  fn<<<(unsigned)grid, 64 * kGdPairs, bytes, s>>>(p, blocks, kq16, order, parts, slots_total);
+  fn<<<(unsigned)grid, 128 * kGdGroups, bytes, s>>>(p, blocks, kq16, order, parts, slots_total);
   DFSSM_CU(cudaGetLastError());
   return DFSSM_OK;
 }

@@ -583,38 +583,39 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 
 // ------------------------------------------------------------------ the walk over a sequence's chunks
 //
-// A pair of warps owns 16 rows of one head's state.  The first, the chain warp, holds S^T as MMA accumulators
-// (64 registers per thread at dk = 128) and computes what the next chunk waits for: S k, r, u, the new S.  The
-// second, the output warp, takes the operands that the first has split anyway (S and u as fp16 pairs, through
-// shared memory) and computes S q + u P^T and the rows of o; it also fetches the next chunk (cp.async): K is
-// double buffered, and Q, V, T, P and the factors are replaced as soon as they have been read, so that two
-// blocks of two pairs fit on an SM.  DEEP, for grids that give every block an SM of its own, has two of all of them and
-// fetches a chunk ahead: 2.35 us a chunk (dk = 128) instead of 2.7.  All products are taken transposed, with S, r and u as left operands: the
-// accumulator layout of one product is the left operand's layout of the next, so nothing of the chain itself
-// passes through shared memory.
+// A block owns 32 rows of one head's state, two groups of 16, and has eight warps.  Each group has two chain warps, which
+// hold S^T as MMA accumulators, half of the dk columns each, and compute what the next chunk waits for: S k, r, u,
+// the new S; and two output warps, which take the operands that the chain warps have split anyway (S and u as
+// fp16 pairs, through shared memory), compute S q + u P^T and the rows of o, half of the tokens each, and fetch the next
+// chunk (cp.async).  All products are taken transposed, with S, r and u as left operands: the accumulator layout of
+// one product is the left operand's layout of the next.
 //   S k, S q : [16 x dk] [dk x 64]     u = r T^T, u P^T : [16 x 64] [64 x 64]     u k : [16 x 64] [64 x dk]
-// The splits of one product's operands are written among the MMAs of the one before it or of its own earlier
-// steps, so that a single warp keeps its tensor core busy.
+// Between its two warps a chain passes, per chunk: half of each one's partial S k (A keeps tokens 0-31, B 32-63), A's r (B's
+// u needs it), and both halves of the weighed u.  The splits of one product's operands are written among the MMAs of
+// its earlier steps, so that a warp keeps its tensor core busy.
 //
-// Bound: the chain of a chunk, at dk = 128 316 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM)
-// and the splits between them, one after the other: 3900 cycles when it runs alone, 4350 with the output warp and
-// the copies beside it.  Where two blocks share an SM the tensor cores are 55% busy.  Measured: 512 chunks of
-// 32 heads in 1.20 ms (128 blocks), 268 chunks of 24 sequences and 32 heads in 0.46 ms.
+// K is double buffered, and Q, V, T, P and the factors are replaced as soon as they have been read, so that two blocks
+// fit on an SM.  DEEP, for grids that give every block an SM of its own, has two of all of them and fetches a chunk ahead.
+//
+// Bound: per chunk and group, at dk = 128, 504 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM) and
+// about 160 KB through shared memory, in a chain of dependent steps.  Alone on its SM a block takes 2.06 us a chunk
+// (512 chunks of 32 heads, 128 blocks, in 1.06 ms; tensor cores 54% busy; 2.35 us with one chain warp per group); two
+// blocks on an SM take 4.1 us for a chunk each (tensor cores 53%, shared memory 70% busy).
 
-constexpr int kGdPairs = 2;  // of warps per block: 32 rows of a head (four measured the same or slower)
+constexpr int kGdGroups = 2;  // of 16 rows per block
 
 template <int DK>
-__host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 192; }
+__host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 4096 + 2048 + 640; }
 template <int DK, bool DEEP>
 __host__ __device__ constexpr int gd_chunk_smem() {
-  return (DEEP ? 4 : 3) * kGdC * DK * 2 + (DEEP ? 2 : 1) * (kGdC * 32 * kGdPairs + kGdBlock) + kGdPairs * gd_exchange<DK>();
+  return (DEEP ? 4 : 3) * kGdC * DK * 2 + (DEEP ? 2 : 1) * (kGdC * 32 * kGdGroups + kGdBlock) + kGdGroups * gd_exchange<DK>();
 }
 
 // Byte offset of 16-byte unit u of token t in the V tile [64][32]: two rows per 128 bytes, the units of four
 // neighbouring pairs of rows permuted.
 __device__ __forceinline__ uint32_t v_off(int t, int u) { return (uint32_t)(t * 64 + ((u ^ ((t >> 1) & 3)) << 4)); }
-// Named barriers: 0 the block, 1 the output warps, 2 + 4 pair + {0: u is split, 1: S and u have been taken, 2: the
-// first half of S is split, 3: all of it}
+// Named barriers: 0 the block, 1 the output warps, 2 + 5 group + {0: the chain's two warps, 1: A's r is split, 2: S is
+// split, 3: u is split, 4: S and u have been taken}
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -622,25 +623,26 @@ __device__ __forceinline__ void bar_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// x[i] += rows of (ah + al) times the 64 x 64 triangular matrix in fragment order, for n-tiles J0 + i
-template <int J0>
-__device__ __forceinline__ void tri_product(float (&x)[4][4], const unsigned (&ah)[4][4], const unsigned (&al)[4][4],
+// x[i] += rows of (ah + al)[kk - K0] times the 64 x 64 triangular matrix in fragment order, for n-tiles J0 + i and the
+// k-steps K0 .. K1 - 1 that they have
+template <int J0, int K0, int K1, int NA>
+__device__ __forceinline__ void tri_product(float (&x)[4][4], const unsigned (&ah)[NA][4], const unsigned (&al)[NA][4],
                                             const uint4* F) {
 #pragma unroll
-  for (int kk = 0; kk <= (J0 + 3) / 2; ++kk) {
+  for (int kk = K0; kk < K1; ++kk) {
     uint4 b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (kk <= (J0 + i) / 2) b[i] = F[gd_frag(J0 + i, kk) * 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk], b[i].z, b[i].w);
+      if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk - K0], b[i].z, b[i].w);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (kk <= (J0 + i) / 2) mma_acc(x[i], al[kk], b[i].x, b[i].y);
+      if (kk <= (J0 + i) / 2) mma_acc(x[i], al[kk - K0], b[i].x, b[i].y);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk], b[i].x, b[i].y);
+      if (kk <= (J0 + i) / 2) mma_acc(x[i], ah[kk - K0], b[i].x, b[i].y);
   }
 }
 // One k-step's left operand from two neighbouring accumulator tiles, rows scaled by f0 (rows g) and f1 (g + 8).
@@ -650,6 +652,15 @@ __device__ __forceinline__ void split_tile(const float (&x)[4], const float (&y)
   split2(mul2(make_float2(x[2], x[3]), dup(f1)), ah[1], al[1]);
   split2(mul2(make_float2(y[0], y[1]), dup(f0)), ah[2], al[2]);
   split2(mul2(make_float2(y[2], y[3]), dup(f1)), ah[3], al[3]);
+}
+__device__ __forceinline__ void put_frag(uint4* to, const unsigned (&h)[4], const unsigned (&l)[4]) {
+  to[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  to[32] = make_uint4(l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ void get_frag(const uint4* from, unsigned (&h)[4], unsigned (&l)[4]) {
+  const uint4 a = from[0], b = from[32];
+  h[0] = a.x, h[1] = a.y, h[2] = a.z, h[3] = a.w;
+  l[0] = b.x, l[1] = b.y, l[2] = b.z, l[3] = b.w;
 }
 // Largest magnitude of two pairs of 16-bit values.
 __device__ __forceinline__ float pair_max(unsigned a, unsigned b, __half) {
@@ -665,14 +676,15 @@ __device__ __forceinline__ float pair_max(unsigned a, unsigned b, __nv_bfloat16)
 
 // kq16: the fp16 tiles of K and Q for bf16 inputs; for fp16 inputs the tiles are rows of k and q themselves.
 template <typename T, int DK, bool DEEP>
-__global__ void __launch_bounds__(64 * kGdPairs, DEEP ? 1 : 2)
+__global__ void __launch_bounds__(128 * kGdGroups, DEEP ? 1 : 2)
 gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
                          const int4* __restrict__ walks, int parts, int slots_total) {
   constexpr bool BF = !std::is_same<T, __half>::value;
-  constexpr int W = kGdPairs, NT = 64 * W, NL = 32 * W, NK = DK / 8, UPR = DK / 8;
+  constexpr int NT = 128 * kGdGroups, NL = NT / 2, UPR = DK / 8;
+  constexpr int NH = DK / 16, KH = DK / 32;  // n-tiles and k-steps of a chain warp's half of dk
   constexpr int TILE = kGdC * DK * 2;
-  constexpr int V_AT = (DEEP ? 4 : 3) * TILE, B_AT = V_AT + kGdC * 32 * W;  // K, K, Q (DEEP: twice), V, {T, P, factors}
-  constexpr int STAGE = kGdC * 32 * W + kGdBlock;  // V and the rest (DEEP: two of them)
+  constexpr int V_AT = (DEEP ? 4 : 3) * TILE, B_AT = V_AT + kGdC * 32 * kGdGroups;  // K, K, Q (DEEP: twice), V, {T, P, factors}
+  constexpr int STAGE = kGdC * 32 * kGdGroups + kGdBlock;                            // V and the rest (DEEP: two of them)
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   const int part = blockIdx.x % parts, h = (blockIdx.x / parts) % p.v_heads, nth = blockIdx.x / (parts * p.v_heads);
@@ -685,43 +697,36 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     gd_range(p.cu, seq, p.tokens, first, count);
     slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
   }
-  // Roles by scheduler.  A block's four warps sit on the SM's four schedulers in an order of the hardware's own (warp slot
-  // modulo 4), and two blocks share an SM, one in slots 0-3 and one in 4-7: the first has its chain warps on
-  // schedulers 0 and 1, the other on 2 and 3, so that no scheduler gets two chains.  Only speed depends on it: where
-  // the slots are not as described the warps' numbers serve.
-  __shared__ unsigned place[2 * W];
-  if (lane == 0) asm volatile("mov.u32 %0, %%warpid;" : "=r"(place[wid]));
-  __syncthreads();
   if (slot < 0 || count == 0) return;
   const int base = first / kGdC + seq;  // gd_chunk_base
   const int chunks = min((count + kGdC - 1) / kGdC, slots_total - base);
   const int hk = h / (p.v_heads / p.k_heads);
-  unsigned seen = 0;
-#pragma unroll
-  for (int i = 0; i < 2 * W; ++i) seen |= 1u << (place[i] & 3);
-  const int at = seen == 15u ? (int)(place[wid] & 3) : wid;
-  const bool chain = (at < W) != (((place[0] >> 2) & 1) != 0);
-  const int pair = at % W;
-  const int dv0 = part * 16 * W, row0 = dv0 + 16 * pair;
-  const bool active = row0 < p.dv;  // dv is a multiple of 16: a pair's rows are all there or none
-  char* ex = smem + V_AT + (DEEP ? 2 : 1) * STAGE + pair * gd_exchange<DK>();
-  uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;                   // S: [dk / 16][hi, lo][32]
-  uint4* u_ex = reinterpret_cast<uint4*>(ex + DK / 16 * 1024) + lane;  // u: [4][hi, lo][32]
-  float* sc = reinterpret_cast<float*>(ex + DK / 16 * 1024 + 4096);    // [3][16] the rows' scales of S and u, and max |v|
-  const int bar = 2 + 4 * pair;
+  // Warps 0-3 are the chains', 4-7 the output warps'; w and w + 4 share a scheduler, a chain's B warp (more of u) with an
+  // output warp of the first half (less of u P^T).
+  const bool chain = wid < 2 * kGdGroups;
+  const int group = (wid >> 1) % kGdGroups, half = chain ? wid & 1 : 1 - (wid & 1);
+  const int dv0 = part * 16 * kGdGroups, row0 = dv0 + 16 * group;
+  const bool active = row0 < p.dv;  // dv is a multiple of 16: a group's rows are all there or none
+  char* ex = smem + V_AT + (DEEP ? 2 : 1) * STAGE + group * gd_exchange<DK>();
+  uint4* s_ex = reinterpret_cast<uint4*>(ex) + lane;     // S: [dk / 16][hi, lo][32]
+  uint4* u_ex = s_ex + DK / 16 * 64;                     // u: [4][hi, lo][32]
+  uint4* d_ex = u_ex + 4 * 64;                           // weighed u, the same; before it, partial S k [A, B][4][32]
+  uint4* r_ex = d_ex + 4 * 64;                           // A's r: [2][hi, lo][32]
+  float* sc = reinterpret_cast<float*>(r_ex - lane + 2 * 64);  // [16] each: scale of S (A, B), max of S (A, B), scale of u, max |v| (2)
+  const int bar = 2 + 5 * group;
   // lane parts of the ldmatrix addresses
   const int bt = ((lane >> 4) << 3) + (lane & 7), bu = (lane >> 3) & 1;  // B from [token][dk] rows, two n-tiles
   const int tt = (((lane >> 3) & 1) << 3) + (lane & 7), tu = lane >> 4;  // the same, transposed
 
   if (!chain) {
-    // ---------------------------------------------------------------- output warp
+    // ---------------------------------------------------------------- output warp, tokens 32 half ..
     // A lane copies one 16-byte column of every RP-th row (K, Q), so that a copy costs a pointer step; rows past
     // the sequence's end are zeros.
-    const int lt = pair * 32 + lane;
-    constexpr int RP = NL / UPR;  // rows per pass: 4 to 16
+    const int lt = tid - NT / 2;
+    constexpr int RP = NL / UPR;  // rows per pass, a multiple of 8
     const uint32_t sm0 = smem_u32(smem);
     const int kt = lt / UPR, ku = lt % UPR;
-    const uint32_t off0 = kq_off<DK>(kt, ku), off1 = kq_off<DK>(kt + RP, ku) - RP * DK * 2;  // even and odd passes
+    const uint32_t off = kq_off<DK>(kt, ku);
     auto load_tile = [&](int ch, uint32_t dst, const void* rows, int ld, int which) {  // K (0) or Q (1) of chunk ch
       const int n = count - ch * kGdC;
       const __half* src;
@@ -735,26 +740,25 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       }
       if (BF || n >= kGdC) {
 #pragma unroll
-        for (int i = 0; i < kGdC / RP; ++i, src += step) cp16(dst + i * (RP * DK * 2) + ((i & 1) ? off1 : off0), src, true);
+        for (int i = 0; i < kGdC / RP; ++i, src += step) cp16(dst + i * (RP * DK * 2) + off, src, true);
       } else {
         for (int i = 0; i < kGdC / RP; ++i, src += step) {
           const bool ok = kt + i * RP < n;
-          cp16(dst + i * (RP * DK * 2) + ((i & 1) ? off1 : off0), ok ? src : static_cast<const __half*>(rows), ok);
+          cp16(dst + i * (RP * DK * 2) + off, ok ? src : static_cast<const __half*>(rows), ok);
         }
       }
     };
     auto load_k = [&](int ch) { load_tile(ch, sm0 + (ch & 1) * TILE, p.k, p.ld_k, 0); };
     auto load_q = [&](int ch) { load_tile(ch, sm0 + (2 + (DEEP ? ch & 1 : 0)) * TILE, p.q, p.ld_q, 1); };
-    const int vu = lt % (2 * W), vt = lt / (2 * W);  // 16 rows of V per pass
+    const int vu = lt & 3, vt = lt >> 2;  // 32 rows of V per pass
     const bool v_there = dv0 + vu * 8 < p.dv;
     auto load_vb = [&](int ch) {  // V, T, P and the factors of chunk ch
       const int n = count - ch * kGdC, stage = DEEP ? (ch & 1) * STAGE : 0;
-      const uint32_t v_s = sm0 + V_AT + stage;
       const T* src = static_cast<const T*>(p.v) + ((size_t)first + (size_t)ch * kGdC + vt) * p.ld_v + h * p.dv + dv0 + vu * 8;
 #pragma unroll
-      for (int i = 0; i < 4; ++i, src += (size_t)16 * p.ld_v) {
-        const bool ok = v_there && vt + 16 * i < n;
-        cp16(v_s + v_off(vt + 16 * i, vu), ok ? src : static_cast<const T*>(p.v), ok);
+      for (int i = 0; i < 2; ++i, src += (size_t)32 * p.ld_v) {
+        const bool ok = v_there && vt + 32 * i < n;
+        cp16(sm0 + V_AT + stage + v_off(vt + 32 * i, vu), ok ? src : static_cast<const T*>(p.v), ok);
       }
       const char* blk = blocks + ((size_t)(base + ch) * p.v_heads + h) * kGdBlock + lt * 16;
       const uint32_t dst = sm0 + B_AT + stage + lt * 16;
@@ -763,20 +767,20 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       constexpr int REST = kGdBlock / 16 % NL;
       if (lt < REST) cp16(dst + kGdBlock / 16 / NL * NL * 16, blk + kGdBlock / 16 / NL * NL * 16, true);
     };
-    // the largest |v| of each row of chunk ch, for the chain's bound of r
+    // the largest |v| of each row over this half of chunk ch, for the chain's bound of r
     auto largest_v = [&](int ch) {
       const uint32_t v_s = sm0 + (DEEP ? (ch & 1) * STAGE : 0) + V_AT;
       float v0 = 0.f, v1 = 0.f;
 #pragma unroll
-      for (int jp = 0; jp < 4; ++jp) {
+      for (int jp = 0; jp < 2; ++jp) {
         unsigned v[4];
-        ldsm4t(v, v_s + v_off(16 * jp + tt, 2 * pair + tu));
+        ldsm4t(v, v_s + v_off(32 * half + 16 * jp + tt, 2 * group + tu));
         v0 = fmaxf(v0, pair_max(v[0], v[1], T()));
         v1 = fmaxf(v1, pair_max(v[2], v[3], T()));
       }
       v0 = quad_max(v0);
       v1 = quad_max(v1);
-      if (c == 0) sc[32 + g] = v0, sc[40 + g] = v1;
+      if (c == 0) sc[80 + 16 * half + g] = v0, sc[88 + 16 * half + g] = v1;
     };
     load_k(0);
     load_q(0);
@@ -792,9 +796,14 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     for (int ch = 0; ch < chunks; ++ch) {
       const bool more = ch + 1 < chunks;
       const char* st = smem + (DEEP ? (ch & 1) * STAGE : 0);
-      const uint32_t v_s = smem_u32(st) + V_AT;
+      const uint32_t v_s = smem_u32(st) + V_AT, q_s = sm0 + (2 + (DEEP ? ch & 1 : 0)) * TILE;
       const float* vec = reinterpret_cast<const float*>(st + B_AT + 2 * kGdTri);
-      if constexpr (!DEEP) {
+      if constexpr (DEEP) {
+        bar_sync(bar + 2, 128);  // S is split
+        bar_sync(1, NL);         // every chain is past the last chunk, and so are the output warps: the other stage is free
+        if (more) load_k(ch + 1), load_q(ch + 1), load_vb(ch + 1);
+        cp_commit();
+      } else {
         cp_wait<1>();
         bar_sync(0, NT);  // K and Q are there, and nobody reads the other K any more
         if (more) load_k(ch + 1);
@@ -802,57 +811,43 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         cp_wait<1>();
         bar_sync(1, NL);  // V, T, P and the factors are there
         largest_v(ch);
+        bar_sync(0, NT);  // they are for the chains too, which have split S
       }
-      const uint32_t q_s = smem_u32(smem) + (2 + (DEEP ? ch & 1 : 0)) * TILE;
-      float o[8][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      bar_sync(bar + 2, 64);  // half of S is split
-      if constexpr (DEEP) {
-        bar_sync(1, NL);  // every chain is past the last chunk, and so are the output warps: the other stage is free
-        if (more) load_k(ch + 1), load_q(ch + 1), load_vb(ch + 1);
-        cp_commit();
-      }
+      float o[4][4] = {}, o2[4][4] = {};  // the two halves of dk have scales of their own
 #pragma unroll
       for (int kk = 0; kk < DK / 16; ++kk) {
-        if (kk == DK / 32) {
-          if constexpr (DEEP) bar_sync(bar + 3, 64);  // all of S is split
-          else bar_sync(0, NT);  // the same of all chains; V, T, P and the factors are there for them too
-        }
-        const uint4 hv = s_ex[(2 * kk) * 32], lv = s_ex[(2 * kk + 1) * 32];
-        const unsigned ah[4] = {hv.x, hv.y, hv.z, hv.w}, al[4] = {lv.x, lv.y, lv.z, lv.w};
-        unsigned b[4][4];
+        unsigned ah[4], al[4], b[2][4];
+        get_frag(s_ex + kk * 64, ah, al);
 #pragma unroll
-        for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], q_s + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
+        for (int jp = 0; jp < 2; ++jp) ldsm4(b[jp], q_s + kq_off<DK>(32 * half + 16 * jp + bt, 2 * kk + bu));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mma_acc(o[j], al, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+        for (int j = 0; j < 4; ++j) mma_acc(kk < KH ? o[j] : o2[j], al, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mma_acc(o[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+        for (int j = 0; j < 4; ++j) mma_acc(kk < KH ? o[j] : o2[j], ah, b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
       }
-      const float ds0 = sc[g], ds1 = sc[g + 8];
+      {
+        const float a0 = sc[g], a1 = sc[g + 8], b0 = sc[16 + g], b1 = sc[24 + g];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 oq = *reinterpret_cast<const float2*>(vec + kGdOq + 32 * half + 8 * j + 2 * c);
+          o[j][0] = oq.x * fmaf(o[j][0], a0, o2[j][0] * b0);
+          o[j][1] = oq.y * fmaf(o[j][1], a0, o2[j][1] * b0);
+          o[j][2] = oq.x * fmaf(o[j][2], a1, o2[j][2] * b1);
+          o[j][3] = oq.y * fmaf(o[j][3], a1, o2[j][3] * b1);
+        }
+      }
       if constexpr (!DEEP) {
         bar_sync(1, NL);  // Q is free
         if (more) load_q(ch + 1);
         cp_commit();
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 oq = *reinterpret_cast<const float2*>(vec + kGdOq + 8 * j + 2 * c);
-        o[j][0] *= oq.x * ds0;
-        o[j][1] *= oq.y * ds0;
-        o[j][2] *= oq.x * ds1;
-        o[j][3] *= oq.y * ds1;
-      }
-      bar_sync(bar, 64);
+      bar_sync(bar + 3, 128);  // u is split
       unsigned ah[4][4], al[4][4];
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const uint4 hv = u_ex[(2 * kk) * 32], lv = u_ex[(2 * kk + 1) * 32];
-        ah[kk][0] = hv.x, ah[kk][1] = hv.y, ah[kk][2] = hv.z, ah[kk][3] = hv.w;
-        al[kk][0] = lv.x, al[kk][1] = lv.y, al[kk][2] = lv.z, al[kk][3] = lv.w;
-      }
-      const float du0 = sc[16 + g], du1 = sc[24 + g];
-      if (more) bar_arrive(bar + 1, 64);
+      for (int kk = 0; kk < 4; ++kk)
+        if (kk < 2 || half) get_frag(u_ex + kk * 64, ah[kk], al[kk]);
+      const float du0 = sc[64 + g], du1 = sc[72 + g];
+      if (more) bar_arrive(bar + 4, 128);
       if (DEEP && more) {
         cp_wait<0>();
         bar_sync(1, NL);
@@ -860,40 +855,36 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         bar_arrive(0, NT);  // the next chunk is there
       }
       const uint4* Pf = reinterpret_cast<const uint4*>(st + B_AT + kGdTri) + lane;
-      float x0[4][4] = {}, x1[4][4] = {};
-      tri_product<0>(x0, ah, al, Pf);
-      tri_product<4>(x1, ah, al, Pf);
+      float x[4][4] = {};
+      if (half == 0) tri_product<0, 0, 2>(x, ah, al, Pf);
+      else tri_product<4, 0, 4>(x, ah, al, Pf);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float(&x)[4][4] = half ? x1 : x0;
+      for (int jp = 0; jp < 2; ++jp) {
+        unsigned out[4];
 #pragma unroll
-        for (int jp = 0; jp < 2; ++jp) {
-          unsigned out[4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int j = 4 * half + 2 * jp + i;
-            const float2 op = *reinterpret_cast<const float2*>(vec + kGdOp + 8 * j + 2 * c);
-            T r[4];
-            r[0] = from_f<T>(fmaf(x[2 * jp + i][0], op.x * du0, o[j][0]));
-            r[1] = from_f<T>(fmaf(x[2 * jp + i][1], op.y * du0, o[j][1]));
-            r[2] = from_f<T>(fmaf(x[2 * jp + i][2], op.x * du1, o[j][2]));
-            r[3] = from_f<T>(fmaf(x[2 * jp + i][3], op.y * du1, o[j][3]));
-            out[i] = (unsigned)__builtin_bit_cast(unsigned short, r[0]) | (unsigned)__builtin_bit_cast(unsigned short, r[1]) << 16;
-            out[2 + i] = (unsigned)__builtin_bit_cast(unsigned short, r[2]) | (unsigned)__builtin_bit_cast(unsigned short, r[3]) << 16;
-          }
-          // into the pair's own columns of V, which its chain warp has read
-          stsm4t(v_s + v_off(32 * half + 16 * jp + tt, 2 * pair + tu), out);
+        for (int i = 0; i < 2; ++i) {
+          const int j = 2 * jp + i;
+          const float2 op = *reinterpret_cast<const float2*>(vec + kGdOp + 32 * half + 8 * j + 2 * c);
+          T r[4];
+          r[0] = from_f<T>(fmaf(x[j][0], op.x * du0, o[j][0]));
+          r[1] = from_f<T>(fmaf(x[j][1], op.y * du0, o[j][1]));
+          r[2] = from_f<T>(fmaf(x[j][2], op.x * du1, o[j][2]));
+          r[3] = from_f<T>(fmaf(x[j][3], op.y * du1, o[j][3]));
+          out[i] = (unsigned)__builtin_bit_cast(unsigned short, r[0]) | (unsigned)__builtin_bit_cast(unsigned short, r[1]) << 16;
+          out[2 + i] = (unsigned)__builtin_bit_cast(unsigned short, r[2]) | (unsigned)__builtin_bit_cast(unsigned short, r[3]) << 16;
         }
+        // into the group's own columns of V, which its chain warps have read
+        stsm4t(v_s + v_off(32 * half + 16 * jp + tt, 2 * group + tu), out);
       }
       __syncwarp();
       if (active) {  // 16 rows of 32 bytes per store
         T* og = static_cast<T*>(p.o) + ((size_t)first + (size_t)ch * kGdC) * p.ld_o + h * p.dv + row0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 16 * i + (lane >> 1);
+        for (int i = 0; i < 2; ++i) {
+          const int t = 32 * half + 16 * i + (lane >> 1);
           if (t < count - ch * kGdC)
             *reinterpret_cast<uint4*>(og + (size_t)t * p.ld_o + (lane & 1) * 8) =
-                *reinterpret_cast<const uint4*>(st + V_AT + v_off(t, 2 * pair + (lane & 1)));
+                *reinterpret_cast<const uint4*>(st + V_AT + v_off(t, 2 * group + (lane & 1)));
         }
       }
       if constexpr (!DEEP) {
@@ -906,11 +897,11 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     return;
   }
 
-  // ------------------------------------------------------------------ chain warp
-  float* Sg = p.state + (((size_t)slot * p.v_heads + h) * p.dv + row0 + g) * DK + 2 * c;
-  float s[NK][4], m0 = 0.f, m1 = 0.f;  // the state and its rows' largest magnitudes
+  // ------------------------------------------------------------------ chain warp, dk columns half * DK / 2 ..
+  float* Sg = p.state + (((size_t)slot * p.v_heads + h) * p.dv + row0 + g) * DK + half * (DK / 2) + 2 * c;
+  float s[NH][4], m0 = 0.f, m1 = 0.f;  // the state and its rows' largest magnitudes
 #pragma unroll
-  for (int j = 0; j < NK; ++j) {
+  for (int j = 0; j < NH; ++j) {
     float2 x = make_float2(0.f, 0.f), y = x;
     if (active) {
       x = *reinterpret_cast<const float2*>(Sg + 8 * j);
@@ -930,113 +921,152 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     float up0, dn0, up1, dn1;
     row_scale(m0, up0, dn0);
     row_scale(m1, up1, dn1);
-    if (ch) bar_sync(bar + 1, 64);  // the last chunk's S and u have been taken
-    if (c == 0) sc[g] = dn0, sc[g + 8] = dn1;
+    if (ch) bar_sync(bar + 4, 128);  // the last chunk's S and u have been taken
+    if (c == 0) {
+      sc[16 * half + g] = dn0, sc[16 * half + 8 + g] = dn1;
+      sc[32 + 16 * half + g] = m0, sc[40 + 16 * half + g] = m1;
+    }
     unsigned sh[2][4], sl[2][4];
     split_tile(s[0], s[1], up0, up1, sh[0], sl[0]);
     bar_sync(0, NT);  // K and Q are there (DEEP: the whole chunk)
     float ks[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) ks[j][0] = ks[j][1] = ks[j][2] = ks[j][3] = 0.f;
-    // S k, the next step's split between the MMAs of this one
+    // this half's part of S k, the next step's split between the MMAs of this one
 #pragma unroll
-    for (int kk = 0; kk < DK / 16; ++kk) {
+    for (int kk = 0; kk < KH; ++kk) {
       unsigned b[4][4];
 #pragma unroll
-      for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], k_s + kq_off<DK>(16 * jp + bt, 2 * kk + bu));
+      for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], k_s + kq_off<DK>(16 * jp + bt, 2 * (half * KH + kk) + bu));
       const int now = kk & 1;
-      s_ex[(2 * kk) * 32] = make_uint4(sh[now][0], sh[now][1], sh[now][2], sh[now][3]);
-      s_ex[(2 * kk + 1) * 32] = make_uint4(sl[now][0], sl[now][1], sl[now][2], sl[now][3]);
-      if (kk + 1 < DK / 16) split_tile(s[2 * kk + 2], s[2 * kk + 3], up0, up1, sh[now ^ 1], sl[now ^ 1]);
-      if (kk == DK / 32 - 1) bar_arrive(bar + 2, 64);  // half of S is split
+      put_frag(s_ex + (half * KH + kk) * 64, sh[now], sl[now]);
+      if (DEEP && kk == KH - 1) bar_arrive(bar + 2, 128);  // S is split
+      if (kk + 1 < KH) split_tile(s[2 * kk + 2], s[2 * kk + 3], up0, up1, sh[now ^ 1], sl[now ^ 1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) mma_acc(ks[j], sl[now], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) mma_acc(ks[j], sh[now], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
     }
-    if constexpr (DEEP) bar_arrive(bar + 3, 64);  // S is split
-    else bar_sync(0, NT);                         // ... and V, T, P and the factors are there
+    // the other warp's tokens to it, in the place where it will put its weighed u
+    float (&mine)[4][4] = *reinterpret_cast<float(*)[4][4]>(&ks[0]);
+    {
+      float t[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float d = i < 2 ? dn0 : dn1, a = ks[j][i] * d, b = ks[4 + j][i] * d;
+          t[j][i] = half ? a : b;
+          mine[j][i] = half ? b : a;
+        }
+        d_ex[((1 - half) * 4 + j) * 32] = make_uint4(__float_as_uint(t[j][0]), __float_as_uint(t[j][1]), __float_as_uint(t[j][2]),
+                                                    __float_as_uint(t[j][3]));
+      }
+    }
+    if constexpr (DEEP) bar_sync(bar, 64);
+    else bar_sync(0, NT);  // also: V, T, P and the factors are there; S is split
     // bounds of r and u, and the scales from them
-    const float root = DK == 128 ? 11.3137085f : 8.f;
-    const float r0 = fmaf(root * vec[kGdKn], m0, sc[32 + g]), r1 = fmaf(root * vec[kGdKn], m1, sc[40 + g]);
+    const float root = (DK == 128 ? 11.3137085f : 8.f) * vec[kGdKn];
+    const float r0 = fmaf(root, fmaxf(sc[32 + g], sc[48 + g]), fmaxf(sc[80 + g], sc[96 + g]));
+    const float r1 = fmaf(root, fmaxf(sc[40 + g], sc[56 + g]), fmaxf(sc[88 + g], sc[104 + g]));
     float ur0, dr0, ur1, dr1, uu0, du0, uu1, du1;
     row_scale(r0, ur0, dr0);
     row_scale(r1, ur1, dr1);
     row_scale(r0 * vec[kGdTsum], uu0, du0);
     row_scale(r1 * vec[kGdTsum], uu1, du1);
     const float tdn = vec[kGdTdn], el = vec[kGdLast], cdn = vec[kGdCdn];
-    // r = v - e^G (S k), in ks, split as the left operand of u = r T^T
+    // r = v - e^G (S k) of this warp's tokens, split as the left operand of u = r T^T
     unsigned ah[4][4], al[4][4];
 #pragma unroll
-    for (int jp = 0; jp < 4; ++jp) {
-      unsigned v[4];  // tokens 16 jp.. x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
-      ldsm4t(v, v_s + v_off(16 * jp + tt, 2 * pair + tu));
+    for (int jp = 0; jp < 2; ++jp) {
+      unsigned v[4];  // 16 tokens x 16 rows: {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
+      ldsm4t(v, v_s + v_off(32 * half + 16 * jp + tt, 2 * group + tu));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int j = 2 * jp + i;
-        const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + 8 * j + 2 * c);
+        const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + 32 * half + 8 * j + 2 * c);
+        const uint4 o = d_ex[(half * 4 + j) * 32];
         const T* x = reinterpret_cast<const T*>(&v[i]);
         const T* y = reinterpret_cast<const T*>(&v[2 + i]);
-        const float2 a = fma2(mul2(bk, dup(dn0)), make_float2(ks[j][0], ks[j][1]), make_float2(to_f(x[0]), to_f(x[1])));
-        const float2 b = fma2(mul2(bk, dup(dn1)), make_float2(ks[j][2], ks[j][3]), make_float2(to_f(y[0]), to_f(y[1])));
-        ks[j][0] = a.x, ks[j][1] = a.y, ks[j][2] = b.x, ks[j][3] = b.y;
+        const float2 a = fma2(bk, make_float2(mine[j][0] + __uint_as_float(o.x), mine[j][1] + __uint_as_float(o.y)),
+                              make_float2(to_f(x[0]), to_f(x[1])));
+        const float2 b = fma2(bk, make_float2(mine[j][2] + __uint_as_float(o.z), mine[j][3] + __uint_as_float(o.w)),
+                              make_float2(to_f(y[0]), to_f(y[1])));
+        mine[j][0] = a.x, mine[j][1] = a.y, mine[j][2] = b.x, mine[j][3] = b.y;
       }
-      split_tile(ks[2 * jp], ks[2 * jp + 1], ur0, ur1, ah[jp], al[jp]);
+      split_tile(mine[2 * jp], mine[2 * jp + 1], ur0, ur1, ah[2 + jp], al[2 + jp]);
     }
     const uint4* Tf = reinterpret_cast<const uint4*>(st + B_AT) + lane;
-    float x0[4][4] = {}, x1[4][4] = {};  // u, scaled as r and T are
-    tri_product<0>(x0, ah, al, Tf);
-    tri_product<4>(x1, ah, al, Tf);
-    // beta e^(G_C - G) u, the left operand of the state's update
-    const float fu0 = dr0 * uu0 * tdn, fu1 = dr1 * uu1 * tdn;
-    auto weigh = [&](const float (&x)[4], int j, float (&y)[4]) {
-      const float2 c2 = *reinterpret_cast<const float2*>(vec + kGdC2 + 8 * j + 2 * c);
-      const float2 a = mul2(make_float2(x[0], x[1]), c2), b = mul2(make_float2(x[2], x[3]), c2);
-      y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
-    };
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      float y[2][4];
-      weigh(kk < 2 ? x0[2 * kk] : x1[2 * kk - 4], 2 * kk, y[0]);
-      weigh(kk < 2 ? x0[2 * kk + 1] : x1[2 * kk - 3], 2 * kk + 1, y[1]);
-      split_tile(y[0], y[1], fu0, fu1, ah[kk], al[kk]);
+    float x[4][4] = {};  // u of this warp's tokens, scaled as r and T are
+    {
+      unsigned (&oh)[2][4] = *reinterpret_cast<unsigned(*)[2][4]>(&ah[2]), (&ol)[2][4] = *reinterpret_cast<unsigned(*)[2][4]>(&al[2]);
+      if (half == 0) {
+        put_frag(r_ex, oh[0], ol[0]);
+        put_frag(r_ex + 64, oh[1], ol[1]);
+        bar_arrive(bar + 1, 64);
+        tri_product<0, 0, 2>(x, oh, ol, Tf);
+      } else {
+        tri_product<4, 2, 4>(x, oh, ol, Tf);
+        bar_sync(bar + 1, 64);
+        get_frag(r_ex, ah[0], al[0]);
+        get_frag(r_ex + 64, ah[1], al[1]);
+        tri_product<4, 0, 2>(x, ah, al, Tf);
+      }
     }
-    // S <- e^G_C S + u k, and u for the output warp between the first MMAs
+    // beta e^(G_C - G) u, the left operand of the state's update, and u for the output warps
+    const float fu0 = dr0 * uu0 * tdn, fu1 = dr1 * uu1 * tdn;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      float y[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 c2 = *reinterpret_cast<const float2*>(vec + kGdC2 + 32 * half + 16 * kk + 8 * i + 2 * c);
+        const float2 a = mul2(make_float2(x[2 * kk + i][0], x[2 * kk + i][1]), c2);
+        const float2 b = mul2(make_float2(x[2 * kk + i][2], x[2 * kk + i][3]), c2);
+        y[i][0] = a.x, y[i][1] = a.y, y[i][2] = b.x, y[i][3] = b.y;
+      }
+      unsigned dh[4], dl[4];
+      split_tile(y[0], y[1], fu0, fu1, dh, dl);
+      put_frag(d_ex + (2 * half + kk) * 64, dh, dl);
+    }
+    bar_sync(bar, 64);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) get_frag(d_ex + kk * 64, ah[kk], al[kk]);
+    // S <- e^G_C S + u k, and u for the output warps between the first MMAs
     const float ds0 = du0 * cdn, ds1 = du1 * cdn;
     m0 = m1 = 0.f;
 #pragma unroll
-    for (int jp = 0; jp < NK / 4; ++jp) {
-      float x[4][4] = {};
+    for (int jp = 0; jp < NH / 4; ++jp) {
+      float z[4][4] = {};
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         unsigned b[4], d[4];
-        ldsm4t(b, k_s + kq_off<DK>(16 * kk + tt, 4 * jp + tu));
-        ldsm4t(d, k_s + kq_off<DK>(16 * kk + tt, 4 * jp + 2 + tu));
-        if (jp == 0) {
+        ldsm4t(b, k_s + kq_off<DK>(16 * kk + tt, half * NH + 4 * jp + tu));
+        ldsm4t(d, k_s + kq_off<DK>(16 * kk + tt, half * NH + 4 * jp + 2 + tu));
+        if (jp == 0 && kk < 2) {
           unsigned uh[4], ul[4];
-          split_tile(kk < 2 ? x0[2 * kk] : x1[2 * kk - 4], kk < 2 ? x0[2 * kk + 1] : x1[2 * kk - 3], fu0, fu1, uh, ul);
-          u_ex[(2 * kk) * 32] = make_uint4(uh[0], uh[1], uh[2], uh[3]);
-          u_ex[(2 * kk + 1) * 32] = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+          split_tile(x[2 * kk], x[2 * kk + 1], fu0, fu1, uh, ul);
+          put_frag(u_ex + (2 * half + kk) * 64, uh, ul);
+          if (kk == 1) {
+            if (half == 0 && c == 0) sc[64 + g] = du0, sc[72 + g] = du1;
+            bar_arrive(bar + 3, 128);  // u is split; this warp reads V, T and the factors no more
+          }
         }
-        mma_acc(x[0], al[kk], b[0], b[1]);
-        mma_acc(x[1], al[kk], b[2], b[3]);
-        mma_acc(x[2], al[kk], d[0], d[1]);
-        mma_acc(x[3], al[kk], d[2], d[3]);
-        mma_acc(x[0], ah[kk], b[0], b[1]);
-        mma_acc(x[1], ah[kk], b[2], b[3]);
-        mma_acc(x[2], ah[kk], d[0], d[1]);
-        mma_acc(x[3], ah[kk], d[2], d[3]);
-      }
-      if (jp == 0) {
-        if (c == 0) sc[16 + g] = du0, sc[24 + g] = du1;
-        bar_arrive(bar, 64);
+        mma_acc(z[0], al[kk], b[0], b[1]);
+        mma_acc(z[1], al[kk], b[2], b[3]);
+        mma_acc(z[2], al[kk], d[0], d[1]);
+        mma_acc(z[3], al[kk], d[2], d[3]);
+        mma_acc(z[0], ah[kk], b[0], b[1]);
+        mma_acc(z[1], ah[kk], b[2], b[3]);
+        mma_acc(z[2], ah[kk], d[0], d[1]);
+        mma_acc(z[3], ah[kk], d[2], d[3]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float(&z)[4] = s[4 * jp + i];
-        const float2 a = fma2(dup(el), make_float2(z[0], z[1]), mul2(make_float2(x[i][0], x[i][1]), dup(ds0)));
-        const float2 b = fma2(dup(el), make_float2(z[2], z[3]), mul2(make_float2(x[i][2], x[i][3]), dup(ds1)));
-        z[0] = a.x, z[1] = a.y, z[2] = b.x, z[3] = b.y;
+        float(&w)[4] = s[4 * jp + i];
+        const float2 a = fma2(dup(el), make_float2(w[0], w[1]), mul2(make_float2(z[i][0], z[i][1]), dup(ds0)));
+        const float2 b = fma2(dup(el), make_float2(w[2], w[3]), mul2(make_float2(z[i][2], z[i][3]), dup(ds1)));
+        w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
         m0 = fmaxf(m0, fmaxf(fabsf(a.x), fabsf(a.y)));
         m1 = fmaxf(m1, fmaxf(fabsf(b.x), fabsf(b.y)));
       }
@@ -1044,7 +1074,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   }
   if (!active) return;
 #pragma unroll
-  for (int j = 0; j < NK; ++j) {
+  for (int j = 0; j < NH; ++j) {
     *reinterpret_cast<float2*>(Sg + 8 * j) = make_float2(s[j][0], s[j][1]);
     *reinterpret_cast<float2*>(Sg + 8 * DK + 8 * j) = make_float2(s[j][2], s[j][3]);
   }
