@@ -598,8 +598,8 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 // fit on an SM.  DEEP, for grids that give every block an SM of its own, has two of all of them and fetches a chunk ahead.
 //
 // Bound: per chunk and group, at dk = 128, 504 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM) and
-// about 160 KB through shared memory, in a chain of dependent steps.  Alone on its SM a block takes 2.06 us a chunk
-// (512 chunks of 32 heads, 128 blocks, in 1.06 ms; tensor cores 54% busy; 2.35 us with one chain warp per group); two
+// about 160 KB through shared memory, in a chain of dependent steps.  Alone on its SM a block takes 2.1 us a chunk
+// (512 chunks of 32 heads, 128 blocks, in 1.08 ms; tensor cores 53% busy; 2.35 us with one chain warp per group); two
 // blocks on an SM take 4.1 us for a chunk each (tensor cores 53%, shared memory 70% busy).
 
 constexpr int kGdGroups = 2;  // of 16 rows per block
@@ -929,6 +929,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     unsigned sh[2][4], sl[2][4];
     split_tile(s[0], s[1], up0, up1, sh[0], sl[0]);
     bar_sync(0, NT);  // K and Q are there (DEEP: the whole chunk)
+    // n-tiles 0-3 are this warp's tokens, 4-7 the other's
     float ks[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) ks[j][0] = ks[j][1] = ks[j][2] = ks[j][3] = 0.f;
@@ -937,7 +938,8 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     for (int kk = 0; kk < KH; ++kk) {
       unsigned b[4][4];
 #pragma unroll
-      for (int jp = 0; jp < 4; ++jp) ldsm4(b[jp], k_s + kq_off<DK>(16 * jp + bt, 2 * (half * KH + kk) + bu));
+      for (int jp = 0; jp < 4; ++jp)
+        ldsm4(b[jp], k_s + (jp < 2 ? 0 : (1 - 2 * half) * 64 * DK) + kq_off<DK>(16 * (jp & 1) + 32 * half + bt, 2 * (half * KH + kk) + bu));
       const int now = kk & 1;
       put_frag(s_ex + (half * KH + kk) * 64, sh[now], sl[now]);
       if (DEEP && kk == KH - 1) bar_arrive(bar + 2, 128);  // S is split
@@ -949,27 +951,18 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     }
     // the other warp's tokens to it, in the place where it will put its weighed u
     float (&mine)[4][4] = *reinterpret_cast<float(*)[4][4]>(&ks[0]);
-    {
-      float t[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float d = i < 2 ? dn0 : dn1, a = ks[j][i] * d, b = ks[4 + j][i] * d;
-          t[j][i] = half ? a : b;
-          mine[j][i] = half ? b : a;
-        }
-        d_ex[((1 - half) * 4 + j) * 32] = make_uint4(__float_as_uint(t[j][0]), __float_as_uint(t[j][1]), __float_as_uint(t[j][2]),
-                                                    __float_as_uint(t[j][3]));
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = mul2(make_float2(ks[4 + j][0], ks[4 + j][1]), dup(dn0)), b = mul2(make_float2(ks[4 + j][2], ks[4 + j][3]), dup(dn1));
+      *reinterpret_cast<float4*>(d_ex + ((1 - half) * 4 + j) * 32) = make_float4(a.x, a.y, b.x, b.y);
     }
     if constexpr (DEEP) bar_sync(bar, 64);
     else bar_sync(0, NT);  // also: V, T, P and the factors are there; S is split
-    // bounds of r and u, and the scales from them
+    // bounds of r and u, and the scales from them (measured: slower before or among the MMAs above)
+    float ur0, dr0, ur1, dr1, uu0, du0, uu1, du1;
     const float root = (DK == 128 ? 11.3137085f : 8.f) * vec[kGdKn];
     const float r0 = fmaf(root, fmaxf(sc[32 + g], sc[48 + g]), fmaxf(sc[80 + g], sc[96 + g]));
     const float r1 = fmaf(root, fmaxf(sc[40 + g], sc[56 + g]), fmaxf(sc[88 + g], sc[104 + g]));
-    float ur0, dr0, ur1, dr1, uu0, du0, uu1, du1;
     row_scale(r0, ur0, dr0);
     row_scale(r1, ur1, dr1);
     row_scale(r0 * vec[kGdTsum], uu0, du0);
@@ -985,12 +978,12 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       for (int i = 0; i < 2; ++i) {
         const int j = 2 * jp + i;
         const float2 bk = *reinterpret_cast<const float2*>(vec + kGdBk + 32 * half + 8 * j + 2 * c);
-        const uint4 o = d_ex[(half * 4 + j) * 32];
+        const float4 o = *reinterpret_cast<const float4*>(d_ex + (half * 4 + j) * 32);
         const T* x = reinterpret_cast<const T*>(&v[i]);
         const T* y = reinterpret_cast<const T*>(&v[2 + i]);
-        const float2 a = fma2(bk, make_float2(mine[j][0] + __uint_as_float(o.x), mine[j][1] + __uint_as_float(o.y)),
+        const float2 a = fma2(bk, fma2(make_float2(mine[j][0], mine[j][1]), dup(dn0), make_float2(o.x, o.y)),
                               make_float2(to_f(x[0]), to_f(x[1])));
-        const float2 b = fma2(bk, make_float2(mine[j][2] + __uint_as_float(o.z), mine[j][3] + __uint_as_float(o.w)),
+        const float2 b = fma2(bk, fma2(make_float2(mine[j][2], mine[j][3]), dup(dn1), make_float2(o.z, o.w)),
                               make_float2(to_f(y[0]), to_f(y[1])));
         mine[j][0] = a.x, mine[j][1] = a.y, mine[j][2] = b.x, mine[j][3] = b.y;
       }
