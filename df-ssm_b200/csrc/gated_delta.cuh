@@ -44,10 +44,13 @@ __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 
-// Log decay of one token; softplus(x) = x from 20 on, where e^-x is below half an fp32 ulp of x.
+// Log decay of one token; softplus(x) = x from 20 on, where e^-x is below half an fp32 ulp of x.  It ends at -256:
+// e^-256 times any fp32 number is 0 in fp32, and sums of what is left tell the later tokens' decays apart, which a gate
+// of -1e20 or -infinity (the largest values of a) would drown.  A NaN stays.
 __device__ __forceinline__ float gd_log_decay(float a, float dt_bias, float A_log) {
   const float x = a + dt_bias;
-  return -expf(A_log) * (x > 20.f ? x : log1pf(expf(x)));
+  const float g = -expf(A_log) * (x > 20.f ? x : log1pf(expf(x)));
+  return g < -256.f ? -256.f : g;
 }
 __device__ __forceinline__ float gd_beta(float b) { return 1.0f / (1.0f + expf(-b)); }
 

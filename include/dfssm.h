@@ -278,8 +278,8 @@ size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_hea
  * tokens changes nothing; rows of o outside every sequence are left as they were.  `workspace` is device
  * memory of dfssm_gated_delta_workspace bytes, 256-byte aligned, used by this call alone until it has run:
  * calls that may overlap (other streams, graphs replayed at once) need one each.  Neither call allocates or
- * synchronises, and both can be captured into a graph.  A NaN or infinite input spoils the rows of o and the
- * state of its own sequence, from the start of its 64 tokens on, and nothing else. */
+ * synchronises, and both can be captured into a graph.  A NaN or infinite q, k or v, or a NaN a or b, spoils the rows
+ * of o and the state of its own sequence, from the start of its 64 tokens on, and nothing else. */
 int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, const void* v, int ld_v, const void* a,
                               int ld_a, const void* b, int ld_b, const float* A_log, const float* dt_bias,
                               float* state, int n_slots, const int32_t* slots, const int32_t* cu_seqlens, int n_seq,
@@ -293,12 +293,12 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
  * index first among equal ones, and w = exp(x - max x):
  *   top-k  the first top_k tokens stay (top_k <= 0: all);
  *   top-p  of these, a token stays while the weight before it is <= top_p of their sum (>= 1: all);
- *   min-p  of these, the first one and those with w >= min_p stay;
+ *   min-p  of these, those with w >= min(min_p, 1) stay;
  *   next   the first kept token in vocabulary order whose running weight exceeds uniform[b] x the kept
  *          weight (uniform is taken into [0, 1)).
  * temperature <= 0 takes the first token of the order.  NaN and -inf logits never stay; a row that holds
  * nothing else gets next = -1, kept_count 0 and prob 0.  temperature, top_p, min_p fp32 [batch] and top_k
- * int32 [batch] (device) may each be NULL: 1, all, 0, all.  seen_bits as in dfssm_sample, or NULL.
+ * int32 [batch] (device) may each be NULL: 1, all, 0, all.  seen_bits as in dfssm_sample but not written, or NULL.
  * Outputs: next int32 [batch]; kept_count int32 [batch] and prob fp32 [batch] (the token's share of the kept
  * weight), either may be NULL.  Weights are summed as 64-bit integers, so the choice does not depend on the
  * order of any sum.  vocab up to 2^24. */

@@ -216,3 +216,20 @@ def test_model_samples_from_its_logits():
     assert torch.equal(m.sample(u, temperature=0.0), logits.argmax(-1).int())
     m.step(tokens)
     m.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[150], [5]])
+def test_decays_of_the_largest_gates(ops, lens, dtype):
+    """a at the type's largest value and at infinity: that token forgets everything before it, and the tokens after it
+    decay by gates of their own, in every form of the op."""
+    heads = (1, 4, 128, 32)
+    x = make(heads, lens[0], 1, dtype, 21)
+    x["a"][2::9, 0] = torch.finfo(dtype).max
+    x["a"][1::70, 1] = float("inf")
+    x["a"][3::20, 2] = float("inf")
+    x["a"][::2, 3] = -torch.finfo(dtype).max
+    x["a"][1, 3] = float("-inf")
+    ref = reference(x, lens, x["state"].cpu().numpy(), 0.3, True)
+    o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.3)
+    check(o, x["state"], ref, lens, dtype)
