@@ -264,8 +264,8 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
   if (n_seq == 0 || tokens == 0) return DFSSM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // The token loop for sequences of few tokens: it takes about 1 us a token of the longest one, the chunked kernels 16 us
-  // and more whatever the length up to 64 (64 heads, one sequence of 12 / 16 tokens: 14.7 / 18.5 us against 17;
-  // 64 sequences of 4 / 16: 83 / 256 us against 252 / 255).  The lengths are not known here, so the average decides,
+  // and more whatever the length up to 64 (64 heads, one sequence of 12 / 16 tokens: 14.7 / 18.5 us against 16;
+  // 64 sequences of 4 / 16: 83 / 256 us against 240).  The lengths are not known here, so the average decides,
   // well below the crossover, since one of the sequences may hold most of the tokens.
   if (tokens <= 15 || tokens <= 4LL * n_seq) return launch_loop(p, dk, dtype, s);
   char* w = static_cast<char*>(workspace);

@@ -2,8 +2,8 @@
 
 Thin checked wrappers of the C ABI's dfssm_gated_delta_step, dfssm_gated_delta_prefill and
 dfssm_sample_filtered (include/dfssm.h has the formulas): they take CUDA tensors, run on the tensors'
-device and its current stream, neither synchronise nor keep anything between calls, and raise ValueError
-for arguments that do not fit.  A gated delta state [slots, v_heads, dv, dk] is the layout of
+device and its current stream, neither synchronise nor keep anything between calls, record no gradients, and
+raise ValueError for arguments that do not fit.  Outputs must not overlap inputs.  A gated delta state [slots, v_heads, dv, dk] is the layout of
 DFSSMModel.h_states; logits come from DFSSMModel.forward or dfssm_lm_head_argmax.
 """
 from __future__ import annotations
@@ -139,7 +139,8 @@ def gated_delta_step(q, k, v, a, b, A_log, dt_bias, state, *, slots=None, scale:
     q, k [B, k_heads, dk], v [B, v_heads, dv], a, b [B, v_heads] in fp16 or bf16 (rows may be strided views,
     as slices of one projection are); A_log, dt_bias fp32 [v_heads]; state fp32 [slots, v_heads, dv, dk],
     updated in place; slots int32 [B] on the device (None: sequence i is in slot i).  scale defaults to
-    dk ** -0.5.  Returns o [B, v_heads, dv] (`out` if given)."""
+    dk ** -0.5.  Returns o [B, v_heads, dv] (`out` if given).  A row whose slot does not exist (-1 for the padding of a
+    batch) or is taken by an earlier row is left out: its row of a new o is undefined."""
     n_seq = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
     index, head, tail, out, dims = _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale)
     _call(index, _lib.load().dfssm_gated_delta_step, *head, n_seq, *tail, int(bool(qk_norm)), dims[-1])
