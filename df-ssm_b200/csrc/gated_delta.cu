@@ -162,8 +162,17 @@ int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16,
   const int parts = (p.dv + 16 * kGdGroups - 1) / (16 * kGdGroups);
   const long long grid = (long long)p.n_seq * p.v_heads * parts;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
-  fn<<<(unsigned)grid, 128 * kGdGroups, bytes, s>>>(p, blocks, kq16, order, parts, slots_total);
-  DFSSM_CU(cudaGetLastError());
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(128 * kGdGroups);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  DFSSM_CU(cudaLaunchKernelEx(&cfg, fn, p, blocks, kq16, order, parts, slots_total));
   return DFSSM_OK;
 }
 
@@ -185,10 +194,11 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
-  const long long walks = (long long)p.n_seq * p.v_heads * ((p.dv + 31) / 32);
+  const bool at_once = (long long)p.n_seq * p.v_heads * ((p.dv + 31) / 32) <= sms;  // every block of the walk has an SM
   // The sequences by falling length (a long one that starts last runs alone), with their slots looked up.  It costs
-  // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself.
-  int4* order = p.n_seq <= 512 ? reinterpret_cast<int4*>(workspace + gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK,
+  // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself, as
+  // it does where all start at once.
+  int4* order = !at_once && p.n_seq <= 512 ? reinterpret_cast<int4*>(workspace + gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK,
                                                                                  std::is_same<T, __half>::value ? DFSSM_F16 : DFSSM_BF16) -
                                                          (size_t)p.n_seq * 16)
                                : nullptr;
@@ -196,8 +206,8 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
   fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group);
   DFSSM_CU(cudaGetLastError());
-  return walks <= sms ? launch_walk<T, DK, true>(p, workspace, kq16, order, (int)n, s)  // every block has an SM
-                      : launch_walk<T, DK, false>(p, workspace, kq16, order, (int)n, s);
+  return at_once ? launch_walk<T, DK, true>(p, workspace, kq16, order, (int)n, s)
+                 : launch_walk<T, DK, false>(p, workspace, kq16, order, (int)n, s);
 }
 
 // What both entry points ask of their arguments.

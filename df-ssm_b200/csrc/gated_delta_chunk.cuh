@@ -108,6 +108,10 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// The walk is launched while the last blocks of the prep kernel still run (programmatic dependent launch): prep_done
+// returns when all of them have ended and what they wrote can be read.
+__device__ __forceinline__ void let_walk_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void prep_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -258,6 +262,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   float* cold = rowd + 64;   // e^(last of w's block - G_w) rk_w beta_w
   float* red = cold + 64;    // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
+  let_walk_start();
   const int rep = p.v_heads / p.k_heads;
   const int grp = blockIdx.x % groups, hk = (blockIdx.x / groups) % p.k_heads, num = blockIdx.x / (groups * p.k_heads);
   if (walks && blockIdx.x == 0) {
@@ -690,6 +695,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   const int part = blockIdx.x % parts, h = (blockIdx.x / parts) % p.v_heads, nth = blockIdx.x / (parts * p.v_heads);
   int first, count, slot, seq;
   if (walks) {
+    prep_done();
     const int4 w = walks[nth];
     first = w.x, count = w.y, slot = w.z, seq = w.w;
   } else {
@@ -697,7 +703,10 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     gd_range(p.cu, seq, p.tokens, first, count);
     slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
   }
-  if (slot < 0 || count == 0) return;
+  if (slot < 0 || count == 0) {
+    prep_done();  // no block ends before the kernel ahead has
+    return;
+  }
   const int base = first / kGdC + seq;  // gd_chunk_base
   const int chunks = min((count + kGdC - 1) / kGdC, slots_total - base);
   const int hk = h / (p.v_heads / p.k_heads);
@@ -782,9 +791,11 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       v1 = quad_max(v1);
       if (c == 0) sc[80 + 16 * half + g] = v0, sc[88 + 16 * half + g] = v1;
     };
+    if (BF) prep_done();
     load_k(0);
     load_q(0);
     if (!DEEP) cp_commit();
+    if (!BF) prep_done();
     load_vb(0);
     cp_commit();
     if constexpr (DEEP) {
