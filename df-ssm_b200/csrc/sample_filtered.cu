@@ -16,12 +16,11 @@
 // where it fits (about 51,000 tokens; else every pass reads the logits again, from L2).  No pass sorts or selects
 // over the whole row:
 //   - with top-k, the k-th largest of the threads' own largest values bounds the k-th largest x from below;
-//     the few tokens above it go to a list that the cluster's first block sorts, and the rest of the row is not
-//     looked at again;
+//     the few tokens above it go to a list that the cluster's first block sorts, filters and draws from, and the
+//     rest of the row is not looked at again;
 //   - with top-p alone, a histogram of the weights (1024 bins of x, one pass) finds the bin that holds the
-//     boundary, whose tokens are sorted;
-//   - the result of either is a cut {x, how many of the tokens equal to it stay}, and the draw is one more pass
-//     that weighs what the cut keeps.
+//     boundary, whose tokens are sorted for the cut {x, how many of the tokens equal to it stay}, and the draw is
+//     one more pass that weighs what the cut keeps.
 // Rows where the list would overflow (thousands of equal logits at the cut, top_k in the thousands) select the
 // cut by four rounds over 8 bits of x's order-preserving key instead.
 //
@@ -301,30 +300,29 @@ __device__ __forceinline__ V sf_warps(const V* red, int wid, V& total) {
   return __shfl_sync(0xffffffffu, upto - own, wid);
 }
 
-// Adds the tokens of a warp's tile that `take` accepts to the warp's pool (64 floats, `have` in use) and runs
-// use(x) whenever 32 are there.
+// Adds the tokens of a warp's tile that `take` accepts to the warp's pool (kSfPool floats, `have` < 32 in use) and runs
+// use(x) for 32 of them as often as there are as many.
+constexpr int kSfPool = 192;
 template <typename F, typename G>
 __device__ __forceinline__ void sf_pool(float* pool, int& have, const float4& v, F take, G use) {
   const int lane = threadIdx.x & 31;
   const float x[4] = {v.x, v.y, v.z, v.w};
+  bool in[4], any = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) any |= in[j] = take(x[j]);
+  if (!__any_sync(0xffffffffu, any)) return;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const bool in = take(x[j]);
-    const unsigned all = __ballot_sync(0xffffffffu, in);
-    if (all) {
-      if (in) pool[have + __popc(all & ((1u << lane) - 1))] = x[j];
-      have += __popc(all);
-      if (have >= 32) {
-        __syncwarp();
-        use(pool[lane]);
-        have -= 32;
-        const float rest = pool[32 + lane];
-        __syncwarp();
-        pool[lane] = rest;
-        __syncwarp();
-      }
-    }
+    const unsigned all = __ballot_sync(0xffffffffu, in[j]);
+    if (in[j]) pool[have + __popc(all & ((1u << lane) - 1))] = x[j];
+    have += __popc(all);
   }
+  __syncwarp();
+  while (have >= 32) {
+    have -= 32;
+    use(pool[have + lane]);
+  }
+  __syncwarp();
 }
 
 // Compare-exchange steps of a bitonic sort at distances 32 .. 1 among the 64 keys of a warp, for the merges of length
@@ -367,24 +365,50 @@ __device__ __forceinline__ void sf_scan64(const u64 (&v)[2], u64 (&before)[2], u
   before[1] = first + b - v[1];
   total = first + __shfl_sync(0xffffffffu, b, 31);
 }
+// The places of a warp's two keys (or zeros) among list[0..n): how many there are larger.
+__device__ __forceinline__ void sf_places(const u64* list, int n, const u64 (&key)[2], int (&place)[2]) {
+  place[0] = place[1] = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) {
+    const u64 o = list[j];
+    place[0] += o > key[0];
+    place[1] += o > key[1];
+  }
+}
 
-// The draw among up to 64 kept tokens {key of x, complement of the index}, zeros behind them, by one warp.
-__device__ __forceinline__ void sf_draw64(const SampleArgs& p, int b, float u, const Weigh& weigh, u64 (&key)[2], int kept) {
-  u64 w[2], before[2], total;
-  double exact[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) key[e] = (key[e] << 32) | (key[e] >> 32);
-  sf_sort64(key);  // in vocabulary order
+// The draw among list[0..kept), kept <= 64, {key of x, complement of the index}, by one warp; exact: the weights of the
+// lane's keys, l and l + 32.  The list is overwritten.
+__device__ __forceinline__ void sf_draw64(const SampleArgs& p, int b, float u, u64* list, const double (&exact)[2], int kept) {
+  const int lane = threadIdx.x & 31;
+  u64 key[2], w[2], before[2], total;
+  int place[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    exact[e] = key[e] ? weigh.scaled(sf_unkey((uint32_t)key[e])) : 0.0;
-    w[e] = Weigh::fix(exact[e]);
+    const u64 k = lane + 32 * e < kept ? list[lane + 32 * e] : 0ull;
+    key[e] = (k << 32) | (k >> 32);
   }
+  __syncwarp();
+  list[lane] = key[0];
+  list[lane + 32] = key[1];
+  __syncwarp();
+  sf_places(list, kept, key, place);  // in vocabulary order
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + 32 * e < kept) list[place[e]] = Weigh::fix(exact[e]);
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 2; ++e) w[e] = lane + 32 * e < kept ? list[lane + 32 * e] : 0ull;
   sf_scan64(w, before, total);
   const u64 target = min((u64)((double)u * (double)total), total - 1);
+  int at = -1;  // the place that is drawn
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (target >= before[e] && target < before[e] + w[e]) at = lane + 32 * e;
+  at = __reduce_max_sync(0xffffffffu, at);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    if (target >= before[e] && target < before[e] + w[e]) {
+    if (lane + 32 * e < kept && place[e] == at) {
       p.next[b] = (int)(0xffffffffu - (unsigned)(key[e] >> 32));
       if (p.kept) p.kept[b] = kept;
       if (p.prob) p.prob[b] = (float)(exact[e] / (double)total);
@@ -392,10 +416,14 @@ __device__ __forceinline__ void sf_draw64(const SampleArgs& p, int b, float u, c
   }
 }
 
-// Descending sort of list[0..n), n <= kSfList, all different: up to 256 by counting, more by a bitonic sort, padded with
-// zeros to a power of two, by half as many threads as entries: distances below 64 in registers, the others
-// through the list.  Begins and ends with a block barrier.
-__device__ void sf_sort(u64* list, int n) {
+// Descending sort of list[0..n), n <= kSfList, all different.  Up to 256 by counting.  More go to kSfBins buckets by
+// bin(key), which must not fall along the order, and are counted within theirs (2 us for some 1500 keys; a bitonic sort takes
+// 15); where a bucket holds more than kSfCrowd, by a bitonic sort, padded with zeros to a power of two, by half as many
+// threads as entries: distances below 64 in registers, the others through the list.  bins: kSfBins words.  Begins and
+// ends with a block barrier.
+constexpr int kSfCrowd = 64;
+template <typename F>
+__device__ __forceinline__ void sf_sort(u64* list, int n, unsigned* bins, u64* red, F bin) {
   int size = 64;
   while (size < n) size <<= 1;
   __syncthreads();
@@ -410,6 +438,46 @@ __device__ void sf_sort(u64* list, int n) {
     if (part == 0 && i < n) list[place] = key;
     __syncthreads();
     return;
+  }
+  {
+    bins[threadIdx.x] = 0u;
+    __syncthreads();
+    u64 e[2], total;
+    int b[2], at[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = threadIdx.x + h * kSfThreads;
+      if (i < n) {
+        e[h] = list[i];
+        b[h] = bin(e[h]);
+        at[h] = atomicAdd(bins + b[h], 1u);
+      }
+    }
+    __syncthreads();
+    const unsigned here = bins[threadIdx.x], first = (unsigned)sf_scan((u64)here, red, total);
+    const bool crowded = __syncthreads_or(here > kSfCrowd);
+    if (!crowded) {
+      bins[threadIdx.x] = first | here << 16;
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if ((int)threadIdx.x + h * kSfThreads < n) list[(bins[b[h]] & 0xffff) + at[h]] = e[h];
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if ((int)threadIdx.x + h * kSfThreads < n) {
+          const unsigned from = bins[b[h]] & 0xffff, to = from + (bins[b[h]] >> 16);
+          at[h] = from;
+          for (unsigned j = from; j < to; ++j) at[h] += list[j] > e[h];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if ((int)threadIdx.x + h * kSfThreads < n) list[at[h]] = e[h];
+      __syncthreads();
+      return;
+    }
   }
   const int workers = size / 2;
   if (threadIdx.x < workers) {
@@ -456,14 +524,17 @@ __device__ int sf_gather(const Row<T>& row, Group& grp, u64* list, Shared& sh, F
 #pragma unroll
     for (int j = 0; j < 4; ++j) any |= in[j] = take(x[j]);
     if (!__any_sync(0xffffffffu, any)) continue;
+    unsigned all[4];
+    int found = 0, at = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) found += __popc(all[j] = __ballot_sync(0xffffffffu, in[j]));
+    if (lane == 0) at = atomicAdd(count, found);
+    at = __shfl_sync(0xffffffffu, at, 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const unsigned all = __ballot_sync(0xffffffffu, in[j]);
-      if (!all) continue;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(count, __popc(all));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
-      if (in[j] && at < kSfList) to[at] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
+      const int place = at + __popc(all[j] & ((1u << lane) - 1));
+      if (in[j] && place < kSfList) to[place] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
+      at += __popc(all[j]);
     }
   }
   grp.sync();
@@ -534,8 +605,10 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   u64* list = reinterpret_cast<u64*>(dyn);  // [kSfList]; before it is filled, the histograms' words
   unsigned* cnt = reinterpret_cast<unsigned*>(dyn);
   unsigned *lo = cnt + 256, *hi = lo + kSfBins;
-  float* pool = reinterpret_cast<float*>(list + kSfList) + (threadIdx.x >> 5) * 64;  // one per warp
-  float* xs = reinterpret_cast<float*>(list + kSfList) + kSfWarps * 64;
+  unsigned* bins = reinterpret_cast<unsigned*>(list + kSfList);  // [2 kSfBins] of a sort
+  float* pool = reinterpret_cast<float*>(dyn) + (threadIdx.x >> 5) * kSfPool;  // in the draw: one per warp, over both
+  float* xs = reinterpret_cast<float*>(bins + 2 * kSfBins);
+  static_assert(kSfWarps * kSfPool * 4 == kSfList * 8 + 2 * kSfBins * 4, "");
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, V = p.vocab;
   Group grp{0, 1, 0};
   if (gridDim.y > 1) {  // a cluster is the blocks of one row
@@ -685,6 +758,7 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
       if (n <= kSfList) n = sf_gather(row, grp, list, sh, [&](float x) { return x >= bound && x > -INFINITY; });
     }
     if (n <= kSfList) {
+      // the first block orders them and draws
       if (chief) {
         const int n_k = min(n, k);
         if (n <= 64) {
@@ -692,28 +766,35 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
           if (wid == 0) {
             u64 key[2], w[2], before[2], total;
             double exact[2];
+            int place[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) key[e] = lane + 32 * e < n ? list[lane + 32 * e] : 0ull;
-            sf_sort64(key);
+            sf_places(list, n, key, place);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (lane + 32 * e < n) list[place[e]] = key[e];
+            __syncwarp();
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              exact[e] = lane + 32 * e < n_k ? weigh.scaled(sf_unkey((uint32_t)(key[e] >> 32))) : 0.0;
+              key[e] = lane + 32 * e < n_k ? list[lane + 32 * e] : 0ull;
+              exact[e] = key[e] ? weigh.scaled(sf_unkey((uint32_t)(key[e] >> 32))) : 0.0;
               w[e] = Weigh::fix(exact[e]);
             }
             sf_scan64(w, before, total);
             const u64 budget = top_p < 1.f ? (u64)(fmax((double)top_p, 0.0) * (double)total) : ~0ull;
-            int kept = 0;
+            int kept = 0;  // the first ones: every condition falls along the order
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const bool stay = lane + 32 * e < n_k && before[e] <= budget &&
-                                (sf_unkey((uint32_t)(key[e] >> 32)) == top || exact[e] >= least);
-              kept += __popc(__ballot_sync(0xffffffffu, stay));
-              if (!stay) key[e] = 0ull;
-            }
-            sf_draw64(p, b, u, weigh, key, kept);
+            for (int e = 0; e < 2; ++e)
+              kept += __popc(__ballot_sync(0xffffffffu, key[e] && before[e] <= budget &&
+                                                            (sf_unkey((uint32_t)(key[e] >> 32)) == top || exact[e] >= least)));
+            sf_draw64(p, b, u, list, exact, kept);
           }
         } else {
-          sf_sort(list, n);
+          const float low = fmaxf(bound, -0x1.fffffep127f), per = kSfBins / fmaxf(top - low, 1e-30f);
+          sf_sort(list, n, bins, sh.red, [&](u64 key) {
+            return min(kSfBins - 1, (int)((top - sf_unkey((uint32_t)(key >> 32))) * per));
+          });
           // weights in order: thread t has the tokens 2t and 2t + 1
           float x[2];
           u64 w[2], total;
@@ -732,33 +813,47 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
           for (int e = 0; e < 2; ++e)
             stay += 2 * tid + e < n_k && before + (e ? w[0] : 0) <= budget && (x[e] == top || exact[e] >= least);
           const int kept = sf_sum(stay, sh.ired);  // the first `kept` tokens: every condition falls along the order
-          if (kept <= 64 && wid == 0) {
-            u64 key[2];
+          if (kept <= 64) {
+            if (wid == 0) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) key[e] = lane + 32 * e < kept ? list[lane + 32 * e] : 0ull;
-            sf_draw64(p, b, u, weigh, key, kept);
+              for (int e = 0; e < 2; ++e)
+                exact[e] = lane + 32 * e < kept ? weigh.scaled(sf_unkey((uint32_t)(list[lane + 32 * e] >> 32))) : 0.0;
+              sf_draw64(p, b, u, list, exact, kept);
+            }
+            return;
           }
-          // more than 64: the draw below finds them again in vocabulary order
-          const uint32_t last = (uint32_t)(list[kept - 1] >> 32);
-          int equal = 0, ties = 0;
+          // the kept tokens in vocabulary order: {complement of the index, key of x}
+          u64 key[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) key[e] = list[2 * tid + e];
+          __syncthreads();
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (2 * tid + e < kept) list[2 * tid + e] = (key[e] << 32) | (key[e] >> 32);
+          const float per_token = (float)kSfBins / (float)V;
+          sf_sort(list, kept, bins, sh.red, [&](u64 key) {
+            return min(kSfBins - 1, (int)((float)(0xffffffffu - (unsigned)(key >> 32)) * per_token));
+          });
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int i = 2 * tid + e;
-            const bool same = i < n && (uint32_t)(list[i] >> 32) == last;
-            equal += same;
-            ties += same && i < kept;
+            exact[e] = i < kept ? weigh.scaled(sf_unkey((uint32_t)list[i])) : 0.0;
+            w[e] = Weigh::fix(exact[e]);
           }
-          equal = sf_sum(equal, sh.ired);
-          ties = sf_sum(ties, sh.ired);
-          if (tid < grp.blocks)
-            *grp.at(&sh.cut, tid) = kept <= 64 ? Cut{INFINITY, 0} : Cut{sf_unkey(last), ties == equal ? kSfAll : ties};
+          u64 from = sf_scan(w[0] + w[1], sh.red, total);
+          const u64 target = min((u64)((double)u * (double)total), total - 1);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (target >= from && target < from + w[e]) {
+              p.next[b] = (int)(0xffffffffu - (unsigned)(list[2 * tid + e] >> 32));
+              if (p.kept) p.kept[b] = kept;
+              if (p.prob) p.prob[b] = (float)(exact[e] / (double)total);
+            }
+            from += w[e];
+          }
         }
       }
-      if (n <= 64) return;  // after the gather no block reaches into another's memory
-      grp.sync();
-      cut = sh.cut;
-      if (cut.ties == 0) return;  // drawn
-      open_p = false;
+      return;  // after the gather no block reaches into another's memory
     } else {
       cut = sf_radix_cut(row, grp, weigh, cut, false, (u64)k, cnt, lo, hi);
     }
@@ -818,7 +913,10 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
         });
       if (n <= kSfList) {
         if (chief) {
-          sf_sort(list, n);
+          sf_sort(list, n, bins, sh.red, [&](u64 key) {
+            const float d = (top - sf_unkey((uint32_t)(key >> 32))) * scale - d0;
+            return min(kSfBins - 1, max(0, (int)(d * kSfBins)));
+          });
           float x[2];
           u64 v[2], total;
 #pragma unroll
@@ -1014,7 +1112,7 @@ template <typename T>
 int launch_sample(SampleArgs p, int batch, cudaStream_t s) {
   static SmemLimit limit;
   const auto fn = sample_filtered_kernel<T>;
-  const int list = kSfList * 8 + kSfWarps * 64 * 4, most = 232448 - 2048;  // 227 KB per block less the static part
+  const int list = kSfWarps * kSfPool * 4, most = 232448 - 2048;  // 227 KB per block less the static part
   const int capacity = (most - list) / 512 * 128;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), list + capacity * 4));
   cudaLaunchConfig_t cfg{};
