@@ -29,6 +29,8 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "op_host.h"
 
@@ -82,12 +84,12 @@ template <typename T>
 struct Row {
   const T* l;
   const uint32_t* seen;
-  const float* xs;  // the slice's x in shared memory (token i at xs[i - from]), or NULL: every pass computes them again
+  float* xs;        // `shared`: the slice's x in shared memory, token i at xs[i - from]; else every pass computes them again
   int V;            // the row's tokens
   int from, to;     // the block's slice of them
   float temp, rtemp, rep;
-  bool divide, mild, aligned;  // aligned: four logits at a time
-  bool lift;                   // the row's largest x is +inf: tokens there count as 0, all others as -inf
+  bool divide, mild, aligned, shared;  // aligned: four logits at a time
+  bool lift;  // the row's largest x is +inf: tokens there count as 0, all others as -inf (in xs they already are)
   __device__ __forceinline__ float4 from4(float4 v, int i) const {
     float* e = reinterpret_cast<float*>(&v);
     if (divide) {
@@ -135,35 +137,41 @@ struct Row {
     }
     return v;
   }
+  static __device__ __forceinline__ float lifted(float x) { return x == INFINITY ? 0.f : -INFINITY; }
+  template <bool SHARED>
   __device__ __forceinline__ float4 x4(int i) const {
-    float4 v = xs ? *reinterpret_cast<const float4*>(xs + (i - from)) : from4(logits4(i), i);
-    if (lift) {
-      v.x = v.x == INFINITY ? 0.f : -INFINITY;
-      v.y = v.y == INFINITY ? 0.f : -INFINITY;
-      v.z = v.z == INFINITY ? 0.f : -INFINITY;
-      v.w = v.w == INFINITY ? 0.f : -INFINITY;
+    if constexpr (SHARED) {
+      return *reinterpret_cast<const float4*>(xs + (i - from));
+    } else {
+      float4 v = from4(logits4(i), i);
+      if (lift) v = make_float4(lifted(v.x), lifted(v.y), lifted(v.z), lifted(v.w));
+      return v;
     }
-    return v;
+  }
+  // f(std::true_type or std::false_type for x4's argument): a pass compiled for each
+  template <typename F>
+  __device__ __forceinline__ void pass(F f) const {
+    if (shared) f(std::true_type());
+    else f(std::false_type());
   }
   // f(x, index) for four tokens at a time
   template <typename F>
   __device__ __forceinline__ void each4(F f) const {
-    for (int i = from + 4 * threadIdx.x; i < to; i += 4 * kSfThreads) {
-      const float4 v = x4(i);
-      const float x[4] = {v.x, v.y, v.z, v.w};
-      f(x, i);
-    }
+    pass([&](auto where) {
+      for (int i = from + 4 * threadIdx.x; i < to; i += 4 * kSfThreads) {
+        const float4 v = x4<decltype(where)::value>(i);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        f(x, i);
+      }
+    });
   }
   // f(x, index) for every token; behind the row's end x is -inf
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (int i = from + 4 * threadIdx.x; i < to; i += 4 * kSfThreads) {
-      const float4 v = x4(i);
-      f(v.x, i);
-      f(v.y, i + 1);
-      f(v.z, i + 2);
-      f(v.w, i + 3);
-    }
+    each4([&](const float(&x)[4], int i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(x[j], i + j);
+    });
   }
 };
 
@@ -516,27 +524,29 @@ __device__ int sf_gather(const Row<T>& row, Group& grp, u64* list, Shared& sh, F
   u64* const to = grp.at(list, 0);
   int* const count = grp.at(&sh.count, 0);
   const int lane = threadIdx.x & 31;
-  for (int i0 = row.from + 4 * (threadIdx.x - lane); i0 < row.to; i0 += 4 * kSfThreads) {
-    const int i = i0 + 4 * lane;
-    const float4 v = i < row.to ? row.x4(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    const float x[4] = {v.x, v.y, v.z, v.w};
-    bool in[4], any = false;
+  row.pass([&](auto where) {
+    for (int i0 = row.from + 4 * (threadIdx.x - lane); i0 < row.to; i0 += 4 * kSfThreads) {
+      const int i = i0 + 4 * lane;
+      const float4 v = i < row.to ? row.template x4<decltype(where)::value>(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      bool in[4], any = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) any |= in[j] = take(x[j]);
-    if (!__any_sync(0xffffffffu, any)) continue;
-    unsigned all[4];
-    int found = 0, at = 0;
+      for (int j = 0; j < 4; ++j) any |= in[j] = take(x[j]);
+      if (!__any_sync(0xffffffffu, any)) continue;
+      unsigned all[4];
+      int found = 0, at = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) found += __popc(all[j] = __ballot_sync(0xffffffffu, in[j]));
-    if (lane == 0) at = atomicAdd(count, found);
-    at = __shfl_sync(0xffffffffu, at, 0);
+      for (int j = 0; j < 4; ++j) found += __popc(all[j] = __ballot_sync(0xffffffffu, in[j]));
+      if (lane == 0) at = atomicAdd(count, found);
+      at = __shfl_sync(0xffffffffu, at, 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int place = at + __popc(all[j] & ((1u << lane) - 1));
-      if (in[j] && place < kSfList) to[place] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
-      at += __popc(all[j]);
+      for (int j = 0; j < 4; ++j) {
+        const int place = at + __popc(all[j] & ((1u << lane) - 1));
+        if (in[j] && place < kSfList) to[place] = ((u64)sf_key(x[j]) << 32) | (0xffffffffu - (unsigned)(i + j));
+        at += __popc(all[j]);
+      }
     }
-  }
+  });
   grp.sync();
   const int n = *count;
   grp.sync();  // everybody has read it: the list may be used again
@@ -621,7 +631,8 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   Row<T> row;
   row.l = static_cast<const T*>(p.logits) + (long long)b * p.ld;
   row.seen = p.seen ? p.seen + (size_t)b * ((V + 31) / 32) : nullptr;
-  row.xs = nullptr;
+  row.xs = xs;
+  row.shared = p.in_shared;
   row.V = V;
   row.from = min(V, grp.rank * p.slice);
   row.to = min(V, row.from + p.slice);
@@ -659,7 +670,6 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
       }
     }
   }
-  if (p.in_shared) row.xs = xs;
   const float mine = fmaxf(mine2[0], mine2[1]);
   if (tid < 64) sh.table[tid] = ldexp(exp2(tid / 64.0), p.shift);
   if (tid == 0) sh.pick = V;
@@ -693,7 +703,11 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
     row.lift = true;
     top = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) mine2[e] = mine2[e] == INFINITY ? 0.f : -INFINITY;
+    for (int e = 0; e < 2; ++e) mine2[e] = Row<T>::lifted(mine2[e]);
+    if (row.shared) {
+      for (int i = row.from + tid; i < row.to; i += kSfThreads) xs[i - row.from] = Row<T>::lifted(xs[i - row.from]);
+      __syncthreads();
+    }
   }
   const Weigh weigh{sh.table, (double)top, top, (p.shift + 1) * 0.69314718f + 0.5f};
   const double unit = sh.table[0], least = (double)min_p * unit;
@@ -974,69 +988,71 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   };
   u64 mass = 0;
   int count = 0, tie0 = 0;  // tie0: tokens equal to the cut before this warp's run
-  if (!count_ties) {
-    // the weights of the runs do not depend on the order within them
-    auto add = [&](float x) {
-      const double w = weight(x);
-      mass += Weigh::fix(fmax(w, 0.0));
-      count += w >= 0.0;
-    };
-    if (floor_x == -INFINITY) {
-      for (int i = i0 + 4 * lane; i < i1; i += 128) {
-        const float4 v = row.x4(i);
-        const float x[4] = {v.x, v.y, v.z, v.w};
+  row.pass([&](auto where) {
+    if (!count_ties) {
+      // the weights of the runs do not depend on the order within them
+      auto add = [&](float x) {
+        const double w = weight(x);
+        mass += Weigh::fix(fmax(w, 0.0));
+        count += w >= 0.0;
+      };
+      if (floor_x == -INFINITY) {
+        for (int i = i0 + 4 * lane; i < i1; i += 128) {
+          const float4 v = row.template x4<decltype(where)::value>(i);
+          const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mass += Weigh::biased(weigh.scaled(x[j]));
-          count += x[j] > -INFINITY;
+          for (int j = 0; j < 4; ++j) {
+            mass += Weigh::biased(weigh.scaled(x[j]));
+            count += x[j] > -INFINITY;
+          }
+          mass -= 4 * Weigh::kBias;
         }
-        mass -= 4 * Weigh::kBias;
+      } else {
+        int have = 0;
+        for (int i = i0; i < i1; i += 128) {
+          const float4 v = i + 4 * lane < i1 ? row.template x4<decltype(where)::value>(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          sf_pool(pool, have, v, kept_by_x, add);
+        }
+        __syncwarp();
+        if (have) add(lane < have ? pool[lane] : -INFINITY);
       }
     } else {
-      int have = 0;
+      int ties = 0;
+      for (int i = i0 + 4 * lane; i < i1; i += 128) {
+        const float4 v = row.template x4<decltype(where)::value>(i);
+        ties += (v.x == cut.x) + (v.y == cut.x) + (v.z == cut.x) + (v.w == cut.x);
+      }
+      ties = warp_sum(ties);
+      __syncthreads();
+      if (lane == 0) sh.ired[wid] = ties;
+      __syncthreads();
+      int all;
+      tie0 = sf_warps(sh.ired, wid, all);
+      const int* theirs = grp.share(sh.bcount, all);
+      for (int r = 0; r < grp.rank; ++r) tie0 += theirs[r];
+      int tie = tie0;
       for (int i = i0; i < i1; i += 128) {
-        const float4 v = i + 4 * lane < i1 ? row.x4(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        sf_pool(pool, have, v, kept_by_x, add);
-      }
-      __syncwarp();
-      if (have) add(lane < have ? pool[lane] : -INFINITY);
-    }
-  } else {
-    int ties = 0;
-    for (int i = i0 + 4 * lane; i < i1; i += 128) {
-      const float4 v = row.x4(i);
-      ties += (v.x == cut.x) + (v.y == cut.x) + (v.z == cut.x) + (v.w == cut.x);
-    }
-    ties = warp_sum(ties);
-    __syncthreads();
-    if (lane == 0) sh.ired[wid] = ties;
-    __syncthreads();
-    int all;
-    tie0 = sf_warps(sh.ired, wid, all);
-    const int* theirs = grp.share(sh.bcount, all);
-    for (int r = 0; r < grp.rank; ++r) tie0 += theirs[r];
-    int tie = tie0;
-    for (int i = i0; i < i1; i += 128) {
-      const float4 v = i + 4 * lane < i1 ? row.x4(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      const float x[4] = {v.x, v.y, v.z, v.w};
-      int before = tie;  // equal tokens before this lane's next one
+        const float4 v = i + 4 * lane < i1 ? row.template x4<decltype(where)::value>(i + 4 * lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        int before = tie;  // equal tokens before this lane's next one
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned eq = __ballot_sync(0xffffffffu, x[j] == cut.x);
-        before += __popc(eq & ((1u << lane) - 1));
-        tie += __popc(eq);
-      }
-      if (!kept_by_x(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])))) continue;
+        for (int j = 0; j < 4; ++j) {
+          const unsigned eq = __ballot_sync(0xffffffffu, x[j] == cut.x);
+          before += __popc(eq & ((1u << lane) - 1));
+          tie += __popc(eq);
+        }
+        if (!kept_by_x(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])))) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double w = weight(x[j]);
-        const bool same = x[j] == cut.x, stay = w >= 0.0 && !(same && before >= cut.ties);
-        mass += Weigh::fix(stay ? w : 0.0);
-        count += stay;
-        before += same;
+        for (int j = 0; j < 4; ++j) {
+          const double w = weight(x[j]);
+          const bool same = x[j] == cut.x, stay = w >= 0.0 && !(same && before >= cut.ties);
+          mass += Weigh::fix(stay ? w : 0.0);
+          count += stay;
+          before += same;
+        }
       }
     }
-  }
+  });
   mass = warp_sum(mass);
   count = warp_sum(count);
   __syncthreads();
@@ -1073,7 +1089,8 @@ __global__ void __launch_bounds__(kSfThreads) sample_filtered_kernel(const Sampl
   const int first = row.from + sh.pick * run, end = min(row.to, first + run);
   for (int i = first; i < end; i += 4 * kSfThreads) {
     const int at = i + 4 * tid;
-    const float4 v = at < end ? row.x4(at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (at < end) row.pass([&](auto where) { v = row.template x4<decltype(where)::value>(at); });
     const float x[4] = {v.x, v.y, v.z, v.w};
     int rank = 0;
     if (count_ties) {
