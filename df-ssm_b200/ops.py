@@ -3,8 +3,9 @@
 Thin checked wrappers of the C ABI's dfssm_gated_delta_step, dfssm_gated_delta_prefill and
 dfssm_sample_filtered (include/dfssm.h has the formulas): they take CUDA tensors, run on the tensors'
 device and its current stream, neither synchronise nor keep anything between calls, record no gradients, and
-raise ValueError for arguments that do not fit.  Outputs must not overlap inputs.  A gated delta state [slots, v_heads, dv, dk] is the layout of
-DFSSMModel.h_states; logits come from DFSSMModel.forward or dfssm_lm_head_argmax.
+raise ValueError for arguments that do not fit.  Outputs must not overlap inputs.  A gated delta state
+[slots, v_heads, dv, dk] is the layout of DFSSMModel.h_states; logits come from DFSSMModel.forward or
+dfssm_lm_head_argmax.
 """
 from __future__ import annotations
 
@@ -121,7 +122,13 @@ def _delta(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out, scale):
             ok = (ok and slots.dtype is torch.int32 and slots.shape == (n_seq,) and slots.get_device() == index
                   and slots.is_contiguous())
         if ok:
-            lq, lk, lv, la, lb, lo = _row(q), _row(k), _row(v), _row(a), _row(b), _row(out)
+            wide, deep = hk * dk, hv * dv
+            lq = wide if q.is_contiguous() else _row(q)
+            lk = wide if k.is_contiguous() else _row(k)
+            lv = deep if v.is_contiguous() else _row(v)
+            lo = deep if out.is_contiguous() else _row(out)
+            la = hv if a.is_contiguous() else _row(a)
+            lb = hv if b.is_contiguous() else _row(b)
             if None not in (lq, lk, lv, la, lb, lo):
                 return (index, (q.data_ptr(), lq, k.data_ptr(), lk, v.data_ptr(), lv, a.data_ptr(), la, b.data_ptr(), lb,
                                 A_log.data_ptr(), dt_bias.data_ptr(), state.data_ptr(), state.shape[0], slot),
