@@ -233,3 +233,31 @@ def test_decays_of_the_largest_gates(ops, lens, dtype):
     ref = reference(x, lens, x["state"].cpu().numpy(), 0.3, True)
     o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.3)
     check(o, x["state"], ref, lens, dtype)
+
+
+@pytest.mark.parametrize("shape", ["bulk", "coarse", "crowded", "far"])
+@pytest.mark.parametrize("B,V", [(9, 50281), (150, 6000)])
+def test_lists_of_every_length(ops, B, V, shape):
+    """top_k around every way a short list is ordered (by one warp, by counting, in buckets, in crowded ones), over
+    spread, equal and crowded logits, alone and with top-p and min-p that keep few or many of the list."""
+    rng = np.random.default_rng(len(shape) + B)
+    logits = (rng.standard_normal((B, V)) * 1.5).astype(np.float32)
+    if shape == "coarse":
+        logits = np.round(logits * 4) / 4  # dozens of equal ones at the cut
+    elif shape == "crowded":
+        logits = 3 + 1e-3 * logits
+        logits[:, 17] = 12.0  # the rest shares one bucket
+    elif shape == "far":
+        logits[:, 5] = 250.0
+        logits[::2, ::3] = -3e38
+    sizes = np.array([2, 31, 64, 65, 130, 257, 900, 1025, 2048])
+    k = sizes[np.arange(B) % len(sizes)]
+    u = rng.random(B).astype(np.float32)
+    dev = {"u": torch.tensor(u, device="cuda"), "logits": torch.tensor(logits, device="cuda")}
+    for top_p, min_p in ((None, None), (0.5, None), (0.97, 0.001), (None, 0.1)):
+        t, kept, prob = ops.sample_filtered(dev["logits"], dev["u"], top_k=torch.tensor(k, dtype=torch.int32, device="cuda"),
+                                            top_p=top_p, min_p=min_p)
+        for r in range(min(B, 27)):
+            want = sample_row(logits[r], u[r], 1.0, int(k[r]), 1.0 if top_p is None else top_p, min_p or 0.0)
+            assert (t[r].item(), kept[r].item()) == want[:2], (r, k[r], top_p, min_p, t[r].item(), kept[r].item(), want)
+            assert abs(prob[r].item() - want[2]) <= 2.0 ** -24 * want[2] + 1e-12
