@@ -18,10 +18,14 @@ namespace dfssm {
 // Bound: HBM.  A one-token call reads and writes 8 dk dv bytes of state per head and computes 7 dk dv
 // operations, far below the balance of the machine.
 constexpr int kGdWarps = 4;
+// Which prompts take the loop (at the C entry): sequences of up to kGdLoopMost tokens, looked for in calls of less than
+// kGdMixed tokens per sequence and up to kGdOrdered sequences, the most that one prep block puts in order.
+constexpr int kGdLoopMost = 12, kGdMixed = 32, kGdOrdered = 512;
 
+// Sequences of more than `most` tokens are left to the chunked kernels.
 template <typename T, int DK, int R>
 __global__ void __launch_bounds__(kGdWarps * 32)
-gated_delta_loop_kernel(const GatedDeltaArgs p, int row_blocks) {
+gated_delta_loop_kernel(const GatedDeltaArgs p, int row_blocks, int most) {
   constexpr int NV = DK / 32;  // columns per lane
   static_assert(R == 8, "the butterfly below is written for 16 sums");
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -32,7 +36,7 @@ gated_delta_loop_kernel(const GatedDeltaArgs p, int row_blocks) {
   int first, count;
   gd_range(p.cu, seq, p.tokens, first, count);
   const int row0 = (rb * kGdWarps + wid) * R;
-  if (count == 0 || row0 >= p.dv) return;  // dv is a multiple of 16: a warp's 8 rows are all there or none
+  if (count == 0 || count > most || row0 >= p.dv) return;  // dv is a multiple of 16: a warp's 8 rows are all there or none
   const int hk = h / (p.v_heads / p.k_heads);
   float* S = p.state + (((size_t)slot * p.v_heads + h) * p.dv + row0) * DK + lane * NV;
   float s[R][NV];
@@ -127,22 +131,14 @@ gated_delta_loop_kernel(const GatedDeltaArgs p, int row_blocks) {
 
 namespace {
 
-int launch_loop(const GatedDeltaArgs& p, int dk, int dtype, cudaStream_t s) {
+int launch_loop(const GatedDeltaArgs& p, int dk, int dtype, int most, cudaStream_t s) {
   const int rows = kGdWarps * 8, row_blocks = (p.dv + rows - 1) / rows;
   const long long blocks = (long long)p.n_seq * p.v_heads * row_blocks;
   if (blocks > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
-  const dim3 grid((unsigned)blocks), block(kGdWarps * 32);
-  if (dtype == DFSSM_F16) {
-    if (dk == 128)
-      gated_delta_loop_kernel<__half, 128, 8><<<grid, block, 0, s>>>(p, row_blocks);
-    else
-      gated_delta_loop_kernel<__half, 64, 8><<<grid, block, 0, s>>>(p, row_blocks);
-  } else {
-    if (dk == 128)
-      gated_delta_loop_kernel<__nv_bfloat16, 128, 8><<<grid, block, 0, s>>>(p, row_blocks);
-    else
-      gated_delta_loop_kernel<__nv_bfloat16, 64, 8><<<grid, block, 0, s>>>(p, row_blocks);
-  }
+  const auto fn = dtype == DFSSM_F16 ? (dk == 128 ? gated_delta_loop_kernel<__half, 128, 8> : gated_delta_loop_kernel<__half, 64, 8>)
+                                     : (dk == 128 ? gated_delta_loop_kernel<__nv_bfloat16, 128, 8>
+                                                  : gated_delta_loop_kernel<__nv_bfloat16, 64, 8>);
+  fn<<<(unsigned)blocks, kGdWarps * 32, 0, s>>>(p, row_blocks, most);
   DFSSM_CU(cudaGetLastError());
   return DFSSM_OK;
 }
@@ -154,13 +150,13 @@ size_t gd_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int
 
 template <typename T, int DK, bool DEEP>
 int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16, const int4* order, int slots_total,
-                cudaStream_t s) {
+                int walkers, int least, cudaStream_t s) {
   static SmemLimit limit;
   constexpr int bytes = gd_chunk_smem<DK, DEEP>();
   const auto fn = gated_delta_chunk_kernel<T, DK, DEEP>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
   const int parts = (p.dv + 16 * kGdGroups - 1) / (16 * kGdGroups);
-  const long long grid = (long long)p.n_seq * p.v_heads * parts;
+  const long long grid = (long long)walkers * p.v_heads * parts;
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d sequences x %d heads are too many", p.n_seq, p.v_heads);
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -172,12 +168,13 @@ int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16,
   cfg.stream = s;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  DFSSM_CU(cudaLaunchKernelEx(&cfg, fn, p, blocks, kq16, order, parts, slots_total));
+  DFSSM_CU(cudaLaunchKernelEx(&cfg, fn, p, blocks, kq16, order, parts, slots_total, least));
   return DFSSM_OK;
 }
 
+// Sequences of at least `least` tokens by the chunked kernels (1: all that have any).
 template <typename T, int DK>
-int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
+int launch_chunked(const GatedDeltaArgs& p, char* workspace, int least, cudaStream_t s) {
   static SmemLimit limit;
   constexpr int bytes = gd_prep_smem<DK>();
   const long long n = gd_chunk_slots(p.tokens, p.n_seq);
@@ -194,20 +191,21 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, cudaStream_t s) {
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
-  const bool at_once = (long long)p.n_seq * p.v_heads * ((p.dv + 31) / 32) <= sms;  // every block of the walk has an SM
+  // No more sequences than this can be so long; in order of falling length they come first.
+  const int walkers = least > 1 && p.tokens / least < p.n_seq ? p.tokens / least : p.n_seq;
+  const bool at_once = (long long)walkers * p.v_heads * ((p.dv + 31) / 32) <= sms;  // every block of the walk has an SM
   // The sequences by falling length (a long one that starts last runs alone), with their slots looked up.  It costs
   // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself, as
   // it does where all start at once.
-  int4* order = !at_once && p.n_seq <= 512 ? reinterpret_cast<int4*>(workspace + gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK,
-                                                                                 std::is_same<T, __half>::value ? DFSSM_F16 : DFSSM_BF16) -
-                                                         (size_t)p.n_seq * 16)
-                               : nullptr;
+  const bool ordered = walkers < p.n_seq || (!at_once && p.n_seq <= kGdOrdered);
+  const size_t all = gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK, std::is_same<T, __half>::value ? DFSSM_F16 : DFSSM_BF16);
+  int4* order = ordered ? reinterpret_cast<int4*>(workspace + all - (size_t)p.n_seq * 16) : nullptr;
   const auto fn = gated_delta_prep_kernel<T, DK>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group);
+  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group, least);
   DFSSM_CU(cudaGetLastError());
-  return at_once ? launch_walk<T, DK, true>(p, workspace, kq16, order, (int)n, s)
-                 : launch_walk<T, DK, false>(p, workspace, kq16, order, (int)n, s);
+  return at_once ? launch_walk<T, DK, true>(p, workspace, kq16, order, (int)n, walkers, least, s)
+                 : launch_walk<T, DK, false>(p, workspace, kq16, order, (int)n, walkers, least, s);
 }
 
 // What both entry points ask of their arguments.
@@ -250,7 +248,7 @@ int dfssm_gated_delta_step(const void* q, int ld_q, const void* k, int ld_k, con
                          state, n_slots, slots, nullptr, batch, batch, o, k_heads, v_heads, dv, scale, qk_norm};
   if (const int rc = check_args(p, dk, dtype)) return rc;
   if (batch == 0) return DFSSM_OK;
-  return launch_loop(p, dk, dtype, static_cast<cudaStream_t>(stream));
+  return launch_loop(p, dk, dtype, 1, static_cast<cudaStream_t>(stream));
 }
 
 size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dv, int dtype) {
@@ -273,14 +271,21 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
     return dfssm_fail(DFSSM_ERR_ARG, "the workspace must be %zu bytes, 256-byte aligned", need);
   if (n_seq == 0 || tokens == 0) return DFSSM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // The token loop for sequences of few tokens: it takes about 1 us a token of the longest one, the chunked kernels 16 us
-  // and more whatever the length up to 64 (64 heads, one sequence of 12 / 16 tokens: 14.7 / 18.5 us against 16;
-  // 64 sequences of 4 / 16: 83 / 256 us against 240).  The lengths are not known here, so the average decides,
-  // well below the crossover, since one of the sequences may hold most of the tokens.
-  if (tokens <= 15 || tokens <= 4LL * n_seq) return launch_loop(p, dk, dtype, s);
+  // The token loop for sequences of few tokens: it takes about 1.1 us a token of the longest one, the chunked kernels
+  // 15 us and more whatever the length up to 64 (64 heads of 64 x 128, one sequence of 12 / 16 tokens: 14.5 / 18.5 us
+  // against 15.1; 64 sequences of 8: 150 us for both launched as below, 241 by chunks).  The lengths are not known here:
+  // where they average less than kGdMixed tokens, both run, each for its sequences (200 sequences of 1 token and 4 of
+  // 500: 297 us, 818 by chunks alone; 255 of 1 and one of 700: 286, by the loop alone 1012; where one of them finds
+  // nothing to do it costs 2 to 12%).  With more sequences than are put in order, the average decides for all of them.
   char* w = static_cast<char*>(workspace);
-  if (dtype == DFSSM_F16) return dk == 128 ? launch_chunked<__half, 128>(p, w, s) : launch_chunked<__half, 64>(p, w, s);
-  return dk == 128 ? launch_chunked<__nv_bfloat16, 128>(p, w, s) : launch_chunked<__nv_bfloat16, 64>(p, w, s);
+  const bool many = n_seq > kGdOrdered, mixed = !many && n_seq > 1 && tokens < (long long)kGdMixed * n_seq;
+  const int least = mixed ? kGdLoopMost + 1 : 1;
+  if (tokens <= kGdLoopMost || (many && tokens <= 4LL * n_seq)) return launch_loop(p, dk, dtype, tokens, s);
+  if (mixed) {
+    if (const int rc = launch_loop(p, dk, dtype, kGdLoopMost, s)) return rc;
+  }
+  if (dtype == DFSSM_F16) return dk == 128 ? launch_chunked<__half, 128>(p, w, least, s) : launch_chunked<__half, 64>(p, w, least, s);
+  return dk == 128 ? launch_chunked<__nv_bfloat16, 128>(p, w, least, s) : launch_chunked<__nv_bfloat16, 64>(p, w, least, s);
 }
 
 }  // extern "C"

@@ -241,10 +241,11 @@ constexpr unsigned long long kFragRow = frag_rows();
 
 // kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.  walks, if not
 // NULL: [n_seq], for the chunk kernel: {first token, tokens, slot or -1, number} of the sequences by falling length.
+// Sequences of fewer than `least` tokens are not these kernels'.
 template <typename T, int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4)
 gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __half* __restrict__ kq16,
-                        int4* __restrict__ walks, int groups, int per_group) {
+                        int4* __restrict__ walks, int groups, int per_group, int least) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int UPR = DK / 8;  // 16-byte units per row
   extern __shared__ __align__(128) char smem[];
@@ -290,7 +291,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   int first, count;
   gd_range(p.cu, lo, p.tokens, first, count);
   const int cn = num - gd_chunk_base(p.cu, lo, p.tokens);
-  if (cn < 0 || cn * kGdC >= count) return;
+  if (cn < 0 || cn * kGdC >= count || count < least) return;
   first += cn * kGdC;
   count = min(count - cn * kGdC, kGdC);
   // K and Q rows as they are, then a thread per row (64 of K, 64 of Q) for its norm and, for bf16, its fp16 form
@@ -683,7 +684,7 @@ __device__ __forceinline__ float pair_max(unsigned a, unsigned b, __nv_bfloat16)
 template <typename T, int DK, bool DEEP>
 __global__ void __launch_bounds__(128 * kGdGroups, DEEP ? 1 : 2)
 gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
-                         const int4* __restrict__ walks, int parts, int slots_total) {
+                         const int4* __restrict__ walks, int parts, int slots_total, int least) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int NT = 128 * kGdGroups, NL = NT / 2, UPR = DK / 8;
   constexpr int NH = DK / 16, KH = DK / 32;  // n-tiles and k-steps of a chain warp's half of dk
@@ -703,7 +704,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     gd_range(p.cu, seq, p.tokens, first, count);
     slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
   }
-  if (slot < 0 || count == 0) {
+  if (slot < 0 || count < least) {
     prep_done();  // no block ends before the kernel ahead has
     return;
   }

@@ -261,3 +261,31 @@ def test_lists_of_every_length(ops, B, V, shape):
             want = sample_row(logits[r], u[r], 1.0, int(k[r]), 1.0 if top_p is None else top_p, min_p or 0.0)
             assert (t[r].item(), kept[r].item()) == want[:2], (r, k[r], top_p, min_p, t[r].item(), kept[r].item(), want)
             assert abs(prob[r].item() - want[2]) <= 2.0 ** -24 * want[2] + 1e-12
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(2, 4, 128, 128), (1, 3, 64, 48)])
+def test_decode_rows_and_prompts_in_one_call(ops, heads, dtype):
+    """One-token rows, short and long prompts, empty ones and padding together: the kernels share them by length."""
+    rng = np.random.default_rng(heads[3])
+    lens = np.array([1] * 40 + [12] * 9 + [13] * 7 + [300, 65, 64, 2] + [0] * 3)
+    rng.shuffle(lens)
+    n_seq, n = len(lens), int(lens.sum())
+    x = make(heads, n + 5, n_seq + 2, dtype, 31)
+    slots = rng.permutation(n_seq + 2)[:n_seq].astype(np.int32)
+    lost = [int(np.flatnonzero(lens == m)[-1]) for m in (1, 13)]
+    slots[lost[0]], slots[lost[1]] = -1, slots[int(np.flatnonzero(lens == 12)[0])]
+    lost = [i for i in range(n_seq) if slots[i] < 0 or slots[i] in slots[:i]]
+    before, out = x["state"].clone(), torch.full_like(x["v"], 7.0)
+    ops.gated_delta_prefill(*args(x), cu(lens), slots=torch.from_numpy(slots).cuda(), out=out, scale=0.2)
+    rows = np.concatenate([[0], np.cumsum(lens)])
+    assert (out[n:] == 7).all() and all((out[rows[i]:rows[i + 1]] == 7).all() for i in lost)
+    part = [i for i in range(n_seq) if i not in lost]
+    own = torch.from_numpy(slots[part].astype(np.int64)).cuda()
+    at = torch.from_numpy(np.concatenate([np.arange(rows[i], rows[i + 1]) for i in part])).cuda()
+    y = {m: t[at] if m in "qkvab" else t for m, t in x.items()}
+    ref = reference(y, lens[part], before[own].cpu().numpy(), 0.2, True)
+    check(out[at], x["state"][own], ref, lens[part], dtype)
+    others = torch.ones(n_seq + 2, dtype=torch.bool, device="cuda")
+    others[own] = False
+    assert torch.equal(x["state"][others], before[others])
