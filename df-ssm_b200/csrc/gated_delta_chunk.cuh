@@ -141,10 +141,13 @@ __host__ __device__ constexpr int gd_prep_tiles() {  // K and Q; once they are m
 template <int DK>
 __host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 9 + 64; }
 
-// Three TF32 MMAs for a product of fp32 values (22 bits): a, b split here.
+// Three TF32 MMAs for a product of fp32 values: a, b split here.  hi is cut off after 11 bits and lo, exact, rounded to
+// 11 (finite values: adding half of its last place may carry into the exponent, as it should), 2^-23 of the value.
+// By integer instructions: cvt.rna.tf32 runs at a fraction of their rate (64 prompts of 64 tokens, 64 heads:
+// 235 us, 246 with it).
 __device__ __forceinline__ void tf32_split2(float v, unsigned& hi, unsigned& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));
+  hi = __float_as_uint(v) & 0xffffe000u;
+  lo = (__float_as_uint(v - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
 }
 __device__ __forceinline__ void mma_tf32_acc(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
