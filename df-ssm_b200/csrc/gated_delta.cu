@@ -183,7 +183,7 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, int least, cudaStre
   DFSSM_CU(cudaGetDevice(&dev));
   DFSSM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   // Heads of one key per prep block: the more, the less is computed twice, as long as there are blocks for every SM
-  // (64 heads on one key, 64 prompts of 64 tokens, whole call: 265 us with 2, 254 with 4, 247 with 8, 246 with 16).
+  // (64 heads on one key, 64 prompts of 64 tokens, whole call: 253 us with 2, 242 with 4, 235 with 8, 235 with 16).
   int per_group = rep < 8 ? rep : 8;
   while (per_group > 1 && n * p.k_heads * ((rep + per_group - 1) / per_group) < 4 * sms) per_group /= 2;
   const int groups = (rep + per_group - 1) / per_group;
