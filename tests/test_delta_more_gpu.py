@@ -289,3 +289,24 @@ def test_decode_rows_and_prompts_in_one_call(ops, heads, dtype):
     others = torch.ones(n_seq + 2, dtype=torch.bool, device="cuda")
     others[own] = False
     assert torch.equal(x["state"][others], before[others])
+
+
+@pytest.mark.parametrize("B", [300, 1025, 4096, 4097])
+def test_more_rows_than_run_at_once(ops, B):
+    """Batches whose rows are taken in another order than their own, with settings of all kinds."""
+    rng = np.random.default_rng(B)
+    V = 600
+    logits = (rng.standard_normal((B, V)) * 2).astype(np.float32)
+    u = rng.random(B).astype(np.float32)
+    kind = rng.integers(0, 5, B)
+    k = np.where(kind < 2, 0, rng.integers(1, 200, B)).astype(np.int32)
+    p = np.where((kind == 1) | (kind == 2), 1.0, rng.uniform(0.3, 0.99, B)).astype(np.float32)
+    t = np.where(kind == 4, 0.0, rng.uniform(0.5, 1.5, B)).astype(np.float32)
+    dev = lambda x: torch.tensor(x, device="cuda")  # noqa: E731
+    token, kept, prob = ops.sample_filtered(dev(logits), dev(u), temperature=dev(t), top_k=dev(k), top_p=dev(p))
+    token, kept, prob = token.tolist(), kept.tolist(), prob.tolist()
+    for r in rng.permutation(B)[:400]:
+        want = sample_row(logits[r], u[r], t[r], int(k[r]), p[r])
+        assert (token[r], kept[r]) == want[:2], (r, kind[r], token[r], kept[r], want)
+        assert abs(prob[r] - want[2]) <= 2.0 ** -24 * want[2] + 1e-12
+    assert min(token) >= 0 and max(token) < V  # every row was taken
