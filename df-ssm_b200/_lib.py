@@ -6,10 +6,12 @@ no fallback: if the library is missing or fails to load, every entry point raise
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int8, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libdfssm.so")
+PYCALLS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "dfssm_pycalls.so")
 
 DFSSM_OK = 0
 STATUS = {1: "ERR_ARG", 2: "ERR_FORMAT", 3: "ERR_UNSUPPORTED", 4: "ERR_CUDA", 5: "ERR_OOM", 6: "ERR_STATE",
@@ -98,6 +100,30 @@ def load(path: str = None) -> ctypes.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_pycalls = None
+
+
+def pycalls():
+    """The native host path of ops.py (csrc/pycalls.cpp), bound to the entry points of the loaded library.  Raises if
+    it is absent."""
+    global _pycalls
+    if _pycalls is None:
+        import torch
+        lib = load()
+        if not os.path.exists(PYCALLS_PATH):
+            raise RuntimeError(f"{PYCALLS_PATH} is not built; run `python -m dfssm_b200.build`")
+        spec = importlib.util.spec_from_file_location("dfssm_pycalls", PYCALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, "dfssm_" + n), c_void_p).value
+                      for n in ("gated_delta_step", "gated_delta_workspace", "gated_delta_prefill", "sample_filtered")),
+                    torch.Tensor, torch.float16, torch.bfloat16, torch.float32, torch.int32, torch.uint8, torch.empty_like,
+                    # the handle alone: torch.cuda.current_stream() also makes a Stream object, 2 us a call
+                    torch._C._cuda_getCurrentRawStream, torch.cuda.current_device)
+        _pycalls = module
+    return _pycalls
 
 
 def check(rc: int) -> None:

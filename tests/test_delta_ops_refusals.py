@@ -98,3 +98,64 @@ def test_wrappers_check_shapes_types_and_devices():
                   ((lg, u), dict(seen_bits=mk(3, 1, t=torch.int32)))):
         with pytest.raises(ValueError):
             ops.sample_filtered(*a, **kw)
+
+
+def test_wrappers_refuse_what_is_no_tensor():
+    """Wrong kinds of arguments are a ValueError that names one, wherever they stand."""
+    torch = pytest.importorskip("torch")
+    from dfssm_b200 import ops
+    x = [torch.zeros(2, 1, 128, dtype=torch.float16)] * 3 + [torch.zeros(2, 1, dtype=torch.float16)] * 2
+    x += [torch.zeros(1), torch.zeros(1), torch.zeros(2, 1, 128, 128)]
+    for bad in (None, 3, "q", torch.zeros(()), torch.zeros(1, 1, 1, 1, 1)):
+        for at in range(8):
+            with pytest.raises(ValueError):
+                ops.gated_delta_step(*x[:at], bad, *x[at + 1:])
+        with pytest.raises(ValueError):
+            ops.gated_delta_prefill(*x, bad)
+        for kw in (dict(logits=bad, uniform=torch.zeros(2)), dict(logits=torch.zeros(2, 9), uniform=bad),
+                   dict(logits=bad, uniform=torch.zeros(2), top_p=0.9)):
+            with pytest.raises(ValueError):
+                ops.sample_filtered(**kw)
+
+
+@pytest.mark.gpu
+def test_wrappers_leak_nothing_and_name_what_is_wrong():
+    import gc
+    import sys
+    import torch
+    from dfssm_b200 import ops
+    mk = lambda *s, t=torch.float16: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    f32, i32 = torch.float32, torch.int32
+    x = [mk(3, 1, 128), mk(3, 1, 128), mk(3, 2, 64), mk(3, 2), mk(3, 2), mk(2, t=f32), mk(2, t=f32), mk(4, 2, 64, 128, t=f32)]
+    cu, slots = torch.tensor([0, 3], dtype=i32, device="cuda"), torch.tensor([2, 1, 0], dtype=i32, device="cuda")
+    lg, u, p = mk(3, 50, t=f32), mk(3, t=f32), torch.full((3,), 0.9, device="cuda")
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    held = [*x, cu, slots, lg, u, p, ws]
+
+    def calls():
+        out = mk(3, 2, 64)
+        assert ops.gated_delta_step(*x, slots=slots, out=out) is out
+        wide = mk(3, 400)
+        ops.gated_delta_step(wide[:, :128].unflatten(1, (1, 128)), *x[1:], scale=0.5)
+        ops.gated_delta_step(*x[:2], wide[:, 128:256].unflatten(1, (2, 64)), *x[3:])
+        ops.gated_delta_prefill(*x, cu, out=out)
+        ops.gated_delta_prefill(*x, cu, workspace=ws)
+        ops.sample_filtered(lg, u, top_p=p, out=(mk(3, t=i32), mk(3, t=i32), mk(3, t=f32)))
+        ops.sample_filtered(lg, u, temperature=0.7, top_k=5)
+        for fn, a, kw, name in ((ops.gated_delta_step, x, dict(out=mk(3, 2, 32)), "out"), (ops.gated_delta_step, x, dict(slots=cu), "slots"),
+                                (ops.gated_delta_prefill, (*x, slots.long()), {}, "cu_seqlens"),
+                                (ops.gated_delta_prefill, (*x, cu), dict(workspace=ws[:8]), "workspace"),
+                                (ops.gated_delta_step, (*x[:7], mk(4, 2, 64, 64, t=f32)), {}, "state"),
+                                (ops.sample_filtered, (lg, u[:2]), {}, "uniform"), (ops.sample_filtered, (lg.t(), u), {}, "logits"),
+                                (ops.sample_filtered, (lg, u), dict(min_p=slots), "min_p"), (ops.sample_filtered, (lg, u), dict(out=(u, u, u)), "out")):
+            with pytest.raises(ValueError, match=name):
+                fn(*a, **kw)
+
+    calls()
+    gc.collect()
+    torch.cuda.synchronize()
+    before, memory = [sys.getrefcount(t) for t in held], torch.cuda.memory_allocated()
+    for _ in range(20):
+        calls()
+    gc.collect()
+    assert [sys.getrefcount(t) for t in held] == before and torch.cuda.memory_allocated() == memory
