@@ -159,3 +159,34 @@ def test_wrappers_leak_nothing_and_name_what_is_wrong():
         calls()
     gc.collect()
     assert [sys.getrefcount(t) for t in held] == before and torch.cuda.memory_allocated() == memory
+
+
+@pytest.mark.gpu
+def test_tensors_on_another_device_than_the_current_one():
+    """The host path steps aside when another device is current; here it is told so once, with the one device there is."""
+    import torch
+    from dfssm_b200 import ops
+    g = torch.Generator("cuda").manual_seed(3)
+    x = [torch.randn(*s, device="cuda", generator=g).half() for s in ((3, 1, 64), (3, 1, 64), (3, 2, 32), (3, 2), (3, 2))]
+    x += [torch.zeros(2, device="cuda"), torch.zeros(2, device="cuda")]
+    lg, u, cu = torch.randn(3, 99, device="cuda", generator=g), torch.rand(3, device="cuda", generator=g), torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda")
+    calls = (lambda s: ops.gated_delta_step(*x, s), lambda s: ops.gated_delta_prefill(*x, s, cu), lambda s: ops.sample_filtered(lg, u, top_p=0.9)[0])
+    state = lambda: torch.ones(3, 2, 32, 64, device="cuda")  # noqa: E731
+    want = [f(state()) for f in calls]
+    native = _lib.pycalls()
+    at = [getattr(_lib.load(), "dfssm_" + n) for n in ("gated_delta_step", "gated_delta_workspace", "gated_delta_prefill", "sample_filtered")]
+    asked = []
+
+    def current():
+        asked.append(1)
+        return 7 if len(asked) % 2 else torch.cuda.current_device()
+
+    import ctypes
+    try:
+        native.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in at), torch.Tensor, torch.float16, torch.bfloat16, torch.float32, torch.int32,
+                    torch.uint8, torch.empty_like, torch._C._cuda_getCurrentRawStream, current)
+        got = [f(state()) for f in calls]
+    finally:
+        _lib._pycalls = None
+        _lib.pycalls()
+    assert len(asked) == 6 and all(torch.equal(a, b) for a, b in zip(got, want))
