@@ -17,8 +17,9 @@
 // and split in two fp16 numbers hi + lo, which keep 22 bits of what is above 2^-17 of that and 2^-39 of it
 // below; a product of two such pairs takes three MMAs (hi hi, hi lo, lo hi).  The scales of S and P come
 // from their largest elements; those of r and u from bounds known before the products end,
-//   |r| <= max |v| + sqrt(dk) max |S| max |k|,   |u| <= max |r| max_t sum_w |T[t][w]|.  Sums run in fp32 accumulators, and the state's update in one of its own, added to the
-// decayed state with one rounding.  Decays are differences of sums in double precision: in fp32 a sum of
+//   |r| <= max |v| + sqrt(dk) max |S| max |k|,   |u| <= max |r| max_t sum_w |T[t][w]|.
+// Sums run in fp32 accumulators, and the state's update in one of its own, added to the decayed state with one
+// rounding.  Decays are differences of sums in double precision: in fp32 a sum of
 // -100 already leaves e^(G_t - G_w) an error of 4e-6.
 #pragma once
 #include "gated_delta.cuh"

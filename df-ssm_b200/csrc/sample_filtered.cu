@@ -205,7 +205,8 @@ struct Weigh {
   __device__ __forceinline__ u64 of(float x) const { return fix(scaled(x)); }
 };
 
-// Adds a weight to a bin's two words in shared memory (64-bit shared atomics are loops: 74 us instead of 60 for 148 rows of 50,280 with top-p).
+// Adds a weight to a bin's two words in shared memory (64-bit shared atomics are loops: 74 us instead of 60 for 148 rows
+// of 50,280 with top-p).
 __device__ __forceinline__ void add_weight(unsigned* lo, unsigned* hi, u64 w) {
   const unsigned wl = (unsigned)w, old = atomicAdd(lo, wl);
   const unsigned wh = (unsigned)(w >> 32) + (old + wl < old ? 1u : 0u);
