@@ -17,7 +17,10 @@
 // and split in two fp16 numbers hi + lo, which keep 22 bits of what is above 2^-17 of that and 2^-39 of it
 // below; a product of two such pairs takes three MMAs (hi hi, hi lo, lo hi).  The scales of S and P come
 // from their largest elements; those of r and u from bounds known before the products end,
-//   |r| <= max |v| + sqrt(dk) max |S| max |k|,   |u| <= max |r| max_t sum_w |T[t][w]|.
+//   |r| <= max |v| + sqrt(dk) max |S| max |k|,   |u| <= max |r| max_t sum_w |T[t][w]|,
+// and a chunk where what matters lies too far below these bounds is taken token by token instead (kGdRangeO).  So the errors are
+// those of fp32 sums, relative to the largest that a row of the state has or, but for its decays, still has: an element far
+// smaller than others of its row that are not forgotten is held in 39 bits below the row's largest in S k and S q.
 // Sums run in fp32 accumulators, and the state's update in one of its own, added to the decayed state with one
 // rounding.  Decays are differences of sums in double precision: in fp32 a sum of
 // -100 already leaves e^(G_t - G_w) an error of 4e-6.
@@ -31,8 +34,9 @@ constexpr int kGdFrags = 20;            // 8 x 16 fragments of a lower triangula
 constexpr int kGdTri = kGdFrags * 512;  // bytes of one such matrix as fp16 hi/lo pairs, in fragment order
 // Factors of a chunk: per token -e^G / |k|, the update's beta e^(G_C - G) / |k| scaled to at most 1, scale e^G / |q|
 // and the inverse scale of P's row; then e^G_C, the inverse scale of T, the largest absolute row sum of T, the
-// update's scale, and the largest norm of a key.
-enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdLast = 256, kGdTdn, kGdTsum, kGdCdn, kGdKn, kGdVecs };
+// update's scale, the largest norm of a key, and the largest weight of a token's u in the update: the largest
+// beta e^(G_C - G) / |k| times the largest norm of a key as it is staged.
+enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdLast = 256, kGdTdn, kGdTsum, kGdCdn, kGdKn, kGdWm, kGdVecs };
 constexpr int kGdBlock = 2 * kGdTri + 1152;  // bytes per chunk and value head: T, P, factors
 static_assert(kGdVecs * 4 <= 1152 && kGdBlock % 128 == 0, "");
 
@@ -265,7 +269,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   float* colf = rowf + 64;  // [3][64]: e^(boundary before block 1, 2, 3 - G_w) rk_w beta_w
   float* rowd = colf + 192;  // e^(G_t - last of t's block), where that is at most e^kMild
   float* cold = rowd + 64;   // e^(last of w's block - G_w) rk_w beta_w
-  float* red = cold + 64;    // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors
+  float* red = cold + 64;    // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors, [2] norms as staged
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   let_walk_start();
   const int rep = p.v_heads / p.k_heads;
@@ -313,7 +317,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   {
     const int t = tid & 63;
     char* rowp = smem + (tid < 64 ? 0 : kGdC * DK * 2);
-    float ss = 0.f, s1 = 0.f, mx = 0.f;
+    float ss = 0.f, s1 = 0.f, mx = 0.f, staged;
 #pragma unroll 4
     for (int u = 0; u < UPR; ++u) {
       const uint4 raw = *reinterpret_cast<const uint4*>(rowp + kq_off<DK>(t, u));
@@ -329,10 +333,13 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
     ss += s1;
     float factor = p.qk_norm ? 1.0f / sqrtf(ss + kQkEps) : 1.0f;
     float kn = p.qk_norm ? 1.0f : sqrtf(ss);  // the norm that the products see
+    staged = sqrtf(ss);                       // and that of the row in shared memory
     if constexpr (BF) {
       float up, down;
       row_scale(mx, up, down);
       factor *= down;
+      // within what the largest element allows: the sum of squares may have over- or underflowed
+      staged = fminf(fmaxf(staged * up, mx * up), (DK == 128 ? 11.3137085f : 8.f) * (mx * up));
 #pragma unroll 4
       for (int u = 0; u < UPR; ++u) {
         uint4* at = reinterpret_cast<uint4*>(rowp + kq_off<DK>(t, u));
@@ -347,7 +354,8 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
     if (tid < 64) {
       rk[t] = factor;
       kn = warp_max(kn);
-      if (lane == 0) red[8 + wid] = kn;
+      staged = warp_max(staged);
+      if (lane == 0) red[8 + wid] = kn, red[12 + wid] = staged;
     } else {
       rq[t] = factor;
     }
@@ -434,9 +442,10 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
       __syncthreads();
       if (tid < 64) {
         float up, down;
-        row_scale(fmaxf(red[10], red[11]), up, down);
+        const float c2max = fmaxf(red[10], red[11]);
+        row_scale(c2max, up, down);
         vec[kGdC2 + t] = colf[128 + t] * (up * 0x1p-14f);
-        if (t == 0) vec[kGdCdn] = down * 0x1p14f;
+        if (t == 0) vec[kGdCdn] = down * 0x1p14f, vec[kGdWm] = c2max * fmaxf(red[12], red[13]);
         if (t < 48) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
       }
     }
@@ -614,6 +623,21 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 
 constexpr int kGdGroups = 2;  // of 16 rows per block
 
+// Where a chunk's values lie far apart, its pairs are not enough: what is 2^-38 of the row's bound or less is lost in r and
+// u, and it may be all that matters, where a gate has forgotten the large values (of the chunk, or of the state before it)
+// or where they come later.  Such a chunk is taken token by token in fp32 by the group's chain warps (gd_by_token).
+// With U the bound of |u|, a row is safe where
+//   - at every token, |v| or what the row holds (the state's largest element and the beta |v| so far, each decayed
+//     since) is 2^-22 U or more: u and its part in o are then off by some 2^-17 of that, and
+//   - at the end, the largest beta e^(G_C - G) |v| or of e^G_C S is 2^-17 U times the largest weight or more: what the update adds
+//     is then off by some 2^-21 of it.
+// The output warps find the least |v| and the largest weighed one; the decays between are looked at only where
+// some |v| is below 2^-22 U and e^G_C S is too, which chance does to one chunk in 1000 or fewer.  Looking costs 1 to 4% of a
+// call (64 prompts of 64 tokens, 64 heads: 245 us, 235 without; 32768 tokens: 1.40 ms, 1.38), looking at the decays 2 us, a chunk
+// token by token 40 us, 2 to 4 otherwise.
+constexpr float kGdRangeO = 0x1p-22f, kGdRangeS = 0x1p-17f;
+constexpr int kGdOfV = 80, kGdByToken = 144;  // places among a group's scales
+
 template <int DK>
 __host__ __device__ constexpr int gd_exchange() { return DK / 16 * 1024 + 4096 + 4096 + 2048 + 640; }
 template <int DK, bool DEEP>
@@ -672,22 +696,127 @@ __device__ __forceinline__ void get_frag(const uint4* from, unsigned (&h)[4], un
   h[0] = a.x, h[1] = a.y, h[2] = a.z, h[3] = a.w;
   l[0] = b.x, l[1] = b.y, l[2] = b.z, l[3] = b.w;
 }
-// Largest magnitude of two pairs of 16-bit values.
-__device__ __forceinline__ float pair_max(unsigned a, unsigned b, __half) {
-  const __half2 x = __habs2(*reinterpret_cast<__half2*>(&a)), y = __habs2(*reinterpret_cast<__half2*>(&b));
-  const float2 f = __half22float2(__hmax2(x, y));
-  return fmaxf(f.x, f.y);
+template <typename T>
+struct PairOf;
+template <>
+struct PairOf<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ float2 floats(__half2 x) { return __half22float2(x); }
+  static __device__ __forceinline__ __half2 round(float2 x) { return __float22half2_rn(x); }
+};
+template <>
+struct PairOf<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ float2 floats(__nv_bfloat162 x) { return __bfloat1622float2(x); }
+  static __device__ __forceinline__ __nv_bfloat162 round(float2 x) { return __float22bfloat162_rn(x); }
+};
+template <typename T>
+__device__ __forceinline__ typename PairOf<T>::type as_pair(unsigned u) { return *reinterpret_cast<typename PairOf<T>::type*>(&u); }
+template <typename P>
+__device__ __forceinline__ unsigned pair_bits(P x) { return *reinterpret_cast<unsigned*>(&x); }
+
+// Whether one of a group's rows comes to a token where it holds less than w0 (rows g; w1: rows g + 8), and something.  m0, m1: the
+// largest of the rows' state; v: the chunk's tile.
+template <typename T>
+__device__ __forceinline__ bool gd_forgets(const GatedDeltaArgs& p, const char* v, int group, int first, int n, int h, float m0,
+                                           float m1, float w0, float w1) {
+  const int lane = threadIdx.x & 31, g = lane >> 2;
+  bool bad = false;
+#pragma unroll 1
+  for (int t0 = 0; t0 < n; t0 += 32) {
+    const size_t at = (size_t)first + min(t0 + lane, n - 1);  // the gates of 32 tokens, one per lane
+    float keep = expf(gd_log_decay(to_f(static_cast<const T*>(p.a)[at * p.ld_a + h]), p.dt_bias[h], p.A_log[h]));
+    float beta = gd_beta(to_f(static_cast<const T*>(p.b)[at * p.ld_b + h]));
+    if (t0 + lane >= n) keep = 1.f, beta = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < 32; ++i) {
+      const float e = __shfl_sync(0xffffffffu, keep, i), b = __shfl_sync(0xffffffffu, beta, i);
+      const float x = fabsf(to_f(reinterpret_cast<const T*>(v + v_off(t0 + i, 2 * group))[g]));  // 0 behind the last token
+      const float y = fabsf(to_f(reinterpret_cast<const T*>(v + v_off(t0 + i, 2 * group + 1))[g]));
+      m0 = fmaxf(e * m0, b * x), m1 = fmaxf(e * m1, b * y);
+      const float x0 = fmaxf(m0, x), x1 = fmaxf(m1, y);
+      bad |= (x0 < w0 && x0 != 0.f) || (x1 < w1 && x1 != 0.f);
+    }
+  }
+  return __any_sync(0xffffffffu, bad);
 }
-__device__ __forceinline__ float pair_max(unsigned a, unsigned b, __nv_bfloat16) {
-  const __nv_bfloat162 x = __habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), y = __habs2(*reinterpret_cast<__nv_bfloat162*>(&b));
-  const float2 f = __bfloat1622float2(__hmax2(x, y));
-  return fmaxf(f.x, f.y);
+
+// The n tokens of a chunk one after the other, from the call's own arrays, for chunks whose values lie too far apart for
+// pairs.  s: the state as the chain warps hold it, s[j] the rows `row` and row + 8, columns half * DK / 2 + 8 j + 2 (lane % 4) +
+// {0, 1}; the rows' sums pass between the two warps through ex.
+template <typename T, int DK>
+__device__ __noinline__ void gd_by_token(const GatedDeltaArgs& p, float (&s)[DK / 16][4], int first, int n, int h, int hk, int row,
+                                         int half, int bar, float4* ex) {
+  constexpr int NH = DK / 16;
+  using T2 = typename PairOf<T>::type;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const float A_log = p.A_log[h], dt_bias = p.dt_bias[h];
+  auto quad_sum = [](float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+  };
+#pragma unroll 1
+  for (int t = 0; t < n; ++t) {
+    const size_t at = (size_t)first + t;
+    const T* kp = static_cast<const T*>(p.k) + at * p.ld_k + hk * DK + 2 * c;
+    const T* qp = static_cast<const T*>(p.q) + at * p.ld_q + hk * DK + 2 * c;
+    const T* vp = static_cast<const T*>(p.v) + at * p.ld_v + h * p.dv + row;
+    const float v0 = to_f(vp[0]), v1 = to_f(vp[8]);
+    const float eg = expf(gd_log_decay(to_f(static_cast<const T*>(p.a)[at * p.ld_a + h]), dt_bias, A_log));
+    const float beta = gd_beta(to_f(static_cast<const T*>(p.b)[at * p.ld_b + h]));
+    float k[NH][2], q[NH][2], kk = 0.f, qq = 0.f, kq = 0.f;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {  // the other warp's columns first, for the norms alone
+#pragma unroll
+      for (int j = 0; j < NH; ++j) {
+        const int col = (part ? half : 1 - half) * (DK / 2) + 8 * j;
+        const T2 x = *reinterpret_cast<const T2*>(kp + col), y = *reinterpret_cast<const T2*>(qp + col);
+        k[j][0] = to_f(x.x), k[j][1] = to_f(x.y), q[j][0] = to_f(y.x), q[j][1] = to_f(y.y);
+        kk = fmaf(k[j][0], k[j][0], fmaf(k[j][1], k[j][1], kk));
+        qq = fmaf(q[j][0], q[j][0], fmaf(q[j][1], q[j][1], qq));
+        kq = fmaf(k[j][0], q[j][0], fmaf(k[j][1], q[j][1], kq));
+      }
+    }
+    kq = quad_sum(kq);
+    if (p.qk_norm) {
+      const float rk = 1.0f / sqrtf(quad_sum(kk) + kQkEps), rq = 1.0f / sqrtf(quad_sum(qq) + kQkEps);
+#pragma unroll
+      for (int j = 0; j < NH; ++j) k[j][0] *= rk, k[j][1] *= rk, q[j][0] *= rq, q[j][1] *= rq;
+      kq *= rk * rq;
+    }
+    float4 sums = make_float4(0.f, 0.f, 0.f, 0.f);  // S k of the two rows, S q
+#pragma unroll
+    for (int j = 0; j < NH; ++j) {
+      sums.x = fmaf(s[j][0], k[j][0], fmaf(s[j][1], k[j][1], sums.x));
+      sums.y = fmaf(s[j][2], k[j][0], fmaf(s[j][3], k[j][1], sums.y));
+      sums.z = fmaf(s[j][0], q[j][0], fmaf(s[j][1], q[j][1], sums.z));
+      sums.w = fmaf(s[j][2], q[j][0], fmaf(s[j][3], q[j][1], sums.w));
+    }
+    sums = make_float4(quad_sum(sums.x), quad_sum(sums.y), quad_sum(sums.z), quad_sum(sums.w));
+    float4* const mail = ex + 16 * (t & 1);  // two, in turn: the other warp has read the one before the last
+    if (c == 0) mail[8 * half + g] = sums;
+    bar_sync(bar, 64);
+    const float4 other = mail[8 * (1 - half) + g];
+    const float u0 = beta * (v0 - eg * (sums.x + other.x)), u1 = beta * (v1 - eg * (sums.y + other.y));
+    if (half == 0 && c == 0) {
+      T* op = static_cast<T*>(p.o) + at * p.ld_o + h * p.dv + row;
+      op[0] = from_f<T>(p.scale * fmaf(kq, u0, eg * (sums.z + other.z)));
+      op[8] = from_f<T>(p.scale * fmaf(kq, u1, eg * (sums.w + other.w)));
+    }
+#pragma unroll
+    for (int j = 0; j < NH; ++j) {
+      s[j][0] = fmaf(u0, k[j][0], eg * s[j][0]);
+      s[j][1] = fmaf(u0, k[j][1], eg * s[j][1]);
+      s[j][2] = fmaf(u1, k[j][0], eg * s[j][2]);
+      s[j][3] = fmaf(u1, k[j][1], eg * s[j][3]);
+    }
+  }
 }
 
 // kq16: the fp16 tiles of K and Q for bf16 inputs; for fp16 inputs the tiles are rows of k and q themselves.
 template <typename T, int DK, bool DEEP>
 __global__ void __launch_bounds__(128 * kGdGroups, DEEP ? 1 : 2)
-gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
+gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* __restrict__ blocks, const __half* __restrict__ kq16,
                          const int4* __restrict__ walks, int parts, int slots_total, int least) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int NT = 128 * kGdGroups, NL = NT / 2, UPR = DK / 8;
@@ -726,7 +855,9 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
   uint4* u_ex = s_ex + DK / 16 * 64;                     // u: [4][hi, lo][32]
   uint4* d_ex = u_ex + 4 * 64;                           // weighed u, the same; before it, partial S k [A, B][4][32]
   uint4* r_ex = d_ex + 4 * 64;                           // A's r: [2][hi, lo][32]
-  float* sc = reinterpret_cast<float*>(r_ex - lane + 2 * 64);  // [16] each: scale of S (A, B), max of S (A, B), scale of u, max |v| (2)
+  // [16] each: scale of S (A, B), max of S (A, B), scale of u; of v [2][8][4]: the largest, the least and the largest weighed
+  // magnitudes of rows g and g + 8, as pairs, over either half of the tokens; whether the chunk goes token by token
+  float* sc = reinterpret_cast<float*>(r_ex - lane + 2 * 64);
   const int bar = 2 + 5 * group;
   // lane parts of the ldmatrix addresses
   const int bt = ((lane >> 4) << 3) + (lane & 7), bu = (lane >> 3) & 1;  // B from [token][dk] rows, two n-tiles
@@ -781,20 +912,43 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       constexpr int REST = kGdBlock / 16 % NL;
       if (lt < REST) cp16(dst + kGdBlock / 16 / NL * NL * 16, blk + kGdBlock / 16 / NL * NL * 16, true);
     };
-    // the largest |v| of each row over this half of chunk ch, for the chain's bound of r
-    auto largest_v = [&](int ch) {
-      const uint32_t v_s = sm0 + (DEEP ? (ch & 1) * STAGE : 0) + V_AT;
-      float v0 = 0.f, v1 = 0.f;
+    // |v| of each row over this half of chunk ch, for the chain's bound of r and for what it asks of the chunk
+    auto sizes_of_v = [&](int ch) {
+      const char* stage = smem + (DEEP ? (ch & 1) * STAGE : 0);
+      const float* factors = reinterpret_cast<const float*>(stage + B_AT + 2 * kGdTri) + kGdC2 + 32 * half + 2 * c;
+      const int n = count - ch * kGdC - 32 * half - 2 * c;
+      using P = PairOf<T>;
+      typename P::type most[2], least[2], weighed[2];  // of rows g, g + 8
+      most[0] = most[1] = weighed[0] = weighed[1] = as_pair<T>(0u);
+      least[0] = least[1] = as_pair<T>(0x7fff7fffu);  // no number: the others stay
 #pragma unroll
       for (int jp = 0; jp < 2; ++jp) {
-        unsigned v[4];
-        ldsm4t(v, v_s + v_off(32 * half + 16 * jp + tt, 2 * group + tu));
-        v0 = fmaxf(v0, pair_max(v[0], v[1], T()));
-        v1 = fmaxf(v1, pair_max(v[2], v[3], T()));
+        unsigned v[4];  // {t, rows 0-7}, {t + 8, ..}, {t, rows 8-15}, {t + 8, ..}
+        ldsm4t(v, smem_u32(stage) + V_AT + v_off(32 * half + 16 * jp + tt, 2 * group + tu));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = 16 * jp + 8 * i;
+          const typename P::type f = P::round(*reinterpret_cast<const float2*>(factors + t));
+          const unsigned behind = (t < n ? 0u : 0x7fffu) | (t + 1 < n ? 0u : 0x7fff0000u);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const typename P::type x = __habs2(as_pair<T>(v[2 * r + i]));
+            most[r] = __hmax2(most[r], x);
+            least[r] = __hmin2(least[r], as_pair<T>(pair_bits(x) | behind));
+            weighed[r] = __hmax2(weighed[r], __habs2(__hmul2(x, f)));
+          }
+        }
       }
-      v0 = quad_max(v0);
-      v1 = quad_max(v1);
-      if (c == 0) sc[80 + 16 * half + g] = v0, sc[88 + 16 * half + g] = v1;
+      auto across = [&](typename P::type (&x)[2], auto op) {  // rows g and g + 8 of a pair, over the quad
+        unsigned w = pair_bits(op(as_pair<T>(__byte_perm(pair_bits(x[0]), pair_bits(x[1]), 0x5410)),
+                                  as_pair<T>(__byte_perm(pair_bits(x[0]), pair_bits(x[1]), 0x7632))));
+        w = pair_bits(op(as_pair<T>(w), as_pair<T>(__shfl_xor_sync(0xffffffffu, w, 1))));
+        return pair_bits(op(as_pair<T>(w), as_pair<T>(__shfl_xor_sync(0xffffffffu, w, 2))));
+      };
+      auto larger = [](typename P::type x, typename P::type y) { return __hmax2(x, y); };
+      auto smaller = [](typename P::type x, typename P::type y) { return __hmin2(x, y); };
+      const uint4 all = make_uint4(across(most, larger), across(least, smaller), across(weighed, larger), 0u);
+      if (c == 0) reinterpret_cast<uint4*>(sc + kGdOfV)[8 * half + g] = all;
     };
     if (BF) prep_done();
     load_k(0);
@@ -806,7 +960,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     if constexpr (DEEP) {
       cp_wait<0>();
       bar_sync(1, NL);
-      largest_v(0);
+      sizes_of_v(0);
       bar_arrive(0, NT);  // the chunk is there
     }
     for (int ch = 0; ch < chunks; ++ch) {
@@ -826,7 +980,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         cp_commit();
         cp_wait<1>();
         bar_sync(1, NL);  // V, T, P and the factors are there
-        largest_v(ch);
+        sizes_of_v(ch);
         bar_sync(0, NT);  // they are for the chains too, which have split S
       }
       float o[4][4] = {}, o2[4][4] = {};  // the two halves of dk have scales of their own
@@ -863,11 +1017,12 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
       for (int kk = 0; kk < 4; ++kk)
         if (kk < 2 || half) get_frag(u_ex + kk * 64, ah[kk], al[kk]);
       const float du0 = sc[64 + g], du1 = sc[72 + g];
+      const bool by_token = sc[kGdByToken] != 0.f;  // the chain warps write these rows of o
       if (more) bar_arrive(bar + 4, 128);
       if (DEEP && more) {
         cp_wait<0>();
         bar_sync(1, NL);
-        largest_v(ch + 1);
+        sizes_of_v(ch + 1);
         bar_arrive(0, NT);  // the next chunk is there
       }
       const uint4* Pf = reinterpret_cast<const uint4*>(st + B_AT + kGdTri) + lane;
@@ -893,7 +1048,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
         stsm4t(v_s + v_off(32 * half + 16 * jp + tt, 2 * group + tu), out);
       }
       __syncwarp();
-      if (active) {  // 16 rows of 32 bytes per store
+      if (active && !by_token) {  // 16 rows of 32 bytes per store
         T* og = static_cast<T*>(p.o) + ((size_t)first + (size_t)ch * kGdC) * p.ld_o + h * p.dv + row0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -977,13 +1132,46 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
     // bounds of r and u, and the scales from them (measured: slower before or among the MMAs above)
     float ur0, dr0, ur1, dr1, uu0, du0, uu1, du1;
     const float root = (DK == 128 ? 11.3137085f : 8.f) * vec[kGdKn];
-    const float r0 = fmaf(root, fmaxf(sc[32 + g], sc[48 + g]), fmaxf(sc[80 + g], sc[96 + g]));
-    const float r1 = fmaf(root, fmaxf(sc[40 + g], sc[56 + g]), fmaxf(sc[88 + g], sc[104 + g]));
+    const float s0 = fmaxf(sc[32 + g], sc[48 + g]), s1 = fmaxf(sc[40 + g], sc[56 + g]);
+    const uint4 va = reinterpret_cast<const uint4*>(sc + kGdOfV)[g], vb = reinterpret_cast<const uint4*>(sc + kGdOfV)[8 + g];
+    const float2 most = PairOf<T>::floats(__hmax2(as_pair<T>(va.x), as_pair<T>(vb.x)));
+    const float r0 = fmaf(root, s0, most.x), r1 = fmaf(root, s1, most.y);
+    const float u0 = r0 * vec[kGdTsum], u1 = r1 * vec[kGdTsum];
     row_scale(r0, ur0, dr0);
     row_scale(r1, ur1, dr1);
-    row_scale(r0 * vec[kGdTsum], uu0, du0);
-    row_scale(r1 * vec[kGdTsum], uu1, du1);
+    row_scale(u0, uu0, du0);
+    row_scale(u1, uu1, du1);
     const float tdn = vec[kGdTdn], el = vec[kGdLast], cdn = vec[kGdCdn];
+    {  // both warps come to the same answers: they look at the same numbers
+      const float2 least = PairOf<T>::floats(__hmin2(as_pair<T>(va.y), as_pair<T>(vb.y)));
+      const float2 weighed = PairOf<T>::floats(__hmax2(as_pair<T>(va.z), as_pair<T>(vb.z)));
+      const float k0 = el * s0, k1 = el * s1, w0 = u0 * kGdRangeO, w1 = u1 * kGdRangeO, wm = vec[kGdWm] * kGdRangeS;
+      const bool weak = (weighed.x < u0 * kGdRangeS && k0 < u0 * wm) || (weighed.y < u1 * kGdRangeS && k1 < u1 * wm);
+      const bool low = (least.x < w0 && k0 < w0) || (least.y < w1 && k1 < w1);
+      bool far = __any_sync(0xffffffffu, weak);
+      if (!far && __any_sync(0xffffffffu, low))
+        far = gd_forgets<T>(p, st + V_AT, group, first + ch * kGdC, min(count - ch * kGdC, kGdC), h, s0, s1, w0, w1);
+      if (far && active) {
+        if (half == 0 && lane == 0) sc[kGdByToken] = 1.f;
+        bar_arrive(bar + 3, 128);  // the output warps need not wait: they leave this chunk's o alone
+        float copy[NH][4];         // the state itself stays in registers
+#pragma unroll
+        for (int j = 0; j < NH; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) copy[j][i] = s[j][i];
+        gd_by_token<T, DK>(p, copy, first + ch * kGdC, min(count - ch * kGdC, kGdC), h, hk, row0 + g, half, bar,
+                           reinterpret_cast<float4*>(d_ex - lane));
+        m0 = m1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[j][i] = copy[j][i];
+          m0 = fmaxf(m0, fmaxf(fabsf(s[j][0]), fabsf(s[j][1])));
+          m1 = fmaxf(m1, fmaxf(fabsf(s[j][2]), fabsf(s[j][3])));
+        }
+        continue;
+      }
+    }
     // r = v - e^G (S k) of this warp's tokens, split as the left operand of u = r T^T
     unsigned ah[4][4], al[4][4];
 #pragma unroll
@@ -1057,7 +1245,7 @@ gated_delta_chunk_kernel(const GatedDeltaArgs p, const char* __restrict__ blocks
           split_tile(x[2 * kk], x[2 * kk + 1], fu0, fu1, uh, ul);
           put_frag(u_ex + (2 * half + kk) * 64, uh, ul);
           if (kk == 1) {
-            if (half == 0 && c == 0) sc[64 + g] = du0, sc[72 + g] = du1;
+            if (half == 0 && c == 0) sc[64 + g] = du0, sc[72 + g] = du1, sc[kGdByToken] = 0.f;
             bar_arrive(bar + 3, 128);  // u is split; this warp reads V, T and the factors no more
           }
         }
