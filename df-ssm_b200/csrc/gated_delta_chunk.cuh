@@ -34,11 +34,14 @@ constexpr int kGdFrags = 20;            // 8 x 16 fragments of a lower triangula
 constexpr int kGdTri = kGdFrags * 512;  // bytes of one such matrix as fp16 hi/lo pairs, in fragment order
 // Factors of a chunk: per token -e^G / |k|, the update's beta e^(G_C - G) / |k| scaled to at most 1, scale e^G / |q|
 // and the inverse scale of P's row; then e^G_C, the inverse scale of T, the largest absolute row sum of T, the
-// update's scale, the largest norm of a key, and the largest weight of a token's u in the update: the largest
-// beta e^(G_C - G) / |k| times the largest norm of a key as it is staged.
-enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdLast = 256, kGdTdn, kGdTsum, kGdCdn, kGdKn, kGdWm, kGdVecs };
-constexpr int kGdBlock = 2 * kGdTri + 1152;  // bytes per chunk and value head: T, P, factors
-static_assert(kGdVecs * 4 <= 1152 && kGdBlock % 128 == 0, "");
+// update's scale, the largest norm of a key, and the largest weight a u could have in the update: the largest
+// beta e^(G_C - G) / |k| times the largest norm of a key as it is staged.  Last, in the inputs' type, each token's own weight
+// beta e^(G_C - G) relative to that (to within 1/4: by powers of two).
+enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdLast = 256, kGdTdn, kGdTsum, kGdCdn, kGdKn, kGdWm, kGdWeights = 264,
+       kGdVecs = kGdWeights + 32 };
+constexpr int kGdFactors = 1280;                   // bytes of them
+constexpr int kGdBlock = 2 * kGdTri + kGdFactors;  // bytes per chunk and value head: T, P, factors
+static_assert(kGdVecs * 4 <= kGdFactors && kGdBlock % 128 == 0, "");
 
 // Chunks are numbered without a plan: sequence i's chunk c is cu[i] / 64 + i + c.  That leaves at most one
 // number per sequence unused and gives no number twice.
@@ -144,7 +147,7 @@ __host__ __device__ constexpr int gd_prep_tiles() {  // K and Q; once they are m
   return 2 * kGdC * DK * 2 > kGdC * kLS * 4 ? 2 * kGdC * DK * 2 : kGdC * kLS * 4;
 }
 template <int DK>
-__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 9 + 64; }
+__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 10 + 64; }
 
 // Three TF32 MMAs for a product of fp32 values: a, b split here.  hi is cut off after 11 bits and lo, exact, rounded to
 // 11 (finite values: adding half of its last place may carry into the exponent, as it should), 2^-23 of the value.
@@ -269,7 +272,8 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   float* colf = rowf + 64;  // [3][64]: e^(boundary before block 1, 2, 3 - G_w) rk_w beta_w
   float* rowd = colf + 192;  // e^(G_t - last of t's block), where that is at most e^kMild
   float* cold = rowd + 64;   // e^(last of w's block - G_w) rk_w beta_w
-  float* red = cold + 64;    // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors, [2] norms as staged
+  float* kst = cold + 64;    // norms of K's rows as staged
+  float* red = kst + 64;     // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors, [2] norms as staged
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   let_walk_start();
   const int rep = p.v_heads / p.k_heads;
@@ -352,7 +356,8 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
       }
     }
     if (tid < 64) {
-      rk[t] = factor;
+      rk[t] = staged > 0.f ? factor : 0.f;  // a key of zeros adds nothing: its 1 / |k| is not to set the update's scale
+      kst[t] = staged;
       kn = warp_max(kn);
       staged = warp_max(staged);
       if (lane == 0) red[8 + wid] = kn, red[12 + wid] = staged;
@@ -445,7 +450,11 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
         const float c2max = fmaxf(red[10], red[11]);
         row_scale(c2max, up, down);
         vec[kGdC2 + t] = colf[128 + t] * (up * 0x1p-14f);
-        if (t == 0) vec[kGdCdn] = down * 0x1p14f, vec[kGdWm] = c2max * fmaxf(red[12], red[13]);
+        const float kmax = fmaxf(red[12], red[13]);
+        float kup, kdown;
+        row_scale(kmax, kup, kdown);
+        reinterpret_cast<T*>(vec + kGdWeights)[t] = from_f<T>((colf[128 + t] * (up * 0x1p-14f)) * (kst[t] * (kup * 0x1p-14f)));
+        if (t == 0) vec[kGdCdn] = down * 0x1p14f, vec[kGdWm] = c2max * kmax;
         if (t < 48) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
       }
     }
@@ -702,13 +711,11 @@ template <>
 struct PairOf<__half> {
   using type = __half2;
   static __device__ __forceinline__ float2 floats(__half2 x) { return __half22float2(x); }
-  static __device__ __forceinline__ __half2 round(float2 x) { return __float22half2_rn(x); }
 };
 template <>
 struct PairOf<__nv_bfloat16> {
   using type = __nv_bfloat162;
   static __device__ __forceinline__ float2 floats(__nv_bfloat162 x) { return __bfloat1622float2(x); }
-  static __device__ __forceinline__ __nv_bfloat162 round(float2 x) { return __float22bfloat162_rn(x); }
 };
 template <typename T>
 __device__ __forceinline__ typename PairOf<T>::type as_pair(unsigned u) { return *reinterpret_cast<typename PairOf<T>::type*>(&u); }
@@ -915,7 +922,7 @@ gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* _
     // |v| of each row over this half of chunk ch, for the chain's bound of r and for what it asks of the chunk
     auto sizes_of_v = [&](int ch) {
       const char* stage = smem + (DEEP ? (ch & 1) * STAGE : 0);
-      const float* factors = reinterpret_cast<const float*>(stage + B_AT + 2 * kGdTri) + kGdC2 + 32 * half + 2 * c;
+      const T* weights = reinterpret_cast<const T*>(stage + B_AT + 2 * kGdTri + 4 * kGdWeights) + 32 * half + 2 * c;
       const int n = count - ch * kGdC - 32 * half - 2 * c;
       using P = PairOf<T>;
       typename P::type most[2], least[2], weighed[2];  // of rows g, g + 8
@@ -928,7 +935,7 @@ gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* _
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int t = 16 * jp + 8 * i;
-          const typename P::type f = P::round(*reinterpret_cast<const float2*>(factors + t));
+          const typename P::type f = *reinterpret_cast<const typename P::type*>(weights + t);
           const unsigned behind = (t < n ? 0u : 0x7fffu) | (t + 1 < n ? 0u : 0x7fff0000u);
 #pragma unroll
           for (int r = 0; r < 2; ++r) {

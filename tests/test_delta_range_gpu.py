@@ -112,3 +112,20 @@ def test_every_distance(ops, dtype, mode):
     ref = reference(x, lens, x["state"].cpu().numpy(), 0.125, True)
     o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.125)
     check(o, x["state"], ref, lens, dtype)
+
+
+@pytest.mark.parametrize("size", [10.0, 100.0, 1000.0, 5000.0])
+@pytest.mark.parametrize("odd", [0.0, 1e-4, 1e-7], ids=["zero", "small", "tiny"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(1, 2, 128, 32), (2, 40, 128, 128)])
+def test_keys_far_apart(ops, heads, dtype, odd, size):
+    """Large keys, scaled to unit length by the op, with a few beside them that are zero or next to nothing."""
+    lens = [64, 100, 20]
+    x = make(heads, sum(lens), len(lens), torch.float32, 5)
+    x["k"] *= size
+    x["k"][5::23] *= odd
+    x["q"][3::31] *= odd
+    x = {name: t.to(dtype) if name in "qkvab" else t for name, t in x.items()}
+    ref = reference(x, lens, x["state"].cpu().numpy(), 0.25, True)
+    o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.25)
+    check(o, x["state"], ref, lens, dtype)
