@@ -143,9 +143,37 @@ int launch_loop(const GatedDeltaArgs& p, int dk, int dtype, int most, cudaStream
   return DFSSM_OK;
 }
 
+// What a prompt call launches, from its sizes alone.
+struct GdPlan {
+  bool loop, chunks;  // which kernels
+  int most;           // sequences of up to so many tokens are the loop's,
+  int least;          // of at least so many the chunked kernels'
+  int walkers;        // no more sequences than this can be so long
+};
+GdPlan gd_plan(int tokens, int n_seq) {
+  // The token loop for sequences of few tokens: it takes about 1.1 us a token of the longest one, the chunked kernels
+  // 15 us and more whatever the length up to 64 (64 heads of 64 x 128, one sequence of 12 / 16 tokens: 14.5 / 18.5 us
+  // against 15.1; 64 sequences of 8: 150 us for both launched as below, 241 by chunks).  The lengths are not known here:
+  // where they average less than kGdMixed tokens, both run, each for its sequences (200 sequences of 1 token and 4 of
+  // 500: 297 us, 818 by chunks alone; 255 of 1 and one of 700: 286, by the loop alone 1012; where one of them finds
+  // nothing to do it costs 2 to 12%).  With more sequences than are put in order, the average decides for all of them.
+  const bool many = n_seq > kGdOrdered;
+  if (tokens <= kGdLoopMost || (many && tokens <= 4LL * n_seq)) return {true, false, tokens, 0, 0};
+  if (!many && n_seq > 1 && tokens < (long long)kGdMixed * n_seq) {
+    const int least = kGdLoopMost + 1;
+    return {true, true, kGdLoopMost, least, tokens / least < n_seq ? tokens / least : n_seq};
+  }
+  return {false, true, 0, 1, n_seq};
+}
+
+// Bytes for the chunks' T, P and factors, the fp16 forms of bf16 rows, and the order of the sequences; kGdScratch where the
+// loop takes the whole call and uses none.
+constexpr size_t kGdScratch = 256;
 size_t gd_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dtype) {
-  const size_t n = (size_t)gd_chunk_slots(tokens, n_seq);
-  return n * v_heads * kGdBlock + (dtype == DFSSM_BF16 ? n * k_heads * 2 * kGdC * dk * 2 : 0) + (size_t)n_seq * 16;
+  const GdPlan plan = gd_plan(tokens, n_seq);
+  if (!plan.chunks) return kGdScratch;
+  const size_t n = (size_t)gd_chunk_slots(tokens, n_seq, plan.least);
+  return n * v_heads * kGdBlock + (dtype == DFSSM_BF16 ? n * k_heads * 2 * kGdC * dk * 2 : 0) + (size_t)plan.walkers * 16;
 }
 
 template <typename T, int DK, bool DEEP>
@@ -172,12 +200,13 @@ int launch_walk(const GatedDeltaArgs& p, const char* blocks, const __half* kq16,
   return DFSSM_OK;
 }
 
-// Sequences of at least `least` tokens by the chunked kernels (1: all that have any).
+// Sequences of at least plan.least tokens by the chunked kernels (1: all that have any).
 template <typename T, int DK>
-int launch_chunked(const GatedDeltaArgs& p, char* workspace, int least, cudaStream_t s) {
+int launch_chunked(const GatedDeltaArgs& p, char* workspace, const GdPlan& plan, cudaStream_t s) {
   static SmemLimit limit;
   constexpr int bytes = gd_prep_smem<DK>();
-  const long long n = gd_chunk_slots(p.tokens, p.n_seq);
+  const int least = plan.least, walkers = plan.walkers;
+  const long long n = gd_chunk_slots(p.tokens, p.n_seq, least);
   const int rep = p.v_heads / p.k_heads;
   int dev = 0, sms = 0;
   DFSSM_CU(cudaGetDevice(&dev));
@@ -191,18 +220,16 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, int least, cudaStre
   if (grid > 0x7fffffffLL) return dfssm_fail(DFSSM_ERR_ARG, "%d tokens x %d heads are too many", p.tokens, p.v_heads);
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
-  // No more sequences than this can be so long; in order of falling length they come first.
-  const int walkers = least > 1 && p.tokens / least < p.n_seq ? p.tokens / least : p.n_seq;
   const bool at_once = (long long)walkers * p.v_heads * ((p.dv + 31) / 32) <= sms;  // every block of the walk has an SM
   // The sequences by falling length (a long one that starts last runs alone), with their slots looked up.  It costs
   // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself, as
   // it does where all start at once.
   const bool ordered = walkers < p.n_seq || (!at_once && p.n_seq <= kGdOrdered);
   const size_t all = gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK, std::is_same<T, __half>::value ? DFSSM_F16 : DFSSM_BF16);
-  int4* order = ordered ? reinterpret_cast<int4*>(workspace + all - (size_t)p.n_seq * 16) : nullptr;
+  int4* order = ordered ? reinterpret_cast<int4*>(workspace + all - (size_t)walkers * 16) : nullptr;
   const auto fn = gated_delta_prep_kernel<T, DK>;
   DFSSM_CU(limit.raise(reinterpret_cast<const void*>(fn), bytes));
-  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group, least);
+  fn<<<(unsigned)grid, kPrepThreads, bytes, s>>>(p, workspace, kq16, order, groups, per_group, least, walkers);
   DFSSM_CU(cudaGetLastError());
   return at_once ? launch_walk<T, DK, true>(p, workspace, kq16, order, (int)n, walkers, least, s)
                  : launch_walk<T, DK, false>(p, workspace, kq16, order, (int)n, walkers, least, s);
@@ -271,21 +298,14 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
     return dfssm_fail(DFSSM_ERR_ARG, "the workspace must be %zu bytes, 256-byte aligned", need);
   if (n_seq == 0 || tokens == 0) return DFSSM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // The token loop for sequences of few tokens: it takes about 1.1 us a token of the longest one, the chunked kernels
-  // 15 us and more whatever the length up to 64 (64 heads of 64 x 128, one sequence of 12 / 16 tokens: 14.5 / 18.5 us
-  // against 15.1; 64 sequences of 8: 150 us for both launched as below, 241 by chunks).  The lengths are not known here:
-  // where they average less than kGdMixed tokens, both run, each for its sequences (200 sequences of 1 token and 4 of
-  // 500: 297 us, 818 by chunks alone; 255 of 1 and one of 700: 286, by the loop alone 1012; where one of them finds
-  // nothing to do it costs 2 to 12%).  With more sequences than are put in order, the average decides for all of them.
+  const GdPlan plan = gd_plan(tokens, n_seq);
   char* w = static_cast<char*>(workspace);
-  const bool many = n_seq > kGdOrdered, mixed = !many && n_seq > 1 && tokens < (long long)kGdMixed * n_seq;
-  const int least = mixed ? kGdLoopMost + 1 : 1;
-  if (tokens <= kGdLoopMost || (many && tokens <= 4LL * n_seq)) return launch_loop(p, dk, dtype, tokens, s);
-  if (mixed) {
-    if (const int rc = launch_loop(p, dk, dtype, kGdLoopMost, s)) return rc;
+  if (plan.loop) {
+    if (const int rc = launch_loop(p, dk, dtype, plan.most, s)) return rc;
   }
-  if (dtype == DFSSM_F16) return dk == 128 ? launch_chunked<__half, 128>(p, w, least, s) : launch_chunked<__half, 64>(p, w, least, s);
-  return dk == 128 ? launch_chunked<__nv_bfloat16, 128>(p, w, least, s) : launch_chunked<__nv_bfloat16, 64>(p, w, least, s);
+  if (!plan.chunks) return DFSSM_OK;
+  if (dtype == DFSSM_F16) return dk == 128 ? launch_chunked<__half, 128>(p, w, plan, s) : launch_chunked<__half, 64>(p, w, plan, s);
+  return dk == 128 ? launch_chunked<__nv_bfloat16, 128>(p, w, plan, s) : launch_chunked<__nv_bfloat16, 64>(p, w, plan, s);
 }
 
 }  // extern "C"

@@ -43,11 +43,16 @@ constexpr int kGdFactors = 1280;                   // bytes of them
 constexpr int kGdBlock = 2 * kGdTri + kGdFactors;  // bytes per chunk and value head: T, P, factors
 static_assert(kGdVecs * 4 <= kGdFactors && kGdBlock % 128 == 0, "");
 
-// Chunks are numbered without a plan: sequence i's chunk c is cu[i] / 64 + i + c.  That leaves at most one
-// number per sequence unused and gives no number twice.
-__host__ __device__ inline long long gd_chunk_slots(int tokens, int n_seq) { return (long long)tokens / kGdC + n_seq; }
-__device__ __forceinline__ int gd_chunk_base(const int* cu, int i, int tokens) {
-  return min(max(cu[i], 0), tokens) / kGdC + i;
+// Chunks are numbered without a plan: sequence i's chunk c is cu[i] / 64 + i + c, or, where only sequences of `least` tokens and
+// more have chunks and least > 1, cu[i] / 64 + cu[i] / least + c if that ends lower.  Either leaves at most one number
+// per such sequence unused and gives no number twice: from one sequence's start to the next one's, the first part grows by the
+// whole chunks between and the second by at least 1.
+__host__ __device__ inline bool gd_by_rows(int tokens, int n_seq, int least) { return least > 1 && tokens / least + 1 < n_seq; }
+__host__ __device__ inline long long gd_chunk_slots(int tokens, int n_seq, int least) {
+  return (long long)tokens / kGdC + (gd_by_rows(tokens, n_seq, least) ? tokens / least + 1 : n_seq);
+}
+__device__ __forceinline__ int gd_chunk_base(int first, int i, bool by_rows, int least) {  // of sequence i, from row `first` on
+  return first / kGdC + (by_rows ? first / least : i);
 }
 
 // Fragments of B = M^T (M lower triangular, rows t): n-tile j holds rows 8j..8j+7, k-step kk columns
@@ -251,12 +256,12 @@ constexpr unsigned long long frag_rows() {
 constexpr unsigned long long kFragRow = frag_rows();
 
 // kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.  walks, if not
-// NULL: [n_seq], for the chunk kernel: {first token, tokens, slot or -1, number} of the sequences by falling length.
+// NULL: [walkers], for the chunk kernel: {first token, tokens, slot or -1, number} of the longest sequences by falling length.
 // Sequences of fewer than `least` tokens are not these kernels'.
 template <typename T, int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4)
 gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __half* __restrict__ kq16,
-                        int4* __restrict__ walks, int groups, int per_group, int least) {
+                        int4* __restrict__ walks, int groups, int per_group, int least, int walkers) {
   constexpr bool BF = !std::is_same<T, __half>::value;
   constexpr int UPR = DK / 8;  // 16-byte units per row
   extern __shared__ __align__(128) char smem[];
@@ -290,19 +295,20 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
         place += n > count || (n == count && j < i);
         if (p.slots && j < i && p.slots[j] == slot) mine = false;
       }
-      walks[place] = make_int4(first, count, mine ? slot : -1, i);
+      if (place < walkers) walks[place] = make_int4(first, count, mine ? slot : -1, i);
     }
   }
   // the sequence of chunk `num`: the last one whose first chunk is not behind it
+  const bool by_rows = gd_by_rows(p.tokens, p.n_seq, least);
   int lo = 0, hi = p.n_seq - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (gd_chunk_base(p.cu, mid, p.tokens) <= num) lo = mid;
+    if (gd_chunk_base(min(max(p.cu[mid], 0), p.tokens), mid, by_rows, least) <= num) lo = mid;
     else hi = mid - 1;
   }
   int first, count;
   gd_range(p.cu, lo, p.tokens, first, count);
-  const int cn = num - gd_chunk_base(p.cu, lo, p.tokens);
+  const int cn = num - gd_chunk_base(first, lo, by_rows, least);
   if (cn < 0 || cn * kGdC >= count || count < least) return;
   first += cn * kGdC;
   count = min(count - cn * kGdC, kGdC);
@@ -848,7 +854,7 @@ gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* _
     prep_done();  // no block ends before the kernel ahead has
     return;
   }
-  const int base = first / kGdC + seq;  // gd_chunk_base
+  const int base = gd_chunk_base(first, seq, gd_by_rows(p.tokens, p.n_seq, least), least);
   const int chunks = min((count + kGdC - 1) / kGdC, slots_total - base);
   const int hk = h / (p.v_heads / p.k_heads);
   // Warps 0-3 are the chains', 4-7 the output warps'; w and w + 4 share a scheduler, a chain's B warp (more of u) with an
