@@ -18,9 +18,9 @@ namespace dfssm {
 // Bound: HBM.  A one-token call reads and writes 8 dk dv bytes of state per head and computes 7 dk dv
 // operations, far below the balance of the machine.
 constexpr int kGdWarps = 4;
-// Which prompts take the loop (at the C entry): sequences of up to kGdLoopMost tokens, looked for in calls of less than
-// kGdMixed tokens per sequence and up to kGdOrdered sequences, the most that one prep block puts in order.
-constexpr int kGdLoopMost = 12, kGdMixed = 32, kGdOrdered = 512;
+// Which prompts take the loop (gd_plan): sequences of up to kGdLoopMost tokens, looked for in calls of less than
+// kGdMixed tokens per sequence.
+constexpr int kGdLoopMost = 12, kGdMixed = 32;
 
 // Sequences of more than `most` tokens are left to the chunked kernels.
 template <typename T, int DK, int R>
@@ -156,10 +156,9 @@ GdPlan gd_plan(int tokens, int n_seq) {
   // against 15.1; 64 sequences of 8: 150 us for both launched as below, 241 by chunks).  The lengths are not known here:
   // where they average less than kGdMixed tokens, both run, each for its sequences (200 sequences of 1 token and 4 of
   // 500: 297 us, 818 by chunks alone; 255 of 1 and one of 700: 286, by the loop alone 1012; where one of them finds
-  // nothing to do it costs 2 to 12%).  With more sequences than are put in order, the average decides for all of them.
-  const bool many = n_seq > kGdOrdered;
-  if (tokens <= kGdLoopMost || (many && tokens <= 4LL * n_seq)) return {true, false, tokens, 0, 0};
-  if (!many && n_seq > 1 && tokens < (long long)kGdMixed * n_seq) {
+  // nothing to do it costs 2 to 12%; 599 of 1 and one of 1700: 550, by the loop alone 2444; 600 of 1: 385, 366 by the loop alone).
+  if (tokens <= kGdLoopMost) return {true, false, tokens, 0, 0};
+  if (n_seq > 1 && tokens < (long long)kGdMixed * n_seq) {
     const int least = kGdLoopMost + 1;
     return {true, true, kGdLoopMost, least, tokens / least < n_seq ? tokens / least : n_seq};
   }
@@ -221,9 +220,8 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, const GdPlan& plan,
   __half* kq16 = std::is_same<T, __half>::value ? nullptr
                                                : reinterpret_cast<__half*>(workspace + (size_t)n * p.v_heads * kGdBlock);
   const bool at_once = (long long)walkers * p.v_heads * ((p.dv + 31) / 32) <= sms;  // every block of the walk has an SM
-  // The sequences by falling length (a long one that starts last runs alone), with their slots looked up.  It costs
-  // n_seq^2 comparisons of one prep block; many sequences even out by themselves, and each block looks for itself, as
-  // it does where all start at once.
+  // A list of the sequences, the long ones first (one that starts last runs alone), where there are fewer walkers than
+  // sequences, or where not all start at once; many of them even out by themselves, and each block looks for itself.
   const bool ordered = walkers < p.n_seq || (!at_once && p.n_seq <= kGdOrdered);
   const size_t all = gd_workspace(p.tokens, p.n_seq, p.k_heads, p.v_heads, DK, std::is_same<T, __half>::value ? DFSSM_F16 : DFSSM_BF16);
   int4* order = ordered ? reinterpret_cast<int4*>(workspace + all - (size_t)walkers * 16) : nullptr;

@@ -255,8 +255,62 @@ constexpr unsigned long long frag_rows() {
 }
 constexpr unsigned long long kFragRow = frag_rows();
 
-// kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.  walks, if not
-// NULL: [walkers], for the chunk kernel: {first token, tokens, slot or -1, number} of the longest sequences by falling length.
+// For the chunk kernel, the sequences of `least` tokens and more as {first token, tokens, slot, number}, and entries without
+// tokens up to `walkers`: by falling length and with their slots looked up (-1: takes no part) where there are no more than
+// kGdOrdered of them in as many sequences, else the slot is kGdUnknown and each block of the walk looks; more than kGdOrdered come
+// as they are.  One block does it: a scan over all lengths, and comparisons among the long ones alone, in shared memory (m: 2 kGdOrdered
+// + 4 words).
+constexpr int kGdOrdered = 512, kGdUnknown = -2;
+__device__ __forceinline__ void gd_order(const GatedDeltaArgs& p, int4* walks, int walkers, int least, int* m, int tid) {
+  int *const number = m, *const length = m + kGdOrdered, *const found = m + 2 * kGdOrdered;
+  const int lane = tid & 31, wid = tid >> 5;
+  auto put = [&](int place, int i) {
+    int first, count;
+    gd_range(p.cu, i, p.tokens, first, count);
+    int slot = p.slots ? p.slots[i] : i;
+    if (p.n_seq > kGdOrdered) {
+      slot = kGdUnknown;
+    } else if (p.slots) {
+      bool mine = slot >= 0 && slot < p.n_slots;
+      for (int j = 0; j < i; ++j) mine = mine && p.slots[j] != slot;
+      if (!mine) slot = -1;
+    }
+    if (place < walkers) walks[place] = make_int4(first, count, slot, i);
+  };
+  int total = 0;
+  for (int i0 = 0; i0 < p.n_seq; i0 += kPrepThreads) {
+    int first, count = 0;
+    if (i0 + tid < p.n_seq) gd_range(p.cu, i0 + tid, p.tokens, first, count);
+    const bool in = count >= least;
+    const unsigned all = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) found[wid] = __popc(all);
+    __syncthreads();
+    int place = total + __popc(all & ((1u << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < kPrepThreads / 32; ++w) {
+      if (w < wid) place += found[w];
+      total += found[w];
+    }
+    if (in) {
+      if (place < kGdOrdered) number[place] = i0 + tid, length[place] = count;
+      else put(place, i0 + tid);
+    }
+    __syncthreads();
+  }
+  for (int e = tid; e < min(total, kGdOrdered); e += kPrepThreads) {
+    int place = e;
+    if (total <= kGdOrdered) {
+      place = 0;
+      for (int j = 0; j < total; ++j) place += length[j] > length[e] || (length[j] == length[e] && j < e);
+    }
+    put(place, number[e]);
+  }
+  for (int e = total + tid; e < walkers; e += kPrepThreads) walks[e] = make_int4(0, 0, -1, 0);
+  __syncthreads();
+}
+
+// kq16: for bf16 inputs, the fp16 tiles K and Q [chunk][k_heads][2][64][DK] that the chunk kernel reads.  walks: NULL, or
+// [walkers] entries to write (gd_order).
 // Sequences of fewer than `least` tokens are not these kernels'.
 template <typename T, int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4)
@@ -283,21 +337,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   let_walk_start();
   const int rep = p.v_heads / p.k_heads;
   const int grp = blockIdx.x % groups, hk = (blockIdx.x / groups) % p.k_heads, num = blockIdx.x / (groups * p.k_heads);
-  if (walks && blockIdx.x == 0) {
-    for (int i = tid; i < p.n_seq; i += kPrepThreads) {
-      int first, count, place = 0;
-      gd_range(p.cu, i, p.tokens, first, count);
-      const int slot = p.slots ? p.slots[i] : i;
-      bool mine = slot >= 0 && slot < p.n_slots;
-      for (int j = 0; j < p.n_seq; ++j) {
-        int f, n;
-        gd_range(p.cu, j, p.tokens, f, n);
-        place += n > count || (n == count && j < i);
-        if (p.slots && j < i && p.slots[j] == slot) mine = false;
-      }
-      if (place < walkers) walks[place] = make_int4(first, count, mine ? slot : -1, i);
-    }
-  }
+  if (walks && blockIdx.x == 0) gd_order(p, walks, walkers, least, reinterpret_cast<int*>(smem), tid);
   // the sequence of chunk `num`: the last one whose first chunk is not behind it
   const bool by_rows = gd_by_rows(p.tokens, p.n_seq, least);
   int lo = 0, hi = p.n_seq - 1;
@@ -845,6 +885,7 @@ gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* _
     prep_done();
     const int4 w = walks[nth];
     first = w.x, count = w.y, slot = w.z, seq = w.w;
+    if (slot == kGdUnknown) slot = gd_slot(p.slots, seq, p.n_slots, tid, NT);
   } else {
     seq = nth;
     gd_range(p.cu, seq, p.tokens, first, count);

@@ -58,3 +58,48 @@ def test_nothing_behind_the_workspace(lib, lens, dtype):
     o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.1, workspace=room[:need])
     check(o, x["state"], ref, lens, t)
     assert (room[need:] == 171).all()
+
+
+def test_many_sequences_have_chunks(lib):
+    """However many sequences there are, a long prompt among one-token rows is not left to the token loop: its chunks have a place."""
+    for tokens, n_seq in ((599 + 1700, 600), (2000, 1000), (100000, 30000)):
+        assert lib.dfssm_gated_delta_workspace(tokens, n_seq, 1, 64, 128, 64, 0) >= (tokens // 64) * 64 * 20480
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("named", [False, True], ids=["slots in order", "slots"])
+@pytest.mark.parametrize("lens", [[1] * 599 + [700], [1] * 700 + [0] * 30 + [13] * 9 + [12] * 9 + [300, 65], [1] * 700 + [14] * 600 + [200]],
+                         ids=lambda v: "%d in %d" % (sum(v), len(v)))
+def test_prompts_among_hundreds_of_rows(lens, named, dtype):
+    """More than 512 sequences with long ones among them; 601 long ones in the last case.  Some without a slot, some twice."""
+    import torch
+    from dfssm_b200 import ops
+    from test_gated_delta_gpu import args, check, cu, make, reference
+    heads, t, rng = (1, 2, 64, 32), getattr(torch, dtype), np.random.default_rng(len(lens))
+    lens = rng.permutation(lens)
+    n_seq, n = len(lens), int(lens.sum())
+    x = make(heads, n + 3, n_seq, t, 6)
+    slots, lost = np.arange(n_seq), []
+    if named:
+        slots = rng.permutation(n_seq)
+        longest, one = int(lens.argmax()), int(np.flatnonzero(lens == 1)[-1])
+        slots[one] = -1
+        slots[int(np.flatnonzero(lens == lens[lens > 1].min())[0])] = n_seq
+        if longest:
+            slots[longest - 1 if longest > 1 else 0] = slots[longest]  # of two on one slot the earlier one has it
+        lost = [i for i in range(n_seq) if not 0 <= slots[i] < n_seq or slots[i] in slots[:i]]
+    before, out = x["state"].clone(), torch.full_like(x["v"], 7.0)
+    ops.gated_delta_prefill(*args(x), cu(lens), out=out, scale=0.2,
+                            slots=torch.tensor(slots, dtype=torch.int32, device="cuda") if named else None)
+    rows = np.concatenate([[0], np.cumsum(lens)])
+    assert (out[n:] == 7).all() and all((out[rows[i]:rows[i + 1]] == 7).all() for i in lost)
+    part = [i for i in range(n_seq) if i not in set(lost)]
+    own = torch.tensor(slots[part], device="cuda")
+    at = torch.from_numpy(np.concatenate([np.arange(rows[i], rows[i + 1]) for i in part])).cuda()
+    y = {m: v[at] if m in "qkvab" else v for m, v in x.items()}
+    ref = reference(y, lens[part], before[own].cpu().numpy(), 0.2, True)
+    check(out[at], x["state"][own], ref, lens[part], t)
+    others = torch.ones(n_seq, dtype=torch.bool, device="cuda")
+    others[own] = False
+    assert torch.equal(x["state"][others], before[others])
