@@ -8,10 +8,12 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
+import sysconfig
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int8, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libdfssm.so")
-PYCALLS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "dfssm_pycalls.so")
+PYCALLS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib",
+                            "dfssm_pycalls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 DFSSM_OK = 0
 STATUS = {1: "ERR_ARG", 2: "ERR_FORMAT", 3: "ERR_UNSUPPORTED", 4: "ERR_CUDA", 5: "ERR_OOM", 6: "ERR_STATE",
