@@ -55,12 +55,13 @@ def _vector(t, name: str, n: int, dtype, device):
         _refuse(t, name, f"a contiguous {dtype} vector of {n}", device)
 
 
-def _rows_fit(t) -> bool:
-    """Whether [rows, heads, width] or [rows, heads] has contiguous rows that do not overlap."""
+def _rows_fit(t, most: int) -> bool:
+    """Whether [rows, heads, width] or [rows, heads] has contiguous rows that do not overlap and start at most `most` elements
+    apart."""
     if t.is_contiguous():
         return True
     width = t[0].numel() if t.shape[0] else 0
-    return t[:1].is_contiguous() and (t.shape[0] < 2 or t.stride(0) >= width)
+    return t[:1].is_contiguous() and (t.shape[0] < 2 or width <= t.stride(0) <= most)
 
 
 def _explain(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out):
@@ -79,8 +80,8 @@ def _explain(q, k, v, a, b, A_log, dt_bias, state, n_seq, slots, out):
                            (a, "a", (n, hv)), (b, "b", (n, hv))):
         if t is None and name == "out":
             continue
-        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev or t.shape != shape or not _rows_fit(t):
-            _refuse(t, name, f"{dtype} {shape} with contiguous rows", dev)
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev or t.shape != shape or not _rows_fit(t, 2 ** 31 - 1):
+            _refuse(t, name, f"{dtype} {shape} with contiguous rows, less than 2^31 elements apart", dev)
     _vector(A_log, "A_log", hv, torch.float32, dev)
     _vector(dt_bias, "dt_bias", hv, torch.float32, dev)
     if slots is not None:
@@ -150,12 +151,17 @@ def sample_filtered(logits, uniform, *, temperature=None, top_k=None, top_p=None
         temperature, top_k = of_rows(temperature, torch.float32), of_rows(top_k, torch.int32)
         top_p, min_p = of_rows(top_p, torch.float32), of_rows(min_p, torch.float32)
 
+    try:
+        triple = None if out is None else tuple(out)
+    except TypeError:
+        triple = ()
+
     def explain():
         _on(logits, "logits")
         if logits.dtype not in _DTYPES or logits.dim() != 2 or logits.shape[1] < 1:
             _refuse(logits, "logits", "[rows, vocab] in fp32, fp16 or bf16")
         dev, (B, V) = logits.device, logits.shape
-        if not _rows_fit(logits):
+        if not _rows_fit(logits, 2 ** 63 - 1):
             _refuse(logits, "logits", "contiguous within a row, rows apart")
         _vector(uniform, "uniform", B, torch.float32, dev)
         for t, name, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
@@ -167,10 +173,12 @@ def sample_filtered(logits, uniform, *, temperature=None, top_k=None, top_p=None
                                       or seen_bits.device != dev or seen_bits.shape != (B, words) or not seen_bits.is_contiguous()):
             _refuse(seen_bits, "seen_bits", f"contiguous int32 [{B}, {words}]", dev)
         if out is not None:
-            token, kept, prob = out
+            if len(triple) != 3:
+                raise ValueError("out must be three tensors: tokens, kept counts and probabilities")
+            token, kept, prob = triple
             _vector(token, "out[0]", B, torch.int32, dev)
             _vector(kept, "out[1]", B, torch.int32, dev)
             _vector(prob, "out[2]", B, torch.float32, dev)
 
     return _run("sample_filtered", logits, (logits, uniform, temperature, top_k, top_p, min_p, seen_bits, rep_penalty,
-                                            None if out is None else tuple(out)), explain)
+                                            triple), explain)
