@@ -684,13 +684,13 @@ constexpr int kGdGroups = 2;  // of 16 rows per block
 // With U the bound of |u|, a row is safe where
 //   - at every token, |v| or what the row holds (the state's largest element and the beta |v| so far, each decayed
 //     since) is 2^-22 U or more: u and its part in o are then off by some 2^-17 of that, and
-//   - at the end, the largest beta e^(G_C - G) |v| or of e^G_C S is 2^-17 U times the largest weight or more: what the update adds
-//     is then off by some 2^-21 of it.
+//   - at the end, the largest beta e^(G_C - G) |v| is 2^-17 U times the largest weight or more, or the largest of e^G_C S 2^-14:
+//     what 64 tokens add to the row is off by some 2^-35 U times that weight.
 // The output warps find the least |v| and the largest weighed one; the decays between are looked at only where
-// some |v| is below 2^-22 U and e^G_C S is too, which chance does to one chunk in 1000 or fewer.  Looking costs 1 to 4% of a
-// call (64 prompts of 64 tokens, 64 heads: 245 us, 235 without; 32768 tokens: 1.40 ms, 1.38), looking at the decays 2 us, a chunk
-// token by token 40 us, 2 to 4 otherwise.
-constexpr float kGdRangeO = 0x1p-22f, kGdRangeS = 0x1p-17f;
+// some |v| is below 2^-22 U and e^G_C S is too, which chance does to one chunk in 1000 or fewer.  Looking costs 3 to 6% of a
+// call (64 prompts of 64 tokens, 64 heads: 249 us, 235 without; 32768 tokens: 1.42 ms, 1.38), looking at the decays 2 us, a chunk
+// token by token 40 to 90 us, 2 to 4 otherwise (fetching its next token early: 70 instead of 90, but 2% on every other chunk).
+constexpr float kGdRangeO = 0x1p-22f, kGdRangeV = 0x1p-17f, kGdRangeS = 0x1p-14f;
 constexpr int kGdOfV = 80, kGdByToken = 144;  // places among a group's scales
 
 template <int DK>
@@ -1200,7 +1200,7 @@ gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* _
       const float2 least = PairOf<T>::floats(__hmin2(as_pair<T>(va.y), as_pair<T>(vb.y)));
       const float2 weighed = PairOf<T>::floats(__hmax2(as_pair<T>(va.z), as_pair<T>(vb.z)));
       const float k0 = el * s0, k1 = el * s1, w0 = u0 * kGdRangeO, w1 = u1 * kGdRangeO, wm = vec[kGdWm] * kGdRangeS;
-      const bool weak = (weighed.x < u0 * kGdRangeS && k0 < u0 * wm) || (weighed.y < u1 * kGdRangeS && k1 < u1 * wm);
+      const bool weak = (weighed.x < u0 * kGdRangeV && k0 < u0 * wm) || (weighed.y < u1 * kGdRangeV && k1 < u1 * wm);
       const bool low = (least.x < w0 && k0 < w0) || (least.y < w1 && k1 < w1);
       bool far = __any_sync(0xffffffffu, weak);
       if (!far && __any_sync(0xffffffffu, low))
