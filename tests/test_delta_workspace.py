@@ -27,6 +27,13 @@ def test_workspace_of_long_sequences(lib):
         assert tokens // 64 * 32 * 20480 <= need <= (tokens // 64 + n_seq) * 32 * CHUNK_BYTES + 16 * n_seq
 
 
+def test_a_workspace_for_the_largest_call_is_enough_for_smaller_ones(lib):
+    """More tokens or more sequences never need less."""
+    sizes = [1, 2, 12, 13, 31, 32, 33, 64, 200, 511, 512, 513, 600, 1023, 1024, 2047, 2048, 5000, 16384, 16385]
+    need = [[lib.dfssm_gated_delta_workspace(t, n, 2, 4, 128, 64, 1) for n in sizes] for t in sizes]
+    assert all(a <= b for row in need for a, b in zip(row, row[1:])) and all(a <= b for col in zip(*need) for a, b in zip(col, col[1:]))
+
+
 def test_chunk_numbers_are_distinct():
     """The numbering by rows that the smaller workspace rests on: cu / 64 + cu / 13 + c for sequences of 13 tokens and more."""
     rng = np.random.default_rng(0)
