@@ -157,7 +157,7 @@ __host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + 
 // Three TF32 MMAs for a product of fp32 values: a, b split here.  hi is cut off after 11 bits and lo, exact, rounded to
 // 11 (finite values: adding half of its last place may carry into the exponent, as it should), 2^-23 of the value.
 // By integer instructions: cvt.rna.tf32 runs at a fraction of their rate (64 prompts of 64 tokens, 64 heads:
-// 235 us, 246 with it).
+// 235 us, 246 with it, before the look at how far values lie apart).
 __device__ __forceinline__ void tf32_split2(float v, unsigned& hi, unsigned& lo) {
   hi = __float_as_uint(v) & 0xffffe000u;
   lo = (__float_as_uint(v - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
@@ -672,9 +672,9 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
 // fit on an SM.  DEEP, for grids that give every block an SM of its own, has two of all of them and fetches a chunk ahead.
 //
 // Bound: per chunk and group, at dk = 128, 504 MMAs of 8 cycles (mma.sync runs 1024 multiply-adds per cycle and SM) and
-// about 160 KB through shared memory, in a chain of dependent steps.  Alone on its SM a block takes 2.1 us a chunk
-// (512 chunks of 32 heads, 128 blocks, in 1.08 ms; tensor cores 53% busy; 2.35 us with one chain warp per group); two
-// blocks on an SM take 4.1 us for a chunk each (tensor cores 53%, shared memory 70% busy).
+// about 160 KB through shared memory, in a chain of dependent steps.  Alone on its SM a block takes 2.2 us a chunk
+// (512 chunks of 32 heads, 128 blocks, in 1.12 ms; tensor cores 51% busy; one chain warp per group: 2.35 us where two took
+// 2.1); two blocks on an SM take 4.1 us for a chunk each (tensor cores 51%, shared memory 69% busy).
 
 constexpr int kGdGroups = 2;  // of 16 rows per block
 

@@ -104,7 +104,8 @@ def gated_delta_step(q, k, v, a, b, A_log, dt_bias, state, *, slots=None, scale:
 
 def gated_delta_workspace(tokens: int, n_seq: int, k_heads: int, v_heads: int, dk: int, dv: int,
                           dtype=torch.float16) -> int:
-    """Bytes of scratch that gated_delta_prefill uses for these sizes."""
+    """Bytes of scratch that gated_delta_prefill uses for these sizes; never less for more tokens or sequences, so that a
+    workspace of the largest call's size serves every one."""
     return _lib.load().dfssm_gated_delta_workspace(tokens, n_seq, k_heads, v_heads, dk, dv, _DTYPES[dtype])
 
 

@@ -269,7 +269,9 @@ int dfssm_gated_delta_step(const void* q, int ld_q, const void* k, int ld_k, con
                            int n_slots, const int32_t* slots, int batch, void* o, int ld_o, int k_heads, int v_heads,
                            int dk, int dv, float scale, int qk_norm, int dtype, void* stream);
 
-/* Scratch bytes dfssm_gated_delta_prefill needs (it may be 0). */
+/* Scratch bytes dfssm_gated_delta_prefill needs (it may be 0).  More tokens, or more sequences, never need less, so that
+ * one workspace of the largest call's size serves all.  Sequences of up to 12 tokens add nothing to it in calls that
+ * average less than 32 tokens per sequence. */
 size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_heads, int dk, int dv, int dtype);
 /* The same recurrence over ragged prompts: sequence i owns the token rows [cu_seqlens[i],
  * cu_seqlens[i + 1]) of q, k, v, a, b and o (`tokens` rows in all), starts from the state in its slot and
@@ -279,7 +281,10 @@ size_t dfssm_gated_delta_workspace(int tokens, int n_seq, int k_heads, int v_hea
  * memory of dfssm_gated_delta_workspace bytes, 256-byte aligned, used by this call alone until it has run:
  * calls that may overlap (other streams, graphs replayed at once) need one each.  Neither call allocates or
  * synchronises, and both can be captured into a graph.  A NaN or infinite q, k or v, or a NaN a or b, spoils the rows
- * of o and the state of its own sequence, from the start of its 64 tokens on, and nothing else. */
+ * of o and the state of its own sequence, from the start of its 64 tokens on, and nothing else.  Errors are those of
+ * fp32 sums, relative to the largest element that a row of the state has or, but for the decays since, had: what a gate
+ * has forgotten costs the tokens after it no bits, nor do large values the tokens before them.  With qk_norm, q and k
+ * whose squares overflow fp32 (elements above some 1e18, in bf16) count as zero, here and in dfssm_gated_delta_step. */
 int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, const void* v, int ld_v, const void* a,
                               int ld_a, const void* b, int ld_b, const float* A_log, const float* dt_bias,
                               float* state, int n_slots, const int32_t* slots, const int32_t* cu_seqlens, int n_seq,
