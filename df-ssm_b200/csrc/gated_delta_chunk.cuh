@@ -36,10 +36,10 @@ constexpr int kGdTri = kGdFrags * 512;  // bytes of one such matrix as fp16 hi/l
 // and the inverse scale of P's row; then e^G_C, the inverse scale of T, the largest absolute row sum of T, the
 // update's scale, the largest norm of a key, and the largest weight a u could have in the update: the largest
 // beta e^(G_C - G) / |k| times the largest norm of a key as it is staged.  Last, in the inputs' type, each token's own weight
-// beta e^(G_C - G) relative to that (to within 1/4: by powers of two).
+// beta e^(G_C - G) |k| relative to that (to within 1/4: by powers of two), and the norm of its key as the products see it.
 enum { kGdBk = 0, kGdC2 = 64, kGdOq = 128, kGdOp = 192, kGdLast = 256, kGdTdn, kGdTsum, kGdCdn, kGdKn, kGdWm, kGdWeights = 264,
-       kGdVecs = kGdWeights + 32 };
-constexpr int kGdFactors = 1280;                   // bytes of them
+       kGdNorms = kGdWeights + 32, kGdVecs = kGdNorms + 32 };
+constexpr int kGdFactors = 1408;                   // bytes of them
 constexpr int kGdBlock = 2 * kGdTri + kGdFactors;  // bytes per chunk and value head: T, P, factors
 static_assert(kGdVecs * 4 <= kGdFactors && kGdBlock % 128 == 0, "");
 
@@ -152,7 +152,7 @@ __host__ __device__ constexpr int gd_prep_tiles() {  // K and Q; once they are m
   return 2 * kGdC * DK * 2 > kGdC * kLS * 4 ? 2 * kGdC * DK * 2 : kGdC * kLS * 4;
 }
 template <int DK>
-__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 10 + 64; }
+__host__ __device__ constexpr int gd_prep_smem() { return gd_prep_tiles<DK>() + kGdC * kLS * 4 + 64 * 8 + 64 * 4 * 11 + 64; }
 
 // Three TF32 MMAs for a product of fp32 values: a, b split here.  hi is cut off after 11 bits and lo, exact, rounded to
 // 11 (finite values: adding half of its last place may carry into the exponent, as it should), 2^-23 of the value.
@@ -332,7 +332,8 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
   float* rowd = colf + 192;  // e^(G_t - last of t's block), where that is at most e^kMild
   float* cold = rowd + 64;   // e^(last of w's block - G_w) rk_w beta_w
   float* kst = cold + 64;    // norms of K's rows as staged
-  float* red = kst + 64;     // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors, [2] norms as staged
+  float* knm = kst + 64;     // and as the products see them
+  float* red = knm + 64;     // [4] max T, [4] row sums, [2] norms of keys, [2] max of the update's factors, [2] norms as staged
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, c = lane & 3;
   let_walk_start();
   const int rep = p.v_heads / p.k_heads;
@@ -382,8 +383,9 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
     }
     ss += s1;
     float factor = p.qk_norm ? 1.0f / sqrtf(ss + kQkEps) : 1.0f;
-    float kn = p.qk_norm ? 1.0f : sqrtf(ss);  // the norm that the products see
-    staged = sqrtf(ss);                       // and that of the row in shared memory
+    staged = sqrtf(ss);                       // the norm of the row in shared memory
+    float kn = p.qk_norm ? 1.0f : staged;     // a bound of those that the products see
+    const float seen = p.qk_norm ? fminf(staged * factor, 1.0f) : staged;
     if constexpr (BF) {
       float up, down;
       row_scale(mx, up, down);
@@ -404,6 +406,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
     if (tid < 64) {
       rk[t] = staged > 0.f ? factor : 0.f;  // a key of zeros adds nothing: its 1 / |k| is not to set the update's scale
       kst[t] = staged;
+      knm[t] = seen;
       kn = warp_max(kn);
       staged = warp_max(staged);
       if (lane == 0) red[8 + wid] = kn, red[12 + wid] = staged;
@@ -500,6 +503,7 @@ gated_delta_prep_kernel(const GatedDeltaArgs p, char* __restrict__ blocks, __hal
         float kup, kdown;
         row_scale(kmax, kup, kdown);
         reinterpret_cast<T*>(vec + kGdWeights)[t] = from_f<T>((colf[128 + t] * (up * 0x1p-14f)) * (kst[t] * (kup * 0x1p-14f)));
+        reinterpret_cast<T*>(vec + kGdNorms)[t] = from_f<T>(knm[t]);
         if (t == 0) vec[kGdCdn] = down * 0x1p14f, vec[kGdWm] = c2max * kmax;
         if (t < 48) colf[128 + t] = expf((float)(G[47] - Gt)) * fk[t];
       }
@@ -682,14 +686,16 @@ constexpr int kGdGroups = 2;  // of 16 rows per block
 // u, and it may be all that matters, where a gate has forgotten the large values (of the chunk, or of the state before it)
 // or where they come later.  Such a chunk is taken token by token in fp32 by the group's chain warps (gd_by_token).
 // With U the bound of |u|, a row is safe where
-//   - at every token, |v| or what the row holds (the state's largest element and the beta |v| so far, each decayed
-//     since) is 2^-22 U or more: u and its part in o are then off by some 2^-17 of that, and
+//   - at every token, what the row holds (the largest of the state's elements and of beta |v| |k| so far, each decayed
+//     since) is 2^-22 U times the largest weight, beta |k| decayed alike, that a token has in o, which is the scale of P's
+//     row, or more: o is then off by some 2^-17 of what it could be; and
 //   - at the end, the largest beta e^(G_C - G) |v| is 2^-17 U times the largest weight or more, or the largest of e^G_C S 2^-14:
 //     what 64 tokens add to the row is off by some 2^-35 U times that weight.
-// The output warps find the least |v| and the largest weighed one; the decays between are looked at only where
-// some |v| is below 2^-22 U and e^G_C S is too, which chance does to one chunk in 1000 or fewer.  Looking costs 3 to 6% of a
-// call (64 prompts of 64 tokens, 64 heads: 249 us, 235 without; 32768 tokens: 1.42 ms, 1.38), looking at the decays 2 us, a chunk
-// token by token 40 to 90 us, 2 to 4 otherwise (fetching its next token early: 70 instead of 90, but 2% on every other chunk).
+// The output warps find the least |v| and the largest weighed one; the decays between are looked at only where some |v| is
+// below 2^-22 U (else what is held cannot be either) and e^G_C S is too, which chance does to one chunk in 1000 or fewer.
+// Looking costs 4 to 7% of a call (64 prompts of 64 tokens, 64 heads: 253 us, 235 without; 32768 tokens: 1.43 ms, 1.38), looking at
+// the decays 2 us, a chunk token by token 40 to 90 us, 2 to 4 otherwise (fetching its next token early: 70 instead of 90, but 2%
+// on every other chunk).
 constexpr float kGdRangeO = 0x1p-22f, kGdRangeV = 0x1p-17f, kGdRangeS = 0x1p-14f;
 constexpr int kGdOfV = 80, kGdByToken = 144;  // places among a group's scales
 
@@ -768,27 +774,28 @@ __device__ __forceinline__ typename PairOf<T>::type as_pair(unsigned u) { return
 template <typename P>
 __device__ __forceinline__ unsigned pair_bits(P x) { return *reinterpret_cast<unsigned*>(&x); }
 
-// Whether one of a group's rows comes to a token where it holds less than w0 (rows g; w1: rows g + 8), and something.  m0, m1: the
-// largest of the rows' state; v: the chunk's tile.
+// Whether one of a group's rows comes to a token where it holds something, but less than w0 (rows g; w1: rows g + 8) times the
+// largest weight.  m0, m1: the largest of the rows' state; v: the chunk's tile; norms: of its keys.
 template <typename T>
-__device__ __forceinline__ bool gd_forgets(const GatedDeltaArgs& p, const char* v, int group, int first, int n, int h, float m0,
+__device__ __forceinline__ bool gd_forgets(const GatedDeltaArgs& p, const char* v, const T* norms, int group, int first, int n, int h, float m0,
                                            float m1, float w0, float w1) {
   const int lane = threadIdx.x & 31, g = lane >> 2;
+  float weight = 0.f;
   bool bad = false;
 #pragma unroll 1
   for (int t0 = 0; t0 < n; t0 += 32) {
     const size_t at = (size_t)first + min(t0 + lane, n - 1);  // the gates of 32 tokens, one per lane
     float keep = expf(gd_log_decay(to_f(static_cast<const T*>(p.a)[at * p.ld_a + h]), p.dt_bias[h], p.A_log[h]));
     float beta = gd_beta(to_f(static_cast<const T*>(p.b)[at * p.ld_b + h]));
+    beta *= to_f(norms[t0 + lane]);
     if (t0 + lane >= n) keep = 1.f, beta = 0.f;
 #pragma unroll 4
     for (int i = 0; i < 32; ++i) {
       const float e = __shfl_sync(0xffffffffu, keep, i), b = __shfl_sync(0xffffffffu, beta, i);
       const float x = fabsf(to_f(reinterpret_cast<const T*>(v + v_off(t0 + i, 2 * group))[g]));  // 0 behind the last token
       const float y = fabsf(to_f(reinterpret_cast<const T*>(v + v_off(t0 + i, 2 * group + 1))[g]));
-      m0 = fmaxf(e * m0, b * x), m1 = fmaxf(e * m1, b * y);
-      const float x0 = fmaxf(m0, x), x1 = fmaxf(m1, y);
-      bad |= (x0 < w0 && x0 != 0.f) || (x1 < w1 && x1 != 0.f);
+      m0 = fmaxf(e * m0, b * x), m1 = fmaxf(e * m1, b * y), weight = fmaxf(e * weight, b);
+      bad |= (m0 < w0 * weight && m0 != 0.f) || (m1 < w1 * weight && m1 != 0.f);
     }
   }
   return __any_sync(0xffffffffu, bad);
@@ -1199,12 +1206,12 @@ gated_delta_chunk_kernel(const __grid_constant__ GatedDeltaArgs p, const char* _
     {  // both warps come to the same answers: they look at the same numbers
       const float2 least = PairOf<T>::floats(__hmin2(as_pair<T>(va.y), as_pair<T>(vb.y)));
       const float2 weighed = PairOf<T>::floats(__hmax2(as_pair<T>(va.z), as_pair<T>(vb.z)));
-      const float k0 = el * s0, k1 = el * s1, w0 = u0 * kGdRangeO, w1 = u1 * kGdRangeO, wm = vec[kGdWm] * kGdRangeS;
+      const float k0 = el * s0, k1 = el * s1, w0 = u0 * kGdRangeO, w1 = u1 * kGdRangeO, kn = fmaxf(vec[kGdKn], 1.f), wm = vec[kGdWm] * kGdRangeS;
       const bool weak = (weighed.x < u0 * kGdRangeV && k0 < u0 * wm) || (weighed.y < u1 * kGdRangeV && k1 < u1 * wm);
-      const bool low = (least.x < w0 && k0 < w0) || (least.y < w1 && k1 < w1);
+      const bool low = (least.x < w0 && k0 < w0 * kn) || (least.y < w1 && k1 < w1 * kn);
       bool far = __any_sync(0xffffffffu, weak);
       if (!far && __any_sync(0xffffffffu, low))
-        far = gd_forgets<T>(p, st + V_AT, group, first + ch * kGdC, min(count - ch * kGdC, kGdC), h, s0, s1, w0, w1);
+        far = gd_forgets<T>(p, st + V_AT, reinterpret_cast<const T*>(vec + kGdNorms), group, first + ch * kGdC, min(count - ch * kGdC, kGdC), h, s0, s1, w0, w1);
       if (far && active) {
         if (half == 0 && lane == 0) sc[kGdByToken] = 1.f;
         bar_arrive(bar + 3, 128);  // the output warps need not wait: they leave this chunk's o alone

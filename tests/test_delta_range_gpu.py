@@ -129,3 +129,39 @@ def test_keys_far_apart(ops, heads, dtype, odd, size):
     ref = reference(x, lens, x["state"].cpu().numpy(), 0.25, True)
     o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.25)
     check(o, x["state"], ref, lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(1, 2, 128, 32), (2, 40, 128, 128)])
+def test_small_betas_after_a_gate(ops, heads, dtype):
+    """A gate that forgets everything, tokens of value 0, then one whose beta is next to nothing: its part is all that o has."""
+    lens = [64, 90]
+    x = make(heads, sum(lens), len(lens), dtype, 9)
+    x["a"][:] = -8.0
+    for at in (0, 64):
+        x["a"][at + 20] = FORGET
+        x["v"][at + 20:at + 26] = 0
+        x["b"][at + 26:at + 30] = -12.0 if dtype is torch.float16 else -30.0
+        x["v"][at + 5] *= 100
+    ref = reference(x, lens, x["state"].cpu().numpy(), 0.25, True)
+    o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.25)
+    check(o, x["state"], ref, lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("norm", [True, False])
+def test_keys_that_hold_nothing(ops, norm, dtype):
+    """A gate leaves e^-25 of the state; its token's key is zero, or next to it, so that the state does not hold its value, and the
+    values after it are zero: what is left of the old state is all there is."""
+    heads, lens = (1, 4, 128, 32), [64, 90]
+    x = make(heads, sum(lens), len(lens), dtype, 13, norm)
+    x["A_log"].zero_()
+    x["dt_bias"].fill_(-4.0)
+    x["a"][:] = -8.0
+    for at in (0, 64):
+        x["a"][at + 20] = 29.0
+        x["k"][at + 20] *= 0 if norm else 2.0 ** -14
+        x["v"][at + 21:at + 40] = 0
+    ref = reference(x, lens, x["state"].cpu().numpy(), 0.25, norm)
+    o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.25, qk_norm=norm)
+    check(o, x["state"], ref, lens, dtype)
