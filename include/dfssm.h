@@ -302,11 +302,12 @@ int dfssm_gated_delta_prefill(const void* q, int ld_q, const void* k, int ld_k, 
  *   next   the first kept token in vocabulary order whose running weight exceeds uniform[b] x the kept
  *          weight (uniform is taken into [0, 1)).
  * temperature <= 0 takes the first token of the order.  NaN and -inf logits never stay; a row that holds
- * nothing else gets next = -1, kept_count 0 and prob 0.  temperature, top_p, min_p fp32 [batch] and top_k
+ * nothing else gets next = -1, kept_count 0 and prob 0.  In a row with x of +inf these alone stay, with equal weights.  temperature, top_p, min_p fp32 [batch] and top_k
  * int32 [batch] (device) may each be NULL: 1, all, 0, all.  seen_bits as in dfssm_sample but not written, or NULL.
  * Outputs: next int32 [batch]; kept_count int32 [batch] and prob fp32 [batch] (the token's share of the kept
- * weight), either may be NULL.  Weights are summed as 64-bit integers, so the choice does not depend on the
- * order of any sum.  vocab up to 2^24. */
+ * weight), either may be NULL.  Weights are summed as 64-bit integers, in units of 2^-50 of the largest (2^-46 at
+ * 50,000 tokens, 2^-38 at 2^24), so the choice does not depend on the order of any sum; a token whose weight is less
+ * than half a unit may stay, and counts, but is never drawn.  vocab up to 2^24. */
 int dfssm_sample_filtered(const void* logits, int64_t ld, int dtype, int batch, int vocab, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, const uint32_t* seen_bits,
                           float rep_penalty, const float* uniform, int32_t* next, int32_t* kept_count, float* prob,
