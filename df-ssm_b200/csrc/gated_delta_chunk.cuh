@@ -694,8 +694,7 @@ constexpr int kGdGroups = 2;  // of 16 rows per block
 // The output warps find the least |v| and the largest weighed one; the decays between are looked at only where some |v| is
 // below 2^-22 U (else what is held cannot be either) and e^G_C S is too, which chance does to one chunk in 1000 or fewer.
 // Looking costs 4 to 7% of a call (64 prompts of 64 tokens, 64 heads: 253 us, 235 without; 32768 tokens: 1.43 ms, 1.38), looking at
-// the decays 2 us, a chunk token by token 40 to 90 us, 2 to 4 otherwise (fetching its next token early: 70 instead of 90, but 2%
-// on every other chunk).
+// the decays 2 us, a chunk token by token 25 us, 2 to 4 otherwise.
 constexpr float kGdRangeO = 0x1p-22f, kGdRangeV = 0x1p-17f, kGdRangeS = 0x1p-14f;
 constexpr int kGdOfV = 80, kGdByToken = 144;  // places among a group's scales
 
@@ -802,47 +801,56 @@ __device__ __forceinline__ bool gd_forgets(const GatedDeltaArgs& p, const char* 
 }
 
 // The n tokens of a chunk one after the other, from the call's own arrays, for chunks whose values lie too far apart for
-// pairs.  s: the state as the chain warps hold it, s[j] the rows `row` and row + 8, columns half * DK / 2 + 8 j + 2 (lane % 4) +
-// {0, 1}; the rows' sums pass between the two warps through ex.
+// pairs; first the gates, norms and k.q of all of them, a lane each (25 us a chunk; 85 with these in the tokens' turns).  s: the
+// state as the chain warps hold it, s[j] the rows `row` and row + 8, columns half * DK / 2 + 8 j + 2 (lane % 4) +
+// {0, 1}; the rows' sums pass between the two warps through ex (112 float4).
 template <typename T, int DK>
 __device__ __noinline__ void gd_by_token(const GatedDeltaArgs& p, float (&s)[DK / 16][4], int first, int n, int h, int hk, int row,
                                          int half, int bar, float4* ex) {
   constexpr int NH = DK / 16;
   using T2 = typename PairOf<T>::type;
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const float A_log = p.A_log[h], dt_bias = p.dt_bias[h];
+  float4* const gates = ex + 32;                            // per token: e^g, beta and the factors of k and q
+  float* const kqs = reinterpret_cast<float*>(ex + 96);     // and k.q
+  if (const int t = 32 * half + lane; t < n) {  // a lane per token
+    const size_t at = (size_t)first + t;
+    const uint4* kp = reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + at * p.ld_k + hk * DK);
+    const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at * p.ld_q + hk * DK);
+    float kk[2] = {}, qq[2] = {}, kq[2] = {};
+#pragma unroll 4
+    for (int u = 0; u < DK / 8; ++u) {
+      const uint4 x = kp[u], y = qp[u];
+      const T *e = reinterpret_cast<const T*>(&x), *f = reinterpret_cast<const T*>(&y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float k = to_f(e[j]), q = to_f(f[j]);
+        kk[j & 1] = fmaf(k, k, kk[j & 1]), qq[j & 1] = fmaf(q, q, qq[j & 1]), kq[j & 1] = fmaf(k, q, kq[j & 1]);
+      }
+    }
+    const float rk = p.qk_norm ? 1.0f / sqrtf(kk[0] + kk[1] + kQkEps) : 1.0f, rq = p.qk_norm ? 1.0f / sqrtf(qq[0] + qq[1] + kQkEps) : 1.0f;
+    gates[t] = make_float4(expf(gd_log_decay(to_f(static_cast<const T*>(p.a)[at * p.ld_a + h]), p.dt_bias[h], p.A_log[h])),
+                           gd_beta(to_f(static_cast<const T*>(p.b)[at * p.ld_b + h])), rk, rq);
+    kqs[t] = (kq[0] + kq[1]) * (rk * rq);
+  }
+  bar_sync(bar, 64);
   auto quad_sum = [](float v) {
     v += __shfl_xor_sync(0xffffffffu, v, 1);
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
   };
+  const T* kp = static_cast<const T*>(p.k) + (size_t)first * p.ld_k + hk * DK + half * (DK / 2) + 2 * c;
+  const T* qp = static_cast<const T*>(p.q) + (size_t)first * p.ld_q + hk * DK + half * (DK / 2) + 2 * c;
+  const T* vp = static_cast<const T*>(p.v) + (size_t)first * p.ld_v + h * p.dv + row;
+  T* op = static_cast<T*>(p.o) + (size_t)first * p.ld_o + h * p.dv + row;
 #pragma unroll 1
-  for (int t = 0; t < n; ++t) {
-    const size_t at = (size_t)first + t;
-    const T* kp = static_cast<const T*>(p.k) + at * p.ld_k + hk * DK + 2 * c;
-    const T* qp = static_cast<const T*>(p.q) + at * p.ld_q + hk * DK + 2 * c;
-    const T* vp = static_cast<const T*>(p.v) + at * p.ld_v + h * p.dv + row;
+  for (int t = 0; t < n; ++t, kp += p.ld_k, qp += p.ld_q, vp += p.ld_v, op += p.ld_o) {
     const float v0 = to_f(vp[0]), v1 = to_f(vp[8]);
-    const float eg = expf(gd_log_decay(to_f(static_cast<const T*>(p.a)[at * p.ld_a + h]), dt_bias, A_log));
-    const float beta = gd_beta(to_f(static_cast<const T*>(p.b)[at * p.ld_b + h]));
-    float k[NH][2], q[NH][2], kk = 0.f, qq = 0.f, kq = 0.f;
+    const float4 gate = gates[t];
+    const float eg = gate.x, beta = gate.y, kq = kqs[t];
+    float k[NH][2], q[NH][2];
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {  // the other warp's columns first, for the norms alone
-#pragma unroll
-      for (int j = 0; j < NH; ++j) {
-        const int col = (part ? half : 1 - half) * (DK / 2) + 8 * j;
-        const T2 x = *reinterpret_cast<const T2*>(kp + col), y = *reinterpret_cast<const T2*>(qp + col);
-        k[j][0] = to_f(x.x), k[j][1] = to_f(x.y), q[j][0] = to_f(y.x), q[j][1] = to_f(y.y);
-        kk = fmaf(k[j][0], k[j][0], fmaf(k[j][1], k[j][1], kk));
-        qq = fmaf(q[j][0], q[j][0], fmaf(q[j][1], q[j][1], qq));
-        kq = fmaf(k[j][0], q[j][0], fmaf(k[j][1], q[j][1], kq));
-      }
-    }
-    kq = quad_sum(kq);
-    if (p.qk_norm) {
-      const float rk = 1.0f / sqrtf(quad_sum(kk) + kQkEps), rq = 1.0f / sqrtf(quad_sum(qq) + kQkEps);
-#pragma unroll
-      for (int j = 0; j < NH; ++j) k[j][0] *= rk, k[j][1] *= rk, q[j][0] *= rq, q[j][1] *= rq;
-      kq *= rk * rq;
+    for (int j = 0; j < NH; ++j) {
+      const T2 x = *reinterpret_cast<const T2*>(kp + 8 * j), y = *reinterpret_cast<const T2*>(qp + 8 * j);
+      k[j][0] = to_f(x.x) * gate.z, k[j][1] = to_f(x.y) * gate.z, q[j][0] = to_f(y.x) * gate.w, q[j][1] = to_f(y.y) * gate.w;
     }
     float4 sums = make_float4(0.f, 0.f, 0.f, 0.f);  // S k of the two rows, S q
 #pragma unroll
@@ -859,7 +867,6 @@ __device__ __noinline__ void gd_by_token(const GatedDeltaArgs& p, float (&s)[DK 
     const float4 other = mail[8 * (1 - half) + g];
     const float u0 = beta * (v0 - eg * (sums.x + other.x)), u1 = beta * (v1 - eg * (sums.y + other.y));
     if (half == 0 && c == 0) {
-      T* op = static_cast<T*>(p.o) + at * p.ld_o + h * p.dv + row;
       op[0] = from_f<T>(p.scale * fmaf(kq, u0, eg * (sums.z + other.z)));
       op[8] = from_f<T>(p.scale * fmaf(kq, u1, eg * (sums.w + other.w)));
     }
