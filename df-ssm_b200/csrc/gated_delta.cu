@@ -83,7 +83,7 @@ gated_delta_loop_kernel(const GatedDeltaArgs p, int row_blocks, int most) {
         q[j] *= rq;
         k[j] *= rk;
       }
-      kq *= rq * rk;
+      kq = unit_dot(kq, rq * rk);
     }
     // sums[0..7] = S k of the rows, sums[8..15] = S q
     float sums[2 * R];

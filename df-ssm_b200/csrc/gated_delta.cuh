@@ -52,6 +52,9 @@ __device__ __forceinline__ float gd_log_decay(float a, float dt_bias, float A_lo
   const float g = -expf(A_log) * (x > 20.f ? x : log1pf(expf(x)));
   return g < -256.f ? -256.f : g;
 }
+// k.q of unit vectors from that of the raw ones and the product of their factors.  A factor is 0 where a square overflowed: the
+// vector counts as zero, although the raw product may be infinite.
+__device__ __forceinline__ float unit_dot(float kq, float factors) { return factors == 0.f ? 0.f : kq * factors; }
 __device__ __forceinline__ float gd_beta(float b) { return 1.0f / (1.0f + expf(-b)); }
 
 // Tokens [first, first + count) of sequence i, clamped to the rows that exist whatever cu holds.

@@ -830,7 +830,7 @@ __device__ __noinline__ void gd_by_token(const GatedDeltaArgs& p, float (&s)[DK 
     const float rk = p.qk_norm ? 1.0f / sqrtf(kk[0] + kk[1] + kQkEps) : 1.0f, rq = p.qk_norm ? 1.0f / sqrtf(qq[0] + qq[1] + kQkEps) : 1.0f;
     gates[t] = make_float4(expf(gd_log_decay(to_f(static_cast<const T*>(p.a)[at * p.ld_a + h]), p.dt_bias[h], p.A_log[h])),
                            gd_beta(to_f(static_cast<const T*>(p.b)[at * p.ld_b + h])), rk, rq);
-    kqs[t] = (kq[0] + kq[1]) * (rk * rq);
+    kqs[t] = unit_dot(kq[0] + kq[1], rk * rq);
   }
   bar_sync(bar, 64);
   auto quad_sum = [](float v) {

@@ -165,3 +165,17 @@ def test_keys_that_hold_nothing(ops, norm, dtype):
     ref = reference(x, lens, x["state"].cpu().numpy(), 0.25, norm)
     o = ops.gated_delta_prefill(*args(x), cu(lens), scale=0.25, qk_norm=norm)
     check(o, x["state"], ref, lens, dtype)
+
+
+@pytest.mark.parametrize("lens", [[5], [64, 70], [1, 1, 1]], ids=["loop", "chunks", "steps"])
+def test_keys_and_queries_past_fp32s_squares(ops, lens):
+    """bf16 keys and queries whose squares overflow fp32 count as zero where they are scaled to unit length, also where both do."""
+    heads, dtype = (1, 2, 128, 32), torch.bfloat16
+    x = make(heads, sum(lens), len(lens), dtype, 3)
+    y = {n: t.clone() for n, t in x.items()}
+    for name, at in (("k", slice(0, None, 3)), ("q", slice(0, None, 2))):
+        x[name][at] = 3e25 * torch.sign(x[name][at] - 0.1)
+        y[name][at] = 0
+    run = (lambda z: ops.gated_delta_step(*args(z))) if len(lens) == 3 else (lambda z: ops.gated_delta_prefill(*args(z), cu(lens)))
+    got, want = run(x), run(y)
+    assert torch.isfinite(want).all() and torch.equal(got, want) and torch.equal(x["state"], y["state"])
