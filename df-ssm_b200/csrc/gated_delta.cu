@@ -212,7 +212,7 @@ int launch_chunked(const GatedDeltaArgs& p, char* workspace, const GdPlan& plan,
   DFSSM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   // Heads of one key per prep block: the more, the less is computed twice, as long as there are blocks for every SM
   // (64 heads on one key, 64 prompts of 64 tokens, whole call: 253 us with 2, 242 with 4, 235 with 8, 235 with 16, before
-  // the look at how far values lie apart, which adds 15).
+  // the look at how far values lie apart, which adds 20).
   int per_group = rep < 8 ? rep : 8;
   while (per_group > 1 && n * p.k_heads * ((rep + per_group - 1) / per_group) < 4 * sms) per_group /= 2;
   const int groups = (rep + per_group - 1) / per_group;

@@ -693,7 +693,7 @@ constexpr int kGdGroups = 2;  // of 16 rows per block
 //     what 64 tokens add to the row is off by some 2^-35 U times that weight.
 // The output warps find the least |v| and the largest weighed one; the decays between are looked at only where some |v| is
 // below 2^-22 U (else what is held cannot be either) and e^G_C S is too, which chance does to one chunk in 1000 or fewer.
-// Looking costs 4 to 7% of a call (64 prompts of 64 tokens, 64 heads: 253 us, 235 without; 32768 tokens: 1.43 ms, 1.38), looking at
+// Looking costs 4 to 8% of a call (64 prompts of 64 tokens, 64 heads: 255 us, 235 without; 32768 tokens: 1.44 ms, 1.38), looking at
 // the decays 2 us, a chunk token by token 25 us, 2 to 4 otherwise.
 constexpr float kGdRangeO = 0x1p-22f, kGdRangeV = 0x1p-17f, kGdRangeS = 0x1p-14f;
 constexpr int kGdOfV = 80, kGdByToken = 144;  // places among a group's scales
